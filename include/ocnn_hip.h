@@ -630,6 +630,83 @@ int ocnn_octree_update(void* octree_dev, void* info, const int* label, int n_lab
 int ocnn_octree_update_copy(void* out_dev, const void* in_dev, void* info, const int* label, int n_label,
     int depth, int split, void* scratch_dev, size_t scratch_bytes, ocnn_stream_t stream);
 
+/* ---- operators along the node order of an octree level; no counterpart in the reference, whose feature
+ * operators mix a node with its 27 neighbours only.  A level of a batched octree is one sequence per
+ * octree: its nodes in Morton order, octree after octree (octree/octree/merge_octrees.cpp:114-198).
+ * Tensors are row-major, a row a node, with strides in elements (the innermost one is 1): [rows, heads,
+ * dim] or [rows, channels].  `offsets` (device, int32 [n_seq + 1], offsets[0] = 0, not decreasing)
+ * says where each sequence begins; rows behind the last sequence belong to none: they are left as
+ * they are, or set to zero with fill_rest != 0 (gradients: always zero).  Offsets are clamped to the
+ * rows that exist.  These calls launch kernels only and can be captured in a HIP graph.
+ *
+ * ocnn_octree_offsets: those offsets (batch_size + 1) for the nodes (nempty: the non-empty nodes) of a
+ * level, from its keys. */
+int ocnn_octree_offsets(int* offsets, const void* octree_dev, const void* info, int depth, int nempty,
+    ocnn_stream_t stream);
+
+/* Rotary positions with several axes.  pairs[i] (host) pairs of channels belong to axis i (the first
+ * pairs[0] to axis 0, the next pairs[1] to axis 1, ...); P pairs in all, 2 P <= dim; channels from 2 P on
+ * are copied.  Pair p is channels (p, P + p), interleaved != 0: (2 p, 2 p + 1); it turns by
+ * position[axis] * frequencies[p] (radians a unit; device, fp64 [P]), inverse != 0 by the negative: the
+ * gradient.  The angle is formed in 64 bits.  positions: OCNN_POS_INT32 / OCNN_POS_F32 [rows, axes]
+ * with rows `position_row` elements apart, at most 4 axes; OCNN_POS_XYZ: the packed coordinates of the
+ * nodes (64-bit, 16 bits an axis, at most 3 axes), what octree_property "xyz" returns.
+ * `out` may be `data` with the same strides; otherwise they must not overlap. */
+enum { OCNN_POS_INT32 = 0, OCNN_POS_F32 = 1, OCNN_POS_XYZ = 2 };
+int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void* data, int64_t row, int64_t head,
+    int rows, int heads, int dim, const void* positions, int position_kind, int64_t position_row,
+    const double* frequencies, const int* pairs, int axes, int interleaved, int inverse, int dtype,
+    ocnn_stream_t stream);
+
+/* Gated linear recurrence over each sequence, per channel:
+ *   h_t = a_t h_{t-1} + (1 - a_t) data_t,  a_t = sigmoid(gate_t),  h_0 = state (or 0 where state is NULL)
+ * from the first row to the last (reverse != 0: from the last to the first).  out = h; last (may be NULL)
+ * [n_seq, channels] = the state behind the last step (of an empty sequence: the state it began with).
+ * States are fp32.  carries: [carry_rows, channels] fp32 as ocnn_recurrence_shape says, kept for the
+ * gradient; NULL where none is wanted.  `out` may be neither `gate` nor `data`.
+ * The gradient takes that of `out` and of `last` (grad_last, may be NULL) and writes those of gate, data
+ * and state (grad_state, may be NULL).  Results do not change from run to run. */
+int ocnn_recurrence_shape(int rows, int channels, int n_seq, int64_t* carry_rows, size_t* workspace_bytes,
+    size_t* grad_workspace_bytes);
+int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carries, const void* gate, int64_t gate_row,
+    const void* data, int64_t data_row, const float* state, const int* offsets, int n_seq, int rows, int channels,
+    int reverse, int fill_rest, int dtype, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream);
+int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* grad_data, int64_t grad_data_row,
+    float* grad_state, const void* grad_out, int64_t grad_out_row, const float* grad_last, const void* gate,
+    int64_t gate_row, const void* data, int64_t data_row, const float* state, const float* carries, const int* offsets,
+    int n_seq, int rows, int channels, int reverse, int dtype, void* workspace_dev, size_t workspace_bytes,
+    ocnn_stream_t stream);
+
+/* Attention inside each sequence.  Query i of a sequence of `queries` queries and `keys` keys stands at position
+ * i + keys - queries (the queries are the last of the keys' rows); key j is visible to the query at position p when
+ *   j <= p + right  and  (j >= p - left  or  j < sinks)  and  key_mask[j] != 0
+ * with -1 for a bound that is absent.  out = sum_j softmax_j(scale q . k_j) v_j over the visible keys, zeros where
+ * there is none; a value of a row that is not visible has no influence, whatever it holds.  lse [rows_q, heads]
+ * fp32 (may be NULL): the logarithm of the softmax's sum, -inf where no key is visible.
+ *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads);
+ *   k_offsets: where the rows of each sequence begin in k and v; k_lengths (device, may be NULL): how many of
+ *     them are keys -- a cache with room to grow; key_mask (device, may be NULL): one byte a key row;
+ *   dim: a multiple of 8 up to 128; sinks <= 64; every row and head begins at a multiple of 16 bytes.
+ * The gradient takes out and lse of the forward call; key rows that are no keys get zeros.  Scores, statistics
+ * and sums are fp32; bf16 probabilities and score gradients are rounded to bf16 as operands of the second
+ * product.  Results do not change from run to run.  Both calls need ocnn_attention_workspace_bytes bytes
+ * (16-byte aligned; the first may need none). */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int *q_offsets, *k_offsets, *k_lengths;
+  const unsigned char* key_mask;
+  int n_seq, rows_q, rows_k, heads, kv_heads, dim, left, right, sinks, dtype;
+  float scale;
+} ocnn_attention_params;
+int ocnn_attention_workspace_bytes(const ocnn_attention_params* params, size_t* workspace_bytes, size_t* grad_workspace_bytes);
+int ocnn_octree_attention(void* out, int64_t out_row, int64_t out_head, float* lse, const ocnn_attention_params* params,
+    int fill_rest, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream);
+int ocnn_octree_attention_grad(void* grad_q, int64_t grad_q_row, int64_t grad_q_head, void* grad_k, int64_t grad_k_row,
+    int64_t grad_k_head, void* grad_v, int64_t grad_v_row, int64_t grad_v_head, const void* grad_out, int64_t grad_out_row,
+    int64_t grad_out_head, const void* out, int64_t out_row, int64_t out_head, const float* lse,
+    const ocnn_attention_params* params, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,8 @@ The directory name is not a Python identifier; load the package with
 
   nn        -- mirror of the reference's `ocnn.nn` extension functions
                (pytorch/cpp/pybind.cpp:3-49) over libocnn_hip.so
+  sequence  -- operators along the node order of a level (rotary positions, attention, gated linear
+               recurrence), re-exported by nn
   autograd  -- torch.autograd functions pairing every operator with its adjoint, as the
                Function classes of pytorch/ocnn do
   layers    -- module front ends of the operators under the reference's class names
@@ -14,7 +16,7 @@ The directory name is not a Python identifier; load the package with
   synthetic -- seeded synthetic point clouds of the benchmark configurations
   transforms -- NormalizePoints / TransformPoints / Points2Octree / TransformCompose / collate_octrees
 """
-from . import lib, nn, autograd, layers, stacks, synthetic, transforms  # noqa: F401
+from . import lib, nn, sequence, autograd, layers, stacks, synthetic, transforms  # noqa: F401
 from .nn import *  # noqa: F401,F403
 from .layers import (OctreeConvolution, OctreeConv, OctreeDeconv, OctreeConvFast,  # noqa: F401
                      OctreeDeconvFast, OctreeMaxPool, OctreeMaxUnpool, OctreeAvgPool, OctreePad,

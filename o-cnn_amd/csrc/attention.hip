@@ -1,0 +1,1267 @@
+// Attention along the node order of an octree level: ragged sequences, a sliding window, the first `sinks`
+// keys of a sequence visible to every later query, query heads that share key heads.
+//
+//   s_ij = scale q_i . k_j,  key j visible to the query at position p = i + keys - queries  iff
+//     j <= p + right and (j >= p - left or j < sinks) and key_mask[j]
+//   o_i = sum_j softmax_j(s_ij) v_j  over the visible keys; zeros where there is none
+//   P = exp(s - lse), dV = P^T dO, dS = P (dO V^T - rowsum(dO o)), dQ = scale dS K, dK = scale dS^T Q
+//
+// Products run on the matrix cores, 32x32 tiles.  Every kernel computes the score tile TRANSPOSED to what
+// its second product wants as an operand: an accumulator of v_mfma_f32_32x32 holds, in lane l, column
+// l % 32 and rows 8 b + 4 (l / 32) + e, and the same lane of a B operand has to hold the same column and 8
+// (bf16: rows of the contraction; fp32: 1) values of the contraction.  The order of the contraction is free
+// as long as both operands agree, so the rows an accumulator lane holds are taken as they are: the
+// probabilities go from the first product to the second in registers, and softmax statistics are one
+// value a lane.  The other operand is read in the matching order: from LDS by ds_read_b64_tr_b16 (bf16) or
+// 4 bytes a lane (fp32).
+//
+// Rows of a key head: the query heads that share it are packed as rows (token, head in group), so one
+// pass over the keys serves the whole group, and a step of one token fills up to 32 columns.
+#include "sequence.h"
+
+#include <algorithm>
+
+namespace ocnn {
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxSinks = 64;
+constexpr int kFarRows = 256;   // tokens of a work item of the sinks' gradient
+
+struct AttnArgs {
+  ocnn_attention_params p;
+  void* out; int64_t out_row, out_head;
+  float* lse;
+  const void* grad; int64_t grad_row, grad_head;              // of the output
+  const void* fwd; int64_t fwd_row, fwd_head;                 // the output of the forward call
+  void* dq; void* dk; void* dv;
+  int64_t dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  float* delta;
+  float* part_o; float* part_ml;                              // split keys: [split][row][dim], [split][row][2]
+  float* sink_part;                                           // [work item][kv head][2][sinks][dim]
+  int splits, fill, group;
+  float scale2;                                               // scale * log2(e)
+};
+
+template <typename T> struct Frag;
+template <> struct Frag<uint16_t> { using type = bf16x8; };
+template <> struct Frag<float> { using type = floatx4; };
+
+// What a tile of rows looks like in LDS and in operands.  A 16-byte piece is kPiece elements; one step of the
+// contraction over channels takes two pieces, one from each half of the wavefront.
+template <typename T, int DP> struct Shape {
+  static constexpr int kPiece = 16 / (int)sizeof(T);
+  static constexpr int kSteps = DP / (2 * kPiece);
+  static constexpr int kPieces = DP / kPiece;           // of a row
+  static constexpr int kPitch = DP + kPiece;            // one piece of padding: rows start 4 banks apart
+  static constexpr int kBlocks = DP / 32;               // 32-channel blocks of a transposed accumulator
+};
+// a lane's pieces of one row: a column of a B operand
+template <typename T, int DP> struct Column { typename Frag<T>::type v[Shape<T, DP>::kSteps]; };
+
+__device__ inline floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx16 mma(floatx4 a, floatx4 b, floatx16 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+__device__ inline floatx16 zero16() {
+  floatx16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+// The lane's pieces of a row (a column of a B operand), straight from memory; zeros where the row or the
+// channels do not exist.
+template <typename T, int DP>
+__device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim) {
+  using S = Shape<T, DP>;
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    const int c = (2 * s + half) * S::kPiece;
+    uintx4 v = {0, 0, 0, 0};
+    if (ok && c < dim) v = *(const uintx4*)(row + c);
+    f.v[s] = __builtin_bit_cast(typename Frag<T>::type, v);
+  }
+}
+
+// acc[row of the tile][column] += tile rows . column
+template <typename T, int DP>
+__device__ inline floatx16 rows_times(const T* tile, const Column<T, DP>& col, floatx16 acc) {
+  using S = Shape<T, DP>;
+  const int lane = threadIdx.x & 63;
+  const T* at = tile + (lane & 31) * S::kPitch + (lane >> 5) * S::kPiece;
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s)
+    acc = mma(*(const typename Frag<T>::type*)(at + 2 * s * S::kPiece), col.v[s], acc);
+  return acc;
+}
+
+__device__ inline shortx4 read_transposed(const uint16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)(p));
+}
+
+__device__ inline uint32_t pack_bf16(float lo, float hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  bf16x2 v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// acc[block][channel][column] += sum over the 32 rows of the tile: tile[row][channel] * w[row][column], w as an
+// accumulator of rows_times holds it.  bf16: w is rounded to bf16 (2^-9 of each weight at most, the same
+// as the tile's own elements carry); statistics and sums stay in 32 bits.
+template <int DP>
+__device__ inline void columns_times(floatx16 (&acc)[DP / 32], const uint16_t* tile, const floatx16& w) {
+  using S = Shape<uint16_t, DP>;
+  const int lane = threadIdx.x & 63;
+  // 16 lanes read 4 rows of 16 channels and get them back by channel
+  const uint16_t* at = tile + ((lane >> 5) * 4 + ((lane >> 2) & 3)) * S::kPitch + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    uintx4 b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = pack_bf16(w[8 * s + 2 * i], w[8 * s + 2 * i + 1]);
+    const bf16x8 bw = __builtin_bit_cast(bf16x8, b);
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d) {
+      struct { shortx4 lo, hi; } a = {read_transposed(at + 16 * s * S::kPitch + 32 * d),
+                                      read_transposed(at + (16 * s + 8) * S::kPitch + 32 * d)};
+      acc[d] = mma(__builtin_bit_cast(bf16x8, a), bw, acc[d]);
+    }
+  }
+}
+template <int DP>
+__device__ inline void columns_times(floatx16 (&acc)[DP / 32], const float* tile, const floatx16& w) {
+  using S = Shape<float, DP>;
+  const int lane = threadIdx.x & 63;
+  const float* at = tile + (lane >> 5) * 4 * S::kPitch + (lane & 31);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+      acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * S::kPitch + 32 * d], w[r], acc[d], 0, 0, 0);
+}
+
+// Row r of an accumulator register in this lane
+__device__ inline int acc_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (r & 3); }
+
+// A tile of ROWS rows on its way from memory to LDS: the loads of the next tile are issued before the current
+// one is used and wait in registers.
+template <typename T, int DP, int ROWS, int THREADS> struct Staged {
+  using S = Shape<T, DP>;
+  static constexpr int kEach = ROWS * S::kPieces / THREADS;
+  static_assert(kEach * THREADS == ROWS * S::kPieces, "whole pieces a thread");
+  uintx4 v[kEach];
+  // row(i): pointer to tile row i or null where there is none
+  template <typename Row> __device__ inline void load(int tid, int dim, Row row) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = tid + i * THREADS, r = at / S::kPieces, c = (at % S::kPieces) * S::kPiece;
+      const T* p = row(r);
+      uintx4 x = {0, 0, 0, 0};
+      if (p && c < dim) x = *(const uintx4*)(p + c);
+      v[i] = x;
+    }
+  }
+  __device__ inline void store(T* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = tid + i * THREADS, r = at / S::kPieces, c = (at % S::kPieces) * S::kPiece;
+      *(uintx4*)(tile + r * S::kPitch + c) = v[i];
+    }
+  }
+};
+
+__device__ inline float wave_max(float x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
+  return x;
+}
+__device__ inline float wave_sum(float x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+__device__ inline bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+// orders the LDS accesses of one wavefront across its lanes
+__device__ inline void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// One sequence as the kernels see it
+struct Seq {
+  int q0, queries, k0, keys, room;      // room: key rows up to the next sequence
+  __device__ inline int shift() const { return keys - queries; }    // position of query 0
+};
+__device__ inline Seq sequence(const ocnn_attention_params& p, int b) {
+  Seq s;
+  s.q0 = clamped(p.q_offsets, b, p.rows_q);
+  s.queries = max(clamped(p.q_offsets, b + 1, p.rows_q) - s.q0, 0);
+  s.k0 = clamped(p.k_offsets, b, p.rows_k);
+  s.room = max(clamped(p.k_offsets, b + 1, p.rows_k) - s.k0, 0);
+  s.keys = p.k_lengths ? min(max(p.k_lengths[b], 0), s.room) : s.room;
+  return s;
+}
+// the keys a query at position pos sees through the window: [lo, hi)
+__device__ inline int window_lo(const ocnn_attention_params& p, int pos) { return p.left < 0 ? 0 : max(pos - p.left, 0); }
+__device__ inline int window_hi(const ocnn_attention_params& p, int pos, int keys) {
+  return p.right < 0 ? keys : max(min(pos + p.right + 1, keys), 0);
+}
+
+// ---- forward -------------------------------------------------------------------------------------------
+// QW = 4: a workgroup takes 128 packed rows, 32 a wavefront; tiles of 64 keys go through LDS once for all
+// four.  QW = 1 (few rows a sequence): 32 packed rows, and the wavefronts take every fourth tile of 32
+// keys each on their own, joined at the end.  Where rows x key heads leave compute units empty, the
+// tiles are dealt out over `splits` workgroups, joined by attention_join_kernel.
+template <typename T, int DP, int QW> struct ForwardShape {
+  static constexpr int kKeys = QW == 4 ? 64 : 32;
+  static constexpr int kTile = kKeys * Shape<T, DP>::kPitch;
+  static constexpr int kBuffers = QW == 4 ? 2 : 4;            // double buffer, or one a wavefront
+  static constexpr size_t kJoin = QW == 4 ? 0 : 3 * (size_t)(DP / 32) * 16 * 64 * 4;
+  static constexpr size_t kTiles = (size_t)kBuffers * 2 * kTile * sizeof(T);
+  static constexpr size_t kLds = kTiles > kJoin ? kTiles : kJoin;
+};
+
+struct Softmax { float m, l; };
+
+// One row again, visible terms only: for rows whose result is not finite.  The products above multiply the
+// values of keys that a row does not see by a probability of zero, which is no zero where such a value is
+// infinite or NaN.  `tiles` (first tile, last tile, sink tiles, keys a tile) are those of this workgroup.
+template <typename T, int DP>
+__device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& s, int kv, int row, int v0, int v1, int sink_tiles,
+    int t0, int key_tile, Softmax* st, float (&o)[(DP + 63) / 64]) {
+  const ocnn_attention_params& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int token = row / a.group, head = kv * a.group + row % a.group;
+  const int pos = token + s.shift(), lo = window_lo(p, pos), hi = window_hi(p, pos, s.keys);
+  const T* q = (const T*)p.q + (int64_t)(s.q0 + token) * p.q_row + head * p.q_head;
+  float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i) o[i] = 0.0f;
+  for (int v = v0; v < v1; ++v) {
+    const int j0 = (v < sink_tiles ? v : t0 + v - sink_tiles) * key_tile;
+    const int j = j0 + lane;
+    bool see = lane < key_tile && j < hi && (j >= lo || j < p.sinks);
+    if (see && p.key_mask) see = p.key_mask[s.k0 + j] != 0;
+    float x = -__builtin_inff();
+    if (see) {
+      const T* k = (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head;
+      float dot = 0.0f;
+      for (int c = 0; c < p.dim; ++c) dot = fmaf(to_f32(q[c]), to_f32(k[c]), dot);
+      x = dot * a.scale2;
+    }
+    uint64_t left = __ballot(see);
+    if (!left) continue;
+    // (fmax drops a NaN: it has to reach the sum)
+    const float top = fmaxf(m, wave_max(x)), base = top == -__builtin_inff() ? 0.0f : top;
+    const float shrink = exp2f(m - base), e = see ? exp2f(x - base) : 0.0f;
+    l = l * shrink + wave_sum(e);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < (DP + 63) / 64; ++i) o[i] *= shrink;
+    while (left) {
+      const int jj = __ffsll((unsigned long long)left) - 1;
+      left &= left - 1;
+      const float w = __shfl(e, jj, 64);
+      const T* vr = (const T*)p.v + (int64_t)(s.k0 + j0 + jj) * p.v_row + kv * p.v_head;
+#pragma unroll
+      for (int i = 0; i < (DP + 63) / 64; ++i)
+        if (lane + 64 * i < p.dim) o[i] = fmaf(w, to_f32(vr[lane + 64 * i]), o[i]);
+    }
+  }
+  st->m = m;
+  st->l = l;
+}
+
+template <typename T, int DP, int QW, bool SPLIT>
+__global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_kernel(AttnArgs a) {
+  using S = Shape<T, DP>;
+  using F = ForwardShape<T, DP, QW>;
+  constexpr int kRows = 32 * QW, kShift = Log2<kRows>::value;
+  __shared__ __attribute__((aligned(16))) char lds[F::kLds];
+  __shared__ Softmax stats[4][32];
+  const ocnn_attention_params& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int kv = blockIdx.y, split = SPLIT ? blockIdx.z : 0;
+  const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, blockIdx.x, kShift, a.group);
+  const int q_begin = clamped(p.q_offsets, b, p.rows_q);
+  const int64_t tile = (int64_t)blockIdx.x - (((int64_t)q_begin * a.group >> kShift) + b);
+  Seq s;
+  if (b >= p.n_seq) {
+    s.q0 = q_begin; s.queries = p.rows_q - q_begin; s.k0 = 0; s.keys = 0; s.room = 0;
+  } else {
+    s = sequence(p, b);
+  }
+  const int64_t row0 = tile * kRows;
+  const int rows = s.queries * a.group;
+  if (tile < 0 || row0 >= rows) return;
+  const int row = (int)row0 + (QW == 4 ? wave * 32 : 0) + col;
+  const bool have = row < rows;
+  const int token = have ? row / a.group : 0, in_group = have ? row - token * a.group : 0;
+  const int head = kv * a.group + in_group;
+  const int64_t out_at = (int64_t)(s.q0 + token);
+
+  if (b >= p.n_seq) {                       // rows behind the last sequence
+    if (SPLIT) {
+      if (have && half == 0 && (QW == 4 || wave == 0)) {
+        float* ml = a.part_ml + (((int64_t)split * p.rows_q + out_at) * p.heads + head) * 2;
+        ml[0] = -__builtin_inff();
+        ml[1] = -1.0f;                      // (what the joining kernel knows them by)
+      }
+      return;
+    }
+    if (a.fill && have && (QW == 4 || wave == 0)) {
+      T* o = (T*)a.out + out_at * a.out_row + head * a.out_head;
+      for (int c = half * S::kPiece; c < p.dim; c += 2 * S::kPiece) *(uintx4*)(o + c) = uintx4{0, 0, 0, 0};
+      if (a.lse && half == 0) a.lse[out_at * p.heads + head] = -__builtin_inff();
+    }
+    return;
+  }
+
+  // what this lane's row sees, and what the wavefront's and the workgroup's rows see
+  const int pos = token + s.shift();
+  const int lo = have ? window_lo(p, pos) : 0, hi = have ? window_hi(p, pos, s.keys) : 0;
+  const int sinks = have ? p.sinks : 0;
+  const int first_row = (int)row0 + (QW == 4 ? wave * 32 : 0), last_row = min(first_row + 31, rows - 1);
+  int w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;            // some row sees / every row sees
+  if (first_row < rows) {
+    const int pa = first_row / a.group + s.shift(), pb = last_row / a.group + s.shift();
+    w_lo = window_lo(p, pa);
+    w_hi = window_hi(p, pb, s.keys);
+    all_lo = window_lo(p, pb);
+    all_hi = first_row + 31 < rows ? window_hi(p, pa, s.keys) : 0;
+  }
+  const int block_last = min((int)row0 + kRows, rows) - 1;
+  const int b_lo = window_lo(p, (int)row0 / a.group + s.shift());
+  const int b_hi = window_hi(p, block_last / a.group + s.shift(), s.keys);
+  constexpr int KT = F::kKeys;
+  const int t0 = b_lo / KT, t1 = max((b_hi + KT - 1) / KT, t0);
+  // tiles of the sinks in front of the window's: their keys are visible up to what causality allows
+  const int sink_tiles = min((min(p.sinks, b_hi) + KT - 1) / KT, t0);
+  const int tiles = sink_tiles + t1 - t0;
+  const int v0 = SPLIT ? (int)((int64_t)tiles * split / a.splits) : 0;
+  const int v1 = SPLIT ? (int)((int64_t)tiles * (split + 1) / a.splits) : tiles;
+  auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
+
+  Column<T, DP> q;
+  load_row<T, DP>(q, (const T*)p.q + out_at * p.q_row + head * p.q_head, have, p.dim);
+  floatx16 o[S::kBlocks];
+#pragma unroll
+  for (int d = 0; d < S::kBlocks; ++d) o[d] = zero16();
+  float m = -__builtin_inff(), l = 0.0f;
+
+  const T* kbase = (const T*)p.k + (int64_t)s.k0 * p.k_row + kv * p.k_head;
+  const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
+  const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
+
+  // scores of 32 keys from j0 on against this wavefront's rows -> probabilities -> o
+  auto subtile = [&](const T* kt, const T* vt, int j0) {
+    const bool reach = (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi);
+    if (!reach) return;
+    floatx16 x = rows_times<T, DP>(kt, q, zero16());
+    const bool whole = j0 >= all_lo && j0 + 32 <= all_hi && !mask;
+    if (!whole) {
+      uint32_t live = ~0u;
+      if (mask) live = (uint32_t)__ballot(j0 + col < s.keys && mask[min(j0 + col, s.keys - 1)] != 0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = j0 + acc_row(r);
+        const bool see = j < hi && (j >= lo || j < sinks) && (live >> acc_row(r) & 1);
+        x[r] = see ? x[r] : -__builtin_inff();
+      }
+    }
+    float top = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale2;
+    const float to = fmaxf(m, top), base = to == -__builtin_inff() ? 0.0f : to;
+    if (__any(to != m)) {
+      const float shrink = __builtin_amdgcn_exp2f(m - base);
+      l *= shrink;
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
+      m = to;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -base));
+      sum += x[r];
+    }
+    l += sum;
+    columns_times<DP>(o, vt, x);
+  };
+
+  if constexpr (QW == 4) {
+    Staged<T, DP, KT, 256> sk, sv;
+    auto fetch = [&](int v) {
+      const int j0 = tile_key(v);
+      sk.load(tid, p.dim, [&](int r) -> const T* {
+        const int j = j0 + r;
+        return j < s.keys && (!mask || mask[j]) ? kbase + (int64_t)j * p.k_row : nullptr;
+      });
+      sv.load(tid, p.dim, [&](int r) -> const T* {
+        const int j = j0 + r;
+        return j < s.keys && (!mask || mask[j]) ? vbase + (int64_t)j * p.v_row : nullptr;
+      });
+    };
+    if (v0 < v1) fetch(v0);
+    for (int v = v0; v < v1; ++v) {
+      T* kt = (T*)lds + (v & 1) * 2 * F::kTile;
+      T* vt = kt + F::kTile;
+      sk.store(kt, tid);
+      sv.store(vt, tid);
+      __syncthreads();                        // (the other buffer's readers are done: they passed the last barrier)
+      if (v + 1 < v1) fetch(v + 1);
+      const int j0 = tile_key(v);
+      subtile(kt, vt, j0);
+      subtile(kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32);
+    }
+  } else {
+    Staged<T, DP, KT, 64> sk, sv;
+    auto fetch = [&](int v) {
+      const int j0 = tile_key(v);
+      sk.load(lane, p.dim, [&](int r) -> const T* {
+        const int j = j0 + r;
+        return j < s.keys && (!mask || mask[j]) ? kbase + (int64_t)j * p.k_row : nullptr;
+      });
+      sv.load(lane, p.dim, [&](int r) -> const T* {
+        const int j = j0 + r;
+        return j < s.keys && (!mask || mask[j]) ? vbase + (int64_t)j * p.v_row : nullptr;
+      });
+    };
+    T* kt = (T*)lds + wave * 2 * F::kTile;
+    T* vt = kt + F::kTile;
+    if (v0 + wave < v1) fetch(v0 + wave);
+    for (int v = v0 + wave; v < v1; v += 4) {
+      wave_lds_fence();
+      sk.store(kt, lane);
+      sv.store(vt, lane);
+      wave_lds_fence();
+      if (v + 4 < v1) fetch(v + 4);
+      subtile(kt, vt, tile_key(v));
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+
+  if constexpr (QW == 1) {                    // the wavefronts' shares, joined in the first one
+    if (half == 0) stats[wave][col] = Softmax{m, l};
+    __syncthreads();
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stats[w][col].m);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    const float mine = __builtin_amdgcn_exp2f(m - base);
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += stats[w][col].l * __builtin_amdgcn_exp2f(stats[w][col].m - base);
+    float* join = (float*)lds;
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        o[d][r] *= mine;
+        if (wave) join[(((wave - 1) * S::kBlocks + d) * 16 + r) * 64 + lane] = o[d][r];
+      }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] += join[((w * S::kBlocks + d) * 16 + r) * 64 + lane];
+    m = top;
+    l = sum;
+  }
+
+  float worst = 0.0f;                         // not finite where any of them is not
+#pragma unroll
+  for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) worst += fabsf(o[d][r]);
+  worst += __shfl_xor(worst, 32, 64);
+  const bool good = finite(worst) && finite(l);
+  const int64_t at_row = out_at * p.heads + head;
+  if (have && good) {
+    if (SPLIT) {
+      float* po = a.part_o + ((int64_t)split * p.rows_q * p.heads + at_row) * p.dim;
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = 32 * d + 8 * i + 4 * half;
+          if (c < p.dim) *(floatx4*)(po + c) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        }
+      if (half == 0) {
+        float* ml = a.part_ml + ((int64_t)split * p.rows_q * p.heads + at_row) * 2;
+        ml[0] = m;
+        ml[1] = l;
+      }
+    } else {
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      T* po = (T*)a.out + out_at * a.out_row + head * a.out_head;
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = 32 * d + 8 * i + 4 * half;
+          Pack<T, 4> x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x.v[e] = from_f32<T>(o[d][4 * i + e] * inv);
+          if (c < p.dim) x.store(po + c);
+        }
+      if (a.lse && half == 0) a.lse[at_row] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -__builtin_inff();
+    }
+  }
+  uint32_t bad = (uint32_t)__ballot(have && !good);
+  while (bad) {
+    const int c = __ffs(bad) - 1;
+    bad &= bad - 1;
+    const int r = __shfl(row, c, 64);
+    Softmax st;
+    float oo[(DP + 63) / 64];
+    forward_row_again<T, DP>(a, s, kv, r, v0, v1, sink_tiles, t0, KT, &st, oo);
+    const int tk = r / a.group, hd = kv * a.group + r % a.group;
+    const int64_t at = (int64_t)(s.q0 + tk) * p.heads + hd;
+#pragma unroll
+    for (int i = 0; i < (DP + 63) / 64; ++i) {
+      const int ch = lane + 64 * i;
+      if (ch >= p.dim) continue;
+      if (SPLIT) a.part_o[((int64_t)split * p.rows_q * p.heads + at) * p.dim + ch] = oo[i];
+      else ((T*)a.out)[(int64_t)(s.q0 + tk) * a.out_row + hd * a.out_head + ch] = from_f32<T>(st.l == 0.0f ? 0.0f : oo[i] / st.l);
+    }
+    if (lane == 0) {
+      if (SPLIT) {
+        float* ml = a.part_ml + ((int64_t)split * p.rows_q * p.heads + at) * 2;
+        ml[0] = st.m;
+        ml[1] = st.l;
+      } else if (a.lse) {
+        a.lse[at] = st.l == 0.0f ? -__builtin_inff() : (st.m + __builtin_amdgcn_logf(st.l)) * kLn2;
+      }
+    }
+  }
+}
+
+// o = sum_s exp(m_s - m) o_s / sum_s exp(m_s - m) l_s, a wavefront a row
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs a) {
+  const ocnn_attention_params& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)p.rows_q * p.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int64_t token = row / p.heads;
+  const int head = (int)(row - token * p.heads);
+  float m = -__builtin_inff(), l = 0.0f;
+  bool none = false;
+  for (int s = 0; s < a.splits; ++s) {
+    m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
+    none = none || a.part_ml[(s * rows + row) * 2 + 1] == -1.0f;
+  }
+  if (none && !a.fill) return;
+  const float base = m == -__builtin_inff() ? 0.0f : m;
+  float o0 = 0.0f, o1 = 0.0f;
+  if (!none)
+    for (int s = 0; s < a.splits; ++s) {
+      const float ls = a.part_ml[(s * rows + row) * 2 + 1];
+      if (ls == 0.0f) continue;               // (a share without a visible key: its values do not count)
+      const float w = __builtin_amdgcn_exp2f(a.part_ml[(s * rows + row) * 2] - base);
+      l += w * ls;
+      const float* po = a.part_o + (s * rows + row) * p.dim;
+      if (lane < p.dim) o0 = fmaf(w, po[lane], o0);
+      if (lane + 64 < p.dim) o1 = fmaf(w, po[lane + 64], o1);
+    }
+  T* out = (T*)a.out + token * a.out_row + head * a.out_head;
+  if (lane < p.dim) out[lane] = from_f32<T>(l == 0.0f ? 0.0f : o0 / l);
+  if (lane + 64 < p.dim) out[lane + 64] = from_f32<T>(l == 0.0f ? 0.0f : o1 / l);
+  if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---- gradient of the queries ---------------------------------------------------------------------------
+// Rows as in the forward kernel (QW = 4); the scores are computed again from lse.  rowsum(dO o) is formed
+// here, from the row's own registers, and left for the kernel of the keys.  No atomics: dQ and dK, dV each
+// have a kernel that owns their rows, at the price of computing the scores twice.
+template <typename T, int DP>
+__device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s, int kv, int row, int t0, int t1, int sink_tiles,
+    float lse2, float delta, float (&dq)[(DP + 63) / 64]) {
+  const ocnn_attention_params& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int token = row / a.group, head = kv * a.group + row % a.group;
+  const int pos = token + s.shift(), lo = window_lo(p, pos), hi = window_hi(p, pos, s.keys);
+  const T* q = (const T*)p.q + (int64_t)(s.q0 + token) * p.q_row + head * p.q_head;
+  const T* go = (const T*)a.grad + (int64_t)(s.q0 + token) * a.grad_row + head * a.grad_head;
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i) dq[i] = 0.0f;
+  for (int v = 0; v < sink_tiles + t1 - t0; ++v) {
+    const int j0 = (v < sink_tiles ? v : t0 + v - sink_tiles) * 64, j = j0 + lane;
+    bool see = j < hi && (j >= lo || j < p.sinks);
+    if (see && p.key_mask) see = p.key_mask[s.k0 + j] != 0;
+    float ds = 0.0f;
+    if (see) {
+      const T* k = (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head;
+      const T* vr = (const T*)p.v + (int64_t)(s.k0 + j) * p.v_row + kv * p.v_head;
+      float dot = 0.0f, dp = 0.0f;
+      for (int c = 0; c < p.dim; ++c) {
+        dot = fmaf(to_f32(q[c]), to_f32(k[c]), dot);
+        dp = fmaf(to_f32(go[c]), to_f32(vr[c]), dp);
+      }
+      ds = exp2f(fmaf(dot, a.scale2, -lse2)) * (dp - delta);
+    }
+    uint64_t left = __ballot(see);
+    while (left) {
+      const int jj = __ffsll((unsigned long long)left) - 1;
+      left &= left - 1;
+      const float w = __shfl(ds, jj, 64);
+      const T* kr = (const T*)p.k + (int64_t)(s.k0 + j0 + jj) * p.k_row + kv * p.k_head;
+#pragma unroll
+      for (int i = 0; i < (DP + 63) / 64; ++i)
+        if (lane + 64 * i < p.dim) dq[i] = fmaf(w, to_f32(kr[lane + 64 * i]), dq[i]);
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_grad_q_kernel(AttnArgs a) {
+  using S = Shape<T, DP>;
+  constexpr int KT = 64, kTile = KT * S::kPitch, kRows = 128, kShift = 7;
+  __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
+  const ocnn_attention_params& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int kv = blockIdx.y;
+  const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, blockIdx.x, kShift, a.group);
+  const int q_begin = clamped(p.q_offsets, b, p.rows_q);
+  const int64_t tile = (int64_t)blockIdx.x - (((int64_t)q_begin * a.group >> kShift) + b);
+  Seq s;
+  if (b >= p.n_seq) {
+    s.q0 = q_begin; s.queries = p.rows_q - q_begin; s.k0 = 0; s.keys = 0; s.room = 0;
+  } else {
+    s = sequence(p, b);
+  }
+  const int64_t row0 = tile * kRows;
+  const int rows = s.queries * a.group;
+  if (tile < 0 || row0 >= rows) return;
+  const int row = (int)row0 + wave * 32 + col;
+  const bool have = row < rows;
+  const int token = have ? row / a.group : 0, in_group = have ? row - token * a.group : 0;
+  const int head = kv * a.group + in_group;
+  const int64_t at = (int64_t)(s.q0 + token);
+  T* dq_row = (T*)a.dq + at * a.dq_row + head * a.dq_head;
+  if (b >= p.n_seq) {
+    if (have)
+      for (int c = half * S::kPiece; c < p.dim; c += 2 * S::kPiece) *(uintx4*)(dq_row + c) = uintx4{0, 0, 0, 0};
+    return;
+  }
+  const int pos = token + s.shift();
+  const int lo = have ? window_lo(p, pos) : 0, hi = have ? window_hi(p, pos, s.keys) : 0, sinks = have ? p.sinks : 0;
+  const int first_row = (int)row0 + wave * 32, last_row = min(first_row + 31, rows - 1);
+  int w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
+  if (first_row < rows) {
+    const int pa = first_row / a.group + s.shift(), pb = last_row / a.group + s.shift();
+    w_lo = window_lo(p, pa);
+    w_hi = window_hi(p, pb, s.keys);
+    all_lo = window_lo(p, pb);
+    all_hi = first_row + 31 < rows ? window_hi(p, pa, s.keys) : 0;
+  }
+  const int block_last = min((int)row0 + kRows, rows) - 1;
+  const int b_lo = window_lo(p, (int)row0 / a.group + s.shift());
+  const int b_hi = window_hi(p, block_last / a.group + s.shift(), s.keys);
+  const int t0 = b_lo / KT, t1 = max((b_hi + KT - 1) / KT, t0);
+  const int sink_tiles = min((min(p.sinks, b_hi) + KT - 1) / KT, t0);
+  const int tiles = sink_tiles + t1 - t0;
+
+  Column<T, DP> q, go;
+  load_row<T, DP>(go, (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
+  float delta = 0.0f;
+  load_row<T, DP>(q, (const T*)a.fwd + at * a.fwd_row + head * a.fwd_head, have, p.dim);
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+    for (int e = 0; e < S::kPiece; ++e) delta = fmaf((float)q.v[i][e], (float)go.v[i][e], delta);
+  delta += __shfl_xor(delta, 32, 64);
+  load_row<T, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim);
+  const int64_t at_row = at * p.heads + head;
+  const float lse = have ? a.lse[at_row] : -__builtin_inff();
+  const float lse2 = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
+  if (have && half == 0) a.delta[at_row] = delta;
+
+  floatx16 dq[S::kBlocks];
+#pragma unroll
+  for (int d = 0; d < S::kBlocks; ++d) dq[d] = zero16();
+  const T* kbase = (const T*)p.k + (int64_t)s.k0 * p.k_row + kv * p.k_head;
+  const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
+  const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
+
+  auto subtile = [&](const T* kt, const T* vt, int j0) {
+    const bool reach = (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi);
+    if (!reach) return;
+    floatx16 x = rows_times<T, DP>(kt, q, zero16());
+    const floatx16 dp = rows_times<T, DP>(vt, go, zero16());
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -lse2)) * (dp[r] - delta);
+    if (!(j0 >= all_lo && j0 + 32 <= all_hi && !mask)) {
+      uint32_t live = ~0u;
+      if (mask) live = (uint32_t)__ballot(j0 + col < s.keys && mask[min(j0 + col, s.keys - 1)] != 0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = j0 + acc_row(r);
+        const bool see = j < hi && (j >= lo || j < sinks) && (live >> acc_row(r) & 1);
+        x[r] = see ? x[r] : 0.0f;
+      }
+    }
+    columns_times<DP>(dq, kt, x);
+  };
+  auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
+  Staged<T, DP, KT, 256> sk, sv;
+  auto fetch = [&](int v) {
+    const int j0 = tile_key(v);
+    sk.load(tid, p.dim, [&](int r) -> const T* {
+      const int j = j0 + r;
+      return j < s.keys && (!mask || mask[j]) ? kbase + (int64_t)j * p.k_row : nullptr;
+    });
+    sv.load(tid, p.dim, [&](int r) -> const T* {
+      const int j = j0 + r;
+      return j < s.keys && (!mask || mask[j]) ? vbase + (int64_t)j * p.v_row : nullptr;
+    });
+  };
+  if (tiles > 0) fetch(0);
+  for (int v = 0; v < tiles; ++v) {
+    T* kt = lds + (v & 1) * 2 * kTile;
+    T* vt = kt + kTile;
+    sk.store(kt, tid);
+    sv.store(vt, tid);
+    __syncthreads();
+    if (v + 1 < tiles) fetch(v + 1);
+    const int j0 = tile_key(v);
+    subtile(kt, vt, j0);
+    subtile(kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32);
+  }
+  float worst = 0.0f;
+#pragma unroll
+  for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) worst += fabsf(dq[d][r]);
+  worst += __shfl_xor(worst, 32, 64);
+  const bool good = finite(worst);
+  if (have && good)
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = 32 * d + 8 * i + 4 * half;
+        Pack<T, 4> x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v[e] = from_f32<T>(dq[d][4 * i + e] * p.scale);
+        if (c < p.dim) x.store(dq_row + c);
+      }
+  uint32_t bad = (uint32_t)__ballot(have && !good);
+  while (bad) {
+    const int c = __ffs(bad) - 1;
+    bad &= bad - 1;
+    const int r = __shfl(row, c, 64);
+    float g[(DP + 63) / 64];
+    grad_q_row_again<T, DP>(a, s, kv, r, t0, t1, sink_tiles, __shfl(lse2, c, 64), __shfl(delta, c, 64), g);
+    const int tk = r / a.group, hd = kv * a.group + r % a.group;
+#pragma unroll
+    for (int i = 0; i < (DP + 63) / 64; ++i)
+      if (lane + 64 * i < p.dim)
+        ((T*)a.dq)[(int64_t)(s.q0 + tk) * a.dq_row + hd * a.dq_head + lane + 64 * i] = from_f32<T>(g[i] * p.scale);
+  }
+}
+
+// ---- gradients of the keys and values --------------------------------------------------------------------
+// A workgroup owns 128 keys of a key head, 32 a wavefront, in registers; the packed rows that see them go
+// through LDS 64 at a time, so the query heads that share the key head are summed where they are
+// accumulated.  The first keys (sinks) are seen by every later row: the rows beyond the window of
+// their tile ("far") are dealt out in items of kFarRows tokens to workgroups of their own, whose sums over
+// the sinks go to memory in 32 bits and are added in order by attention_sink_kernel.
+struct FarRange { int first; bool any; };        // tokens [first, queries) see the sinks only
+__device__ inline FarRange far_tokens(const ocnn_attention_params& p, const Seq& s) {
+  FarRange f;
+  f.first = min(max(127 + p.left - s.shift() + 1, 0), s.queries);
+  f.any = p.sinks > 0 && p.left >= 0 && s.keys > 0 && f.first < s.queries;
+  return f;
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void grad_k_row_again(const AttnArgs& a, const Seq& s, int kv, int j, int from, int to,
+    float (&dk)[(DP + 63) / 64], float (&dv)[(DP + 63) / 64]) {
+  const ocnn_attention_params& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const T* k = (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head;
+  const T* v = (const T*)p.v + (int64_t)(s.k0 + j) * p.v_row + kv * p.v_head;
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i) dk[i] = dv[i] = 0.0f;
+  for (int r0 = from; r0 < to; r0 += 64) {
+    const int r = r0 + lane;
+    float w = 0.0f, ds = 0.0f;
+    if (r < to) {
+      const int token = r / a.group, head = kv * a.group + r % a.group;
+      const int64_t at = (int64_t)(s.q0 + token);
+      const T* q = (const T*)p.q + at * p.q_row + head * p.q_head;
+      const T* go = (const T*)a.grad + at * a.grad_row + head * a.grad_head;
+      float dot = 0.0f, dp = 0.0f;
+      for (int c = 0; c < p.dim; ++c) {
+        dot = fmaf(to_f32(q[c]), to_f32(k[c]), dot);
+        dp = fmaf(to_f32(go[c]), to_f32(v[c]), dp);
+      }
+      const float lse = a.lse[at * p.heads + head];
+      w = exp2f(fmaf(dot, a.scale2, lse == -__builtin_inff() ? 0.0f : -lse * kLog2e));
+      ds = w * (dp - a.delta[at * p.heads + head]);
+    }
+    for (int i = 0; i < min(64, to - r0); ++i) {
+      const float wi = __shfl(w, i, 64), di = __shfl(ds, i, 64);
+      const int token = (r0 + i) / a.group, head = kv * a.group + (r0 + i) % a.group;
+      const int64_t at = (int64_t)(s.q0 + token);
+      const T* q = (const T*)p.q + at * p.q_row + head * p.q_head;
+      const T* go = (const T*)a.grad + at * a.grad_row + head * a.grad_head;
+#pragma unroll
+      for (int n = 0; n < (DP + 63) / 64; ++n)
+        if (lane + 64 * n < p.dim) {
+          dk[n] = fmaf(di, to_f32(q[lane + 64 * n]), dk[n]);
+          dv[n] = fmaf(wi, to_f32(go[lane + 64 * n]), dv[n]);
+        }
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 : 2) attention_grad_kv_kernel(AttnArgs a,
+    int near_items) {
+  using S = Shape<T, DP>;
+  constexpr int RT = 64, kTile = RT * S::kPitch;
+  __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
+  __shared__ float row_lse[2][RT], row_delta[2][RT];
+  const ocnn_attention_params& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int kv = blockIdx.y;
+  const bool far = (int)blockIdx.x >= near_items;
+  int b, j0 = 0;
+  int64_t item;
+  if (!far) {
+    b = locate_packed(p.k_offsets, p.n_seq, p.rows_k, blockIdx.x, 7, 1);
+    item = (int64_t)blockIdx.x - ((clamped(p.k_offsets, b, p.rows_k) >> 7) + b);
+  } else {
+    const int id = (int)blockIdx.x - near_items;
+    b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, id, Log2<kFarRows>::value, 1);
+    item = (int64_t)id - ((clamped(p.q_offsets, b, p.rows_q) >> Log2<kFarRows>::value) + b);
+    if (b >= p.n_seq) return;
+  }
+  if (item < 0) return;
+  if (b >= p.n_seq) {                              // key rows behind the last sequence
+    const int k_begin = clamped(p.k_offsets, b, p.rows_k);
+    const int64_t r = k_begin + item * 128 + wave * 32 + col;
+    if (r < p.rows_k)
+      for (int c = half * S::kPiece; c < p.dim; c += 2 * S::kPiece) {
+        *(uintx4*)((T*)a.dk + r * a.dk_row + kv * a.dk_head + c) = uintx4{0, 0, 0, 0};
+        *(uintx4*)((T*)a.dv + r * a.dv_row + kv * a.dv_head + c) = uintx4{0, 0, 0, 0};
+      }
+    return;
+  }
+  const Seq s = sequence(p, b);
+  const FarRange fr = far_tokens(p, s);
+  const int shift = s.shift();
+  // the tokens that see the window keys [x, y]
+  auto first_token = [&](int x) { return p.right < 0 ? 0 : min(max(x - p.right - shift, 0), s.queries); };
+  auto end_token = [&](int y) { return p.left < 0 ? s.queries : min(max(y + p.left + 1 - shift, 0), s.queries); };
+  int ta, tb;                                      // tokens of this workgroup
+  if (!far) {
+    if (item * 128 >= s.room) return;
+    j0 = (int)item * 128;
+    ta = first_token(j0);
+    tb = end_token(j0 + 127);
+  } else {
+    if (!fr.any) return;
+    ta = max((int)item * kFarRows, fr.first);
+    tb = (int)min((item + 1) * kFarRows, (int64_t)s.queries);
+    if (ta >= tb) return;
+  }
+  const bool sink_tile = j0 == 0 && fr.any;        // its first keys' sums go to memory
+  const int j = j0 + wave * 32 + col;
+  bool key = j < s.keys && (!far || j < p.sinks);
+  if (key && p.key_mask) key = p.key_mask[s.k0 + j] != 0;
+  // this key's packed rows: [lo, hi), and what some / every key of the wavefront has
+  int lo = 0, hi = 0;
+  if (key) {
+    lo = first_token(j);
+    hi = j < p.sinks ? s.queries : end_token(j);
+    lo = max(lo, ta) * a.group;
+    hi = min(hi, tb) * a.group;
+  }
+  const int jw = j0 + wave * 32;
+  int w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
+  if (jw < s.keys && (!far || jw < p.sinks)) {
+    const bool any_sink = jw < p.sinks;
+    w_lo = max(first_token(jw), ta) * a.group;
+    w_hi = min(any_sink ? s.queries : end_token(jw + 31), tb) * a.group;
+    if (jw + 32 <= s.keys && !p.key_mask && (!far || jw + 32 <= p.sinks)) {
+      all_lo = max(first_token(jw + 31), ta) * a.group;
+      all_hi = min(end_token(jw), tb) * a.group;
+    }
+  }
+  Column<T, DP> k, vv;
+  load_row<T, DP>(k, (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head, key, p.dim);
+  load_row<T, DP>(vv, (const T*)p.v + (int64_t)(s.k0 + j) * p.v_row + kv * p.v_head, key, p.dim);
+  floatx16 dk[S::kBlocks], dv[S::kBlocks];
+#pragma unroll
+  for (int d = 0; d < S::kBlocks; ++d) dk[d] = dv[d] = zero16();
+
+  auto subtile = [&](const T* qt, const T* gt, const float* lse2, const float* delta, int r0) {
+    if (r0 + 32 <= w_lo || r0 >= w_hi) return;
+    floatx16 x = rows_times<T, DP>(qt, k, zero16());
+    floatx16 dp = rows_times<T, DP>(gt, vv, zero16());
+    floatx4 ls[4], de[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ls[i] = *(const floatx4*)(lse2 + 8 * i + 4 * half);
+      de[i] = *(const floatx4*)(delta + 8 * i + 4 * half);
+    }
+    const bool whole = r0 >= all_lo && r0 + 32 <= all_hi;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -ls[r >> 2][r & 3]));
+      dp[r] = x[r] * (dp[r] - de[r >> 2][r & 3]);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + acc_row(r);
+        const bool see = row >= lo && row < hi;
+        x[r] = see ? x[r] : 0.0f;
+        dp[r] = see ? dp[r] : 0.0f;
+      }
+    }
+    columns_times<DP>(dv, gt, x);
+    columns_times<DP>(dk, qt, dp);
+  };
+
+  const int ra = ta * a.group, rb = tb * a.group, tiles = s.keys > 0 ? max(rb - ra + RT - 1, 0) / RT : 0;
+  Staged<T, DP, RT, 256> sq, sg;
+  float one_lse = 0.0f, one_delta = 0.0f;
+  auto fetch = [&](int v) {
+    const int r0 = ra + v * RT;
+    sq.load(tid, p.dim, [&](int i) -> const T* {
+      const int r = r0 + i, token = a.group == 1 ? r : r / a.group;
+      return r < rb ? (const T*)p.q + (int64_t)(s.q0 + token) * p.q_row + (kv * a.group + r - token * a.group) * p.q_head : nullptr;
+    });
+    sg.load(tid, p.dim, [&](int i) -> const T* {
+      const int r = r0 + i, token = a.group == 1 ? r : r / a.group;
+      return r < rb ? (const T*)a.grad + (int64_t)(s.q0 + token) * a.grad_row + (kv * a.group + r - token * a.group) * a.grad_head
+                    : nullptr;
+    });
+    if (tid < RT) {
+      const int r = r0 + tid, token = r / a.group;
+      one_lse = one_delta = 0.0f;
+      if (r < rb) {
+        const int64_t at = (int64_t)(s.q0 + token) * p.heads + kv * a.group + r - token * a.group;
+        const float lse = a.lse[at];
+        one_lse = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
+        one_delta = a.delta[at];
+      }
+    }
+  };
+  if (tiles > 0) fetch(0);
+  for (int v = 0; v < tiles; ++v) {
+    const int buf = v & 1;
+    T* qt = lds + buf * 2 * kTile;
+    T* gt = qt + kTile;
+    sq.store(qt, tid);
+    sg.store(gt, tid);
+    if (tid < RT) {
+      row_lse[buf][tid] = one_lse;
+      row_delta[buf][tid] = one_delta;
+    }
+    __syncthreads();
+    if (v + 1 < tiles) fetch(v + 1);
+    const int r0 = ra + v * RT;
+    subtile(qt, gt, row_lse[buf], row_delta[buf], r0);
+    subtile(qt + 32 * S::kPitch, gt + 32 * S::kPitch, row_lse[buf] + 32, row_delta[buf] + 32, r0 + 32);
+  }
+
+  float worst = 0.0f;
+#pragma unroll
+  for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) worst += fabsf(dk[d][r]) + fabsf(dv[d][r]);
+  worst += __shfl_xor(worst, 32, 64);
+  const bool good = finite(worst), mine = j < s.room;
+  const bool to_memory = sink_tile && j < min(p.sinks, s.keys);
+  const int64_t slot = far ? (int64_t)p.n_seq + ((int)blockIdx.x - near_items) : b;
+  float* part = a.sink_part + (slot * p.kv_heads + kv) * 2 * p.sinks * p.dim + (int64_t)(to_memory ? j : 0) * p.dim;
+  const int64_t part_dv = (int64_t)p.sinks * p.dim;
+  T* dk_row = (T*)a.dk + (int64_t)(s.k0 + j) * a.dk_row + kv * a.dk_head;
+  T* dv_row = (T*)a.dv + (int64_t)(s.k0 + j) * a.dv_row + kv * a.dv_head;
+  if (mine && good && (to_memory || !far))
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = 32 * d + 8 * i + 4 * half;
+        if (c >= p.dim) continue;
+        if (to_memory) {
+          *(floatx4*)(part + c) = floatx4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
+          *(floatx4*)(part + part_dv + c) = floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+        } else {
+          Pack<T, 4> x, y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x.v[e] = from_f32<T>(dk[d][4 * i + e] * p.scale);
+            y.v[e] = from_f32<T>(dv[d][4 * i + e]);
+          }
+          x.store(dk_row + c);
+          y.store(dv_row + c);
+        }
+      }
+  uint32_t bad = (uint32_t)__ballot(mine && !good && (to_memory || !far));
+  while (bad) {
+    const int c = __ffs(bad) - 1;
+    bad &= bad - 1;
+    const int jj = __shfl(j, c, 64);
+    float gk[(DP + 63) / 64], gv[(DP + 63) / 64];
+    grad_k_row_again<T, DP>(a, s, kv, jj, __shfl(lo, c, 64), __shfl(hi, c, 64), gk, gv);
+    const bool mem = sink_tile && jj < min(p.sinks, s.keys);
+#pragma unroll
+    for (int i = 0; i < (DP + 63) / 64; ++i) {
+      const int ch = lane + 64 * i;
+      if (ch >= p.dim) continue;
+      if (mem) {
+        float* at = a.sink_part + (slot * p.kv_heads + kv) * 2 * p.sinks * p.dim + (int64_t)jj * p.dim + ch;
+        at[0] = gk[i];
+        at[part_dv] = gv[i];
+      } else {
+        ((T*)a.dk)[(int64_t)(s.k0 + jj) * a.dk_row + kv * a.dk_head + ch] = from_f32<T>(gk[i] * p.scale);
+        ((T*)a.dv)[(int64_t)(s.k0 + jj) * a.dv_row + kv * a.dv_head + ch] = from_f32<T>(gv[i]);
+      }
+    }
+  }
+}
+
+// The sinks' sums: the tile's own, then the far items in order.  Grid: (sinks, kv heads, sequences); threads:
+// (dk, dv) x 128 channels x 4 shares of the items.
+template <typename T>
+__global__ void __launch_bounds__(1024) attention_sink_kernel(AttnArgs a) {
+  __shared__ float shares[4][256];
+  const ocnn_attention_params& p = a.p;
+  const int j = blockIdx.x, kv = blockIdx.y, b = blockIdx.z;
+  const Seq s = sequence(p, b);
+  const FarRange fr = far_tokens(p, s);
+  if (!fr.any || j >= s.keys) return;
+  const int t = threadIdx.x & 255, share = threadIdx.x >> 8, c = t & 127, which = t >> 7;
+  const int64_t one = (int64_t)p.kv_heads * 2 * p.sinks * p.dim;
+  const float* base = a.sink_part + ((int64_t)kv * 2 + which) * p.sinks * p.dim + (int64_t)j * p.dim + c;
+  const int i0 = fr.first / kFarRows, i1 = (s.queries - 1) / kFarRows + 1, each = (i1 - i0 + 3) / 4;
+  const int64_t id0 = (int64_t)p.n_seq + (s.q0 >> Log2<kFarRows>::value) + b;
+  float sum = 0.0f;
+  if (c < p.dim) {
+    if (share == 0) sum = base[(int64_t)b * one];
+    for (int i = i0 + share * each; i < min(i0 + (share + 1) * each, i1); ++i) sum += base[(id0 + i) * one];
+  }
+  shares[share][t] = sum;
+  __syncthreads();
+  if (share || c >= p.dim) return;
+  sum += shares[1][t];
+  sum += shares[2][t];
+  sum += shares[3][t];
+  if (which) ((T*)a.dv)[(int64_t)(s.k0 + j) * a.dv_row + kv * a.dv_head + c] = from_f32<T>(sum);
+  else ((T*)a.dk)[(int64_t)(s.k0 + j) * a.dk_row + kv * a.dk_head + c] = from_f32<T>(sum * p.scale);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+int check_params(const ocnn_attention_params* p) {
+  OCNN_REQUIRE(p, OCNN_E_BADARG, "null pointer");
+  OCNN_REQUIRE(p->dtype == OCNN_F32 || p->dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", p->dtype);
+  OCNN_REQUIRE(p->rows_q >= 0 && p->rows_k >= 0 && p->n_seq >= 1 && p->n_seq <= 65535, OCNN_E_BADARG,
+      "%d queries, %d keys, %d sequences (1 .. 65535)", p->rows_q, p->rows_k, p->n_seq);
+  OCNN_REQUIRE(p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0 && p->kv_heads <= 65535, OCNN_E_SHAPE,
+      "%d query heads over %d key heads", p->heads, p->kv_heads);
+  OCNN_REQUIRE(p->dim > 0 && p->dim <= 128 && p->dim % 8 == 0, OCNN_E_UNSUPPORTED,
+      "%d channels a head: multiples of 8 up to 128", p->dim);
+  OCNN_REQUIRE(p->left >= -1 && p->right >= -1, OCNN_E_BADARG, "window %d, %d: -1 for no bound", p->left, p->right);
+  OCNN_REQUIRE(p->sinks >= 0 && p->sinks <= kMaxSinks, OCNN_E_UNSUPPORTED, "%d sinks: at most %d", p->sinks, kMaxSinks);
+  OCNN_REQUIRE((int64_t)p->rows_q * p->heads < (1ll << 30) && p->rows_k < (1 << 30), OCNN_E_UNSUPPORTED,
+      "%d x %d query rows, %d key rows: at most 2^30", p->rows_q, p->heads, p->rows_k);
+  OCNN_REQUIRE(p->q_offsets && p->k_offsets && (p->rows_q == 0 || p->q) && (p->rows_k == 0 || (p->k && p->v)), OCNN_E_BADARG,
+      "null pointer");
+  return OCNN_OK;
+}
+
+// 16-byte rows: pointers and strides of every row tensor
+int check_rows(int dtype, const char* name, const void* at, int64_t row, int64_t head) {
+  const int64_t piece = dtype == OCNN_F32 ? 4 : 8;
+  OCNN_REQUIRE((uintptr_t)at % 16 == 0 && row % piece == 0 && head % piece == 0, OCNN_E_BADARG,
+      "%s: rows and heads must begin at multiples of 16 bytes", name);
+  return OCNN_OK;
+}
+
+struct Plan { bool few; int splits; int64_t tiles; };
+// few: 32 packed rows a workgroup, where a sequence has that many or fewer on average.  splits: the keys are
+// dealt out where the row tiles leave compute units empty, as long as a workgroup keeps some tiles.
+Plan plan_of(const ocnn_attention_params& p) {
+  Plan n;
+  const int64_t group = p.heads / p.kv_heads, packed = (int64_t)p.rows_q * group;
+  n.few = packed <= 32 * (int64_t)p.n_seq;
+  n.tiles = (packed >> (n.few ? 5 : 7)) + p.n_seq + 1;
+  int64_t keys = p.rows_k / p.n_seq;
+  if (p.left >= 0 && p.right >= 0) keys = std::min<int64_t>(keys, (int64_t)p.left + p.right + p.rows_q / p.n_seq + p.sinks);
+  const int64_t blocks = std::max<int64_t>((packed + (n.few ? 31 : 127)) / (n.few ? 32 : 128), n.few ? p.n_seq : 1) * p.kv_heads;
+  const int64_t most = n.few ? keys / 512 : keys / 1024;
+  n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, 256}));
+  return n;
+}
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+size_t split_bytes(const ocnn_attention_params& p, const Plan& n) {
+  if (n.splits == 1) return 0;
+  const size_t rows = (size_t)n.splits * p.rows_q * p.heads;
+  return round256(rows * p.dim * 4) + round256(rows * 8);
+}
+int64_t far_items(const ocnn_attention_params& p) { return (p.rows_q >> Log2<kFarRows>::value) + p.n_seq + 1; }
+bool has_far(const ocnn_attention_params& p) { return p.sinks > 0 && p.left >= 0 && p.rows_q > 0; }
+size_t sink_bytes(const ocnn_attention_params& p) {
+  return has_far(p) ? (size_t)(p.n_seq + far_items(p)) * p.kv_heads * 2 * p.sinks * p.dim * 4 : 0;
+}
+size_t grad_bytes(const ocnn_attention_params& p) {
+  return round256((size_t)p.rows_q * p.heads * 4) + round256(sink_bytes(p));
+}
+
+AttnArgs args_of(const ocnn_attention_params& p) {
+  AttnArgs a = {};
+  a.p = p;
+  a.p.left = std::min(p.left, 1 << 30);
+  a.p.right = std::min(p.right, 1 << 30);
+  a.group = p.heads / p.kv_heads;
+  a.scale2 = p.scale * kLog2e;
+  return a;
+}
+
+template <typename F> void by_dim(int dim, F f) {
+  if (dim <= 32) f(std::integral_constant<int, 32>());
+  else if (dim <= 64) f(std::integral_constant<int, 64>());
+  else if (dim <= 96) f(std::integral_constant<int, 96>());
+  else f(std::integral_constant<int, 128>());
+}
+
+template <typename T, int DP> void forward_launch(const AttnArgs& a, const Plan& n, hipStream_t s) {
+  const dim3 grid((unsigned)n.tiles, a.p.kv_heads, n.splits);
+  if (n.few) {
+    if (n.splits > 1) attention_kernel<T, DP, 1, true><<<grid, 256, 0, s>>>(a);
+    else attention_kernel<T, DP, 1, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (n.splits > 1) attention_kernel<T, DP, 4, true><<<grid, 256, 0, s>>>(a);
+    else attention_kernel<T, DP, 4, false><<<grid, 256, 0, s>>>(a);
+  }
+  if (n.splits > 1) attention_join_kernel<T><<<blocks_for((int64_t)a.p.rows_q * a.p.heads, 4), 256, 0, s>>>(a);
+}
+
+template <typename T, int DP> void backward_launch(const AttnArgs& a, hipStream_t s) {
+  const ocnn_attention_params& p = a.p;
+  if (p.rows_q > 0) {
+    const int64_t tiles = ((int64_t)p.rows_q * a.group >> 7) + p.n_seq + 1;
+    attention_grad_q_kernel<T, DP><<<dim3((unsigned)tiles, p.kv_heads), 256, 0, s>>>(a);
+  }
+  if (p.rows_k > 0) {
+    const int64_t near_items = (p.rows_k >> 7) + p.n_seq + 1;
+    const int64_t all = near_items + (has_far(p) ? far_items(p) : 0);
+    attention_grad_kv_kernel<T, DP><<<dim3((unsigned)all, p.kv_heads), 256, 0, s>>>(a, (int)near_items);
+    if (has_far(p)) attention_sink_kernel<T><<<dim3(p.sinks, p.kv_heads, p.n_seq), 1024, 0, s>>>(a);
+  }
+}
+
+}  // namespace
+}  // namespace ocnn
+
+using namespace ocnn;
+
+extern "C" {
+
+int ocnn_attention_workspace_bytes(const ocnn_attention_params* params, size_t* workspace_bytes, size_t* grad_workspace_bytes) {
+  int rc = check_params(params);
+  if (rc) return rc;
+  if (workspace_bytes) *workspace_bytes = split_bytes(*params, plan_of(*params));
+  if (grad_workspace_bytes) *grad_workspace_bytes = grad_bytes(*params);
+  return OCNN_OK;
+}
+
+int ocnn_octree_attention(void* out, int64_t out_row, int64_t out_head, float* lse, const ocnn_attention_params* params,
+    int fill_rest, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream) {
+  int rc = check_params(params);
+  if (rc) return rc;
+  const ocnn_attention_params& p = *params;
+  if (p.rows_q == 0) return OCNN_OK;
+  OCNN_REQUIRE(out, OCNN_E_BADARG, "null pointer");
+  if ((rc = check_rows(p.dtype, "q", p.q, p.q_row, p.q_head)) || (rc = check_rows(p.dtype, "k", p.k, p.k_row, p.k_head)) ||
+      (rc = check_rows(p.dtype, "v", p.v, p.v_row, p.v_head)) || (rc = check_rows(p.dtype, "out", out, out_row, out_head)))
+    return rc;
+  const Plan n = plan_of(p);
+  const size_t need = split_bytes(p, n);
+  OCNN_REQUIRE(need == 0 || (workspace_dev && workspace_bytes >= need && (uintptr_t)workspace_dev % 16 == 0), OCNN_E_WORKSPACE,
+      "octree_attention needs %zu bytes, 16-byte aligned, got %zu", need, workspace_bytes);
+  AttnArgs a = args_of(p);
+  a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.fill = fill_rest != 0;
+  a.splits = n.splits;
+  if (n.splits > 1) {
+    a.part_o = (float*)workspace_dev;
+    a.part_ml = (float*)((char*)workspace_dev + round256((size_t)n.splits * p.rows_q * p.heads * p.dim * 4));
+  }
+  hipStream_t s = as_stream(stream);
+  by_dim(p.dim, [&](auto d) {
+    if (p.dtype == OCNN_F32) forward_launch<float, d.value>(a, n, s);
+    else forward_launch<uint16_t, d.value>(a, n, s);
+  });
+  OCNN_LAUNCH_OK("octree_attention");
+  return OCNN_OK;
+}
+
+int ocnn_octree_attention_grad(void* grad_q, int64_t grad_q_row, int64_t grad_q_head, void* grad_k, int64_t grad_k_row,
+    int64_t grad_k_head, void* grad_v, int64_t grad_v_row, int64_t grad_v_head, const void* grad_out, int64_t grad_out_row,
+    int64_t grad_out_head, const void* out, int64_t out_row, int64_t out_head, const float* lse,
+    const ocnn_attention_params* params, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream) {
+  int rc = check_params(params);
+  if (rc) return rc;
+  const ocnn_attention_params& p = *params;
+  if (p.rows_q == 0 && p.rows_k == 0) return OCNN_OK;
+  OCNN_REQUIRE((p.rows_q == 0 || (grad_q && grad_out && out && lse)) && (p.rows_k == 0 || (grad_k && grad_v)), OCNN_E_BADARG,
+      "null pointer");
+  if ((rc = check_rows(p.dtype, "q", p.q, p.q_row, p.q_head)) || (rc = check_rows(p.dtype, "k", p.k, p.k_row, p.k_head)) ||
+      (rc = check_rows(p.dtype, "v", p.v, p.v_row, p.v_head)) || (rc = check_rows(p.dtype, "out", out, out_row, out_head)) ||
+      (rc = check_rows(p.dtype, "grad_out", grad_out, grad_out_row, grad_out_head)) ||
+      (rc = check_rows(p.dtype, "grad_q", grad_q, grad_q_row, grad_q_head)) ||
+      (rc = check_rows(p.dtype, "grad_k", grad_k, grad_k_row, grad_k_head)) ||
+      (rc = check_rows(p.dtype, "grad_v", grad_v, grad_v_row, grad_v_head)))
+    return rc;
+  const size_t need = grad_bytes(p);
+  OCNN_REQUIRE(need == 0 || (workspace_dev && workspace_bytes >= need && (uintptr_t)workspace_dev % 16 == 0), OCNN_E_WORKSPACE,
+      "octree_attention_grad needs %zu bytes, 16-byte aligned, got %zu", need, workspace_bytes);
+  AttnArgs a = args_of(p);
+  a.dq = grad_q; a.dq_row = grad_q_row; a.dq_head = grad_q_head;
+  a.dk = grad_k; a.dk_row = grad_k_row; a.dk_head = grad_k_head;
+  a.dv = grad_v; a.dv_row = grad_v_row; a.dv_head = grad_v_head;
+  a.grad = grad_out; a.grad_row = grad_out_row; a.grad_head = grad_out_head;
+  a.fwd = out; a.fwd_row = out_row; a.fwd_head = out_head;
+  a.lse = const_cast<float*>(lse);
+  a.delta = (float*)workspace_dev;
+  a.sink_part = (float*)((char*)workspace_dev + round256((size_t)p.rows_q * p.heads * 4));
+  hipStream_t s = as_stream(stream);
+  by_dim(p.dim, [&](auto d) {
+    if (p.dtype == OCNN_F32) backward_launch<float, d.value>(a, s);
+    else backward_launch<uint16_t, d.value>(a, s);
+  });
+  OCNN_LAUNCH_OK("octree_attention_grad");
+  return OCNN_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,769 @@
+// Operators along the node order of an octree level.  A level of a batched octree is one sequence
+// per octree (its nodes in Morton order, octree after octree, octree/octree/merge_octrees.cpp:114-198);
+// `offsets` (int32 [n_seq + 1], device) says where each begins.
+//   * octree_offsets: those offsets, from the keys of the level
+//   * rotary positions with several axes
+//   * the gated linear recurrence and its gradient
+// Tensors are row-major (a row is a node), so consecutive lanes hold consecutive channels.
+#include "sequence.h"
+
+namespace ocnn {
+namespace {
+
+// ---- octree_offsets ---------------------------------------------------------------------------------
+// The octree index is the top 16 bits of a key in both key forms, and the keys of a level are sorted by
+// it: offsets[b] = the first node with index >= b.  Over the non-empty nodes it is that node's rank,
+// i.e. the child entry of the first non-empty node from there on.  One wavefront per octree.
+__global__ void octree_offsets_kernel(int* __restrict__ offsets, const uint64_t* __restrict__ key,
+    const int* __restrict__ child, int nnum, int nnum_nempty, int batch, int nempty) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  int lo = 0, hi = nnum;
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if ((int)(key[mid] >> 48) < b) lo = mid + 1; else hi = mid;
+  }
+  if (b >= batch) lo = nnum;
+  int out = nempty ? nnum_nempty : lo;
+  if (nempty) {
+    for (int at = lo; at < nnum; at += 64) {
+      const int c = at + lane < nnum ? child[at + lane] : -1;
+      const uint64_t live = __ballot(c >= 0);
+      if (live) { out = __shfl(c, __ffsll((unsigned long long)live) - 1, 64); break; }
+    }
+  }
+  if (lane == 0) offsets[b] = out;
+}
+
+// ---- rotary positions -----------------------------------------------------------------------------
+// Pair p of channels belongs to one axis and turns by t = position[axis] * frequency[p]:
+//   (x, y) -> (x cos t - y sin t, x sin t + y cos t);  the inverse turns by -t (the gradient).
+// The angle is formed in 64 bits and reduced to a fraction of a turn before it is rounded to 32: at
+// position 2^20 a 32-bit product is off by 2^-5 rad, the fraction by 2^-25 of a turn.  One angle
+// serves all heads of a row, so the sines (a 64-bit product, a reduction and a polynomial) are computed
+// once a row into LDS and the streaming part is two fused multiply-adds per channel: bound by HBM.
+// A thread takes 16 bytes of the first channels of V pairs and 16 of the second ones (interleaved: 32
+// neighbouring bytes) and writes them back in the same places, so `out` may be `data`.
+constexpr int kRotaryAngles = 2048;   // (rows of a workgroup) x (pairs): 16 KiB of LDS
+
+struct RotaryArgs {
+  void* out; const void* data;
+  int64_t out_row, out_head, row, head;
+  const void* pos; int64_t pos_row;
+  const double* freq;
+  int rows, heads, dim, pairs, axis_end[3], block_rows, items_head, pair_items, copy;
+  uint32_t div_pairs, div_row, div_head;   // reciprocals: see fast_div
+  int inverse;
+};
+
+// n / d for n * d < 2^32, by a multiplication with m = floor(2^32 / d) + 1 (m = 0 stands for d = 1)
+__device__ inline uint32_t fast_div(uint32_t n, uint32_t m) { return m ? __umulhi(n, m) : n; }
+
+template <int KIND> __device__ inline double rotary_position(const void* pos, int64_t row, int64_t stride, int axis) {
+  if (KIND == OCNN_POS_INT32) return (double)((const int*)pos)[row * stride + axis];
+  if (KIND == OCNN_POS_F32) return (double)((const float*)pos)[row * stride + axis];
+  return (double)(int)((((const uint64_t*)pos)[row] >> (16 * axis)) & 0xffffu);
+}
+
+template <typename T, int KIND, bool INTERLEAVED>
+__global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryArgs a) {
+  constexpr int V = 16 / (int)sizeof(T);
+  __shared__ float2 turn[kRotaryAngles];
+  const int64_t row0 = (int64_t)blockIdx.x * a.block_rows;
+  const int rows = (int)min((int64_t)a.block_rows, (int64_t)a.rows - row0);
+  for (int i = threadIdx.x; i < rows * a.pairs; i += kBlock) {
+    const int r = (int)fast_div((uint32_t)i, a.div_pairs), p = i - r * a.pairs;
+    const int axis = (p >= a.axis_end[0]) + (p >= a.axis_end[1]) + (p >= a.axis_end[2]);
+    double t = rotary_position<KIND>(a.pos, row0 + r, a.pos_row, axis) * a.freq[p] * 0.15915494309189535;
+    t -= rint(t);
+    float s, c;
+    sincospif(2.0f * (float)t, &s, &c);
+    turn[i] = make_float2(c, a.inverse ? -s : s);
+  }
+  __syncthreads();
+  const int items_row = a.heads * a.items_head;
+  const T* data = (const T*)a.data + row0 * a.row;
+  T* out = (T*)a.out + row0 * a.out_row;
+  for (int i = threadIdx.x; i < rows * items_row; i += kBlock) {
+    const int r = (int)fast_div((uint32_t)i, a.div_row), in_row = i - r * items_row;
+    const int h = (int)fast_div((uint32_t)in_row, a.div_head), item = in_row - h * a.items_head;
+    const T* src = data + (int64_t)r * a.row + (int64_t)h * a.head;
+    T* dst = out + (int64_t)r * a.out_row + (int64_t)h * a.out_head;
+    if (item >= a.pair_items) {                       // channels that carry no position
+      const int c = 2 * a.pairs + (item - a.pair_items) * V, n = min(V, a.dim - c);
+      if (n == V) { Pack<T, V> x; x.load(src + c); x.store(dst + c); }
+      else for (int j = 0; j < n; ++j) dst[c + j] = src[c + j];
+      continue;
+    }
+    const int p = item * V, n = min(V, a.pairs - p);
+    const float2* cs = turn + r * a.pairs + p;
+    const int c0 = INTERLEAVED ? 2 * p : p, c1 = INTERLEAVED ? 2 * p + V : a.pairs + p;
+    Pack<T, V> u, w;
+    if (n == V) {
+      u.load(src + c0);
+      w.load(src + c1);
+    } else {
+      u.fill(0);
+      w.fill(0);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if ((INTERLEAVED ? j < 2 * n : j < n)) u.v[j] = src[c0 + j];
+        if ((INTERLEAVED ? j + V < 2 * n : j < n)) w.v[j] = src[c1 + j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 k = j < n ? cs[j] : make_float2(1.0f, 0.0f);
+      T& first = INTERLEAVED ? (2 * j < V ? u.v[(2 * j) % V] : w.v[(2 * j) % V]) : u.v[j];
+      T& second = INTERLEAVED ? (2 * j < V ? u.v[(2 * j + 1) % V] : w.v[(2 * j + 1) % V]) : w.v[j];
+      const float x = to_f32(first), y = to_f32(second);
+      first = from_f32<T>(fmaf(x, k.x, -(y * k.y)));
+      second = from_f32<T>(fmaf(x, k.y, y * k.x));
+    }
+    if (n == V) {
+      u.store(dst + c0);
+      w.store(dst + c1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if ((INTERLEAVED ? j < 2 * n : j < n)) dst[c0 + j] = u.v[j];
+        if ((INTERLEAVED ? j + V < 2 * n : j < n)) dst[c1 + j] = w.v[j];
+      }
+    }
+  }
+}
+
+uint32_t reciprocal(uint32_t d) { return d <= 1 ? 0u : (uint32_t)((1ull << 32) / d) + 1u; }
+
+// ---- gated linear recurrence ----------------------------------------------------------------------
+//   h_t = a_t h_{t-1} + b_t x_t,  a = sigmoid(g), b = 1 - a = sigmoid(-g)
+// The map of a run of rows is (A, H): h -> A h + H, and runs compose.  Three launches:
+//   run    every chunk of L rows of a sequence: its (A, H)           reads g, x
+//   carry  per sequence: the state in front of each chunk            reads and writes 8 bytes / L rows
+//   apply  every chunk again from its state: h                       reads g, x, writes h
+// The chunks' states are folded in a fixed order, so results do not change from run to run (a
+// single pass that takes whatever prefix its predecessors have published would not give that).
+// Threads enumerate (chunk, channels) with the channels innermost.  The state is 32 bits throughout.
+// Sequences of a few rows (a step of a running sequence) take one launch, a thread per (sequence,
+// channels) that walks the rows.
+//
+// The gradient, with L_t = dh_t + a_{t+1} L_{t+1} (L_end += the gradient of the last state):
+//   dx = b L,  dg = a b L (h_{t-1} - x),  d state = a_1 L_1
+// runs the same three steps from the other end on (a, dh).  h_{t-1} is computed again from the
+// chunk's state (kept from the forward pass, 32 bits): the stored h of a bf16 call is rounded, and
+// h_{t-1} - x cancels where a sequence hardly changes.
+
+template <typename T> __device__ inline void gates(float g, float* a, float* b);
+// sigmoid(g) and sigmoid(-g) without cancellation: e = exp(-|g|), 1 / (1 + e) and e / (1 + e).  The fp32
+// form carries the rounding error of g * log2(e), 2^-24 |g| / ln 2 of the result, as a factor.
+template <> __device__ inline void gates<float>(float g, float* a, float* b) {
+  const float x = -fabsf(g), t = x * 1.44269502f;
+  const float lost = fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;
+  float e = __builtin_amdgcn_exp2f(t);
+  e = (x > -100.0f) ? fmaf(e, lost * 0.693147182f, e) : (x == x ? 0.0f : x);
+  const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+  *a = g >= 0.0f ? big : small;
+  *b = g >= 0.0f ? small : big;
+}
+template <> __device__ inline void gates<uint16_t>(float g, float* a, float* b) {
+  const float e = __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269502f);   // |g| < 100: 2^-17 of the result at most
+  const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+  *a = g >= 0.0f ? big : small;
+  *b = g >= 0.0f ? small : big;
+}
+
+struct ScanArgs {
+  void* out; const void* gate; const void* data; const void* grad;      // grad: of the outputs
+  void* grad_gate; void* grad_data;
+  int64_t out_row, gate_row, data_row, grad_row, grad_gate_row, grad_data_row;
+  const float* state; float* last; const float* grad_last; float* grad_state;
+  float* run_a; float* run_h; float* carry;      // [ids][channels]
+  const int* offsets;
+  int n_seq, rows, channels, groups, reverse, fill;
+  int64_t threads;                                // ids x groups
+};
+
+constexpr int kScanRows = 8;   // rows whose loads are in flight together
+
+// The rows of chunk `id`: their sequence, where they begin and how many there are.
+struct Chunk {
+  int seq, index, first, count, length;   // row of step j: first + j * step
+  int step;
+  bool live;                              // false: beyond its sequence
+};
+
+template <int L> __device__ inline Chunk chunk_of(const ScanArgs& a, int64_t id) {
+  Chunk c;
+  c.seq = locate(a.offsets, a.n_seq, a.rows, id, Log2<L>::value);
+  const int begin = clamped(a.offsets, c.seq, a.rows);
+  const int end = c.seq < a.n_seq ? clamped(a.offsets, c.seq + 1, a.rows) : a.rows;
+  c.length = max(end - begin, 0);
+  const int64_t index = id - ((begin >> Log2<L>::value) + c.seq);
+  const int64_t at = index * L;
+  c.live = index >= 0 && (at < c.length || (index == 0 && c.seq < a.n_seq));
+  c.index = (int)index;
+  c.count = c.live ? (int)min((int64_t)L, c.length - at) : 0;
+  c.step = a.reverse ? -1 : 1;
+  c.first = a.reverse ? end - 1 - (int)at : begin + (int)at;
+  return c;
+}
+
+// ids whose chunk is the first one of its sequence's chunk ids
+__device__ inline int64_t first_id(const ScanArgs& a, int seq, int shift) {
+  return (int64_t)(clamped(a.offsets, seq, a.rows) >> shift) + seq;
+}
+
+template <typename T, int V, int L>
+__global__ void __launch_bounds__(kBlock) scan_run_kernel(ScanArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= a.threads) return;
+  const int64_t id = i / a.groups;
+  const int c0 = (int)(i - id * a.groups) * V;
+  const Chunk ch = chunk_of<L>(a, id);
+  // (the run of a sequence's last chunk is not needed by anything)
+  if (!ch.live || ch.seq >= a.n_seq || (int64_t)(ch.index + 1) * L >= ch.length) return;
+  const T* gate = (const T*)a.gate + c0;
+  const T* data = (const T*)a.data + c0;
+  float A[V], H[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) { A[v] = 1.0f; H[v] = 0.0f; }
+  for (int t = 0; t < L; t += kScanRows) {       // the chunk is full: it is not its sequence's last
+    Pack<T, V> g[kScanRows], x[kScanRows];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j) {
+      const int64_t row = ch.first + (int64_t)(t + j) * ch.step;
+      g[j].load(gate + row * a.gate_row);
+      x[j].load(data + row * a.data_row);
+    }
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float p, q;
+        gates<T>(to_f32(g[j].v[v]), &p, &q);
+        H[v] = fmaf(p, H[v], q * to_f32(x[j].v[v]));
+        A[v] *= p;
+      }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    a.run_a[id * a.channels + c0 + v] = A[v];
+    a.run_h[id * a.channels + c0 + v] = H[v];
+  }
+}
+
+// The same from the other end for the gradient: m = a (dh + m'), m' from the row behind.  Runs of the chunks
+// behind a sequence's first one.
+template <typename T, int V, int L>
+__global__ void __launch_bounds__(kBlock) scan_run_back_kernel(ScanArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= a.threads) return;
+  const int64_t id = i / a.groups;
+  const int c0 = (int)(i - id * a.groups) * V;
+  const Chunk ch = chunk_of<L>(a, id);
+  if (!ch.live || ch.seq >= a.n_seq || ch.index == 0) return;
+  const T* gate = (const T*)a.gate + c0;
+  const T* grad = (const T*)a.grad + c0;
+  float A[V], M[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) { A[v] = 1.0f; M[v] = 0.0f; }
+  for (int t = L - kScanRows; t >= 0; t -= kScanRows) {
+    if (t >= ch.count) continue;
+    Pack<T, V> g[kScanRows], d[kScanRows];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j) {
+      const int64_t row = ch.first + (int64_t)min(t + j, ch.count - 1) * ch.step;
+      g[j].load(gate + row * a.gate_row);
+      d[j].load(grad + row * a.grad_row);
+    }
+#pragma unroll
+    for (int j = kScanRows - 1; j >= 0; --j)
+      if (t + j < ch.count)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float p, q;
+          gates<T>(to_f32(g[j].v[v]), &p, &q);
+          M[v] = p * (to_f32(d[j].v[v]) + M[v]);
+          A[v] *= p;
+        }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    a.run_a[id * a.channels + c0 + v] = A[v];
+    a.run_h[id * a.channels + c0 + v] = M[v];
+  }
+}
+
+// The state in front of each chunk of a sequence: kSegments threads a channel fold a share of the runs
+// each, the shares are folded in order, and each thread walks its share again writing the states.
+// A workgroup serves 16 channels of one sequence.
+constexpr int kCarryChannels = 16, kSegments = 64;
+
+template <int SHIFT, bool BACK>
+__global__ void __launch_bounds__(kCarryChannels * kSegments) scan_carry_kernel(ScanArgs a) {
+  __shared__ float sa[kSegments][kCarryChannels], sh[kSegments][kCarryChannels];
+  const int seq = blockIdx.y, lane = threadIdx.x % kCarryChannels, seg = threadIdx.x / kCarryChannels;
+  const int c = blockIdx.x * kCarryChannels + lane;
+  const int begin = clamped(a.offsets, seq, a.rows), end = clamped(a.offsets, seq + 1, a.rows);
+  const int chunks = (max(end - begin, 0) + (1 << SHIFT) - 1) >> SHIFT;
+  if (chunks < 2) return;                       // its only chunk starts from the caller's state
+  const int64_t id0 = first_id(a, seq, SHIFT);
+  const int share = (chunks + kSegments - 1) / kSegments;
+  const int from = min(seg * share, chunks), to = min(from + share, chunks);
+  // chunk j in the order of the walk; the run of the walk's last chunk does not exist
+  auto at = [&](int j) { return (id0 + (BACK ? chunks - 1 - j : j)) * a.channels + c; };
+  float A = 1.0f, H = 0.0f;
+  if (c < a.channels)
+    for (int j = from; j < min(to, chunks - 1); ++j) {
+      const float ra = a.run_a[at(j)], rh = a.run_h[at(j)];
+      H = fmaf(ra, H, rh);
+      A *= ra;
+    }
+  sa[seg][lane] = A;
+  sh[seg][lane] = H;
+  __syncthreads();
+  if (c >= a.channels) return;
+  const float* start = BACK ? a.grad_last : a.state;
+  float h = start ? start[(int64_t)seq * a.channels + c] : 0.0f;
+  for (int s = 0; s < seg; ++s) h = fmaf(sa[s][lane], h, sh[s][lane]);
+  float* carry = BACK ? a.run_h : a.carry;       // (back: in place, a share is read before it is written)
+  for (int j = from; j < to; ++j) {
+    float ra = 0.0f, rh = 0.0f;
+    if (j < chunks - 1) { ra = a.run_a[at(j)]; rh = a.run_h[at(j)]; }
+    carry[at(j)] = h;
+    h = fmaf(ra, h, rh);
+  }
+}
+
+template <typename T, int V> __device__ inline void zero_rows(T* out, int64_t row_stride, const Chunk& ch) {
+  Pack<T, V> z;
+  z.fill(0);
+  for (int j = 0; j < ch.count; ++j) z.store(out + (ch.first + (int64_t)j * ch.step) * row_stride);
+}
+
+template <typename T, int V, int L>
+__global__ void __launch_bounds__(kBlock) scan_apply_kernel(ScanArgs a) {
+  const int64_t i = a.threads - 1 - ((int64_t)blockIdx.x * kBlock + threadIdx.x);   // last chunk first: its rows were read last
+  if (i < 0) return;
+  const int64_t id = i / a.groups;
+  const int c0 = (int)(i - id * a.groups) * V;
+  const Chunk ch = chunk_of<L>(a, id);
+  if (!ch.live) return;
+  T* out = (T*)a.out + c0;
+  if (ch.seq >= a.n_seq) {
+    if (a.fill) zero_rows<T, V>(out, a.out_row, ch);
+    return;
+  }
+  const T* gate = (const T*)a.gate + c0;
+  const T* data = (const T*)a.data + c0;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    h[v] = ch.index ? a.carry[id * a.channels + c0 + v]
+                    : a.state ? a.state[(int64_t)ch.seq * a.channels + c0 + v] : 0.0f;
+  for (int t = 0; t < ch.count; t += kScanRows) {
+    Pack<T, V> g[kScanRows], x[kScanRows];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j) {
+      const int64_t row = ch.first + (int64_t)min(t + j, ch.count - 1) * ch.step;
+      g[j].load(gate + row * a.gate_row);
+      x[j].load(data + row * a.data_row);
+    }
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j)
+      if (t + j < ch.count) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float p, q;
+          gates<T>(to_f32(g[j].v[v]), &p, &q);
+          h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
+          x[j].v[v] = from_f32<T>(h[v]);
+        }
+        x[j].store(out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row);
+      }
+  }
+  if (a.last && (int64_t)(ch.index + 1) * L >= ch.length)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.last[(int64_t)ch.seq * a.channels + c0 + v] = h[v];
+}
+
+// d gate, d data of a chunk: forward over the chunk once for the state in front of every kScanRows rows,
+// then group by group from the end.
+template <typename T, int V, int L>
+__global__ void __launch_bounds__(kBlock) scan_apply_back_kernel(ScanArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= a.threads) return;
+  const int64_t id = i / a.groups;
+  const int c0 = (int)(i - id * a.groups) * V;
+  const Chunk ch = chunk_of<L>(a, id);
+  if (!ch.live) return;
+  T* dgate = (T*)a.grad_gate + c0;
+  T* ddata = (T*)a.grad_data + c0;
+  if (ch.seq >= a.n_seq) {
+    zero_rows<T, V>(dgate, a.grad_gate_row, ch);
+    zero_rows<T, V>(ddata, a.grad_data_row, ch);
+    return;
+  }
+  const T* gate = (const T*)a.gate + c0;
+  const T* data = (const T*)a.data + c0;
+  const T* grad = (const T*)a.grad + c0;
+  constexpr int kGroups = L / kScanRows;
+  float front[kGroups][V], m[V];
+  const int64_t at_seq = (int64_t)ch.seq * a.channels + c0;
+  const bool is_last = (int64_t)(ch.index + 1) * L >= ch.length;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    h[v] = ch.index ? a.carry[id * a.channels + c0 + v] : a.state ? a.state[at_seq + v] : 0.0f;
+    m[v] = !is_last ? a.run_h[id * a.channels + c0 + v] : a.grad_last ? a.grad_last[at_seq + v] : 0.0f;
+  }
+#pragma unroll
+  for (int s = 0; s < kGroups; ++s) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) front[s][v] = h[v];
+    if (s + 1 < kGroups && (s + 1) * kScanRows < ch.count) {     // (a whole group)
+      Pack<T, V> g[kScanRows], x[kScanRows];
+#pragma unroll
+      for (int j = 0; j < kScanRows; ++j) {
+        const int64_t row = ch.first + (int64_t)(s * kScanRows + j) * ch.step;
+        g[j].load(gate + row * a.gate_row);
+        x[j].load(data + row * a.data_row);
+      }
+#pragma unroll
+      for (int j = 0; j < kScanRows; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float p, q;
+          gates<T>(to_f32(g[j].v[v]), &p, &q);
+          h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
+        }
+    }
+  }
+#pragma unroll
+  for (int s = kGroups - 1; s >= 0; --s) {
+    const int t = s * kScanRows;
+    if (t >= ch.count) continue;
+    Pack<T, V> g[kScanRows], x[kScanRows], d[kScanRows];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j) {
+      const int64_t row = ch.first + (int64_t)min(t + j, ch.count - 1) * ch.step;
+      g[j].load(gate + row * a.gate_row);
+      x[j].load(data + row * a.data_row);
+      d[j].load(grad + row * a.grad_row);
+    }
+    float p[kScanRows][V], q[kScanRows][V], before[kScanRows][V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = front[s][v];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        gates<T>(to_f32(g[j].v[v]), &p[j][v], &q[j][v]);
+        before[j][v] = h[v];
+        h[v] = fmaf(p[j][v], h[v], q[j][v] * to_f32(x[j].v[v]));
+      }
+#pragma unroll
+    for (int j = kScanRows - 1; j >= 0; --j)
+      if (t + j < ch.count) {
+        Pack<T, V> og, ox;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float lam = to_f32(d[j].v[v]) + m[v];
+          og.v[v] = from_f32<T>(p[j][v] * q[j][v] * lam * (before[j][v] - to_f32(x[j].v[v])));
+          ox.v[v] = from_f32<T>(q[j][v] * lam);
+          m[v] = p[j][v] * lam;
+        }
+        const int64_t row = ch.first + (int64_t)(t + j) * ch.step;
+        og.store(dgate + row * a.grad_gate_row);
+        ox.store(ddata + row * a.grad_data_row);
+      }
+  }
+  if (a.grad_state && ch.index == 0)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.grad_state[at_seq + v] = m[v];
+}
+
+// One launch for sequences of a few rows: a thread walks the rows of one sequence (and, behind the last
+// sequence, zeroes the rows that belong to none).
+template <typename T, int V>
+__global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (i >= a.threads) return;
+  const int seq = (int)(i / a.groups);
+  const int c0 = (int)(i - (int64_t)seq * a.groups) * V;
+  const int begin = clamped(a.offsets, seq, a.rows);
+  const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows;
+  T* out = (T*)a.out + c0;
+  Chunk ch;
+  ch.count = max(end - begin, 0);
+  ch.first = seq < a.n_seq && a.reverse ? end - 1 : begin;
+  ch.step = seq < a.n_seq && a.reverse ? -1 : 1;
+  if (seq >= a.n_seq) {
+    if (a.fill) zero_rows<T, V>(out, a.out_row, ch);
+    return;
+  }
+  const T* gate = (const T*)a.gate + c0;
+  const T* data = (const T*)a.data + c0;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = a.state ? a.state[(int64_t)seq * a.channels + c0 + v] : 0.0f;
+  for (int t = 0; t < ch.count; t += kScanRows) {
+    Pack<T, V> g[kScanRows], x[kScanRows];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j) {
+      const int64_t row = ch.first + (int64_t)min(t + j, ch.count - 1) * ch.step;
+      g[j].load(gate + row * a.gate_row);
+      x[j].load(data + row * a.data_row);
+    }
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j)
+      if (t + j < ch.count) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float p, q;
+          gates<T>(to_f32(g[j].v[v]), &p, &q);
+          h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
+          x[j].v[v] = from_f32<T>(h[v]);
+        }
+        x[j].store(out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row);
+      }
+  }
+  if (a.last)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.last[(int64_t)seq * a.channels + c0 + v] = h[v];
+}
+
+// Rows of a chunk: 64 where that leaves enough threads for the chip, else 16.  The rule sees sizes that the
+// forward and the backward call share, so their chunks are the same.
+int scan_shift(int64_t rows, int64_t channels) { return rows * channels >= (int64_t)1 << 22 ? 6 : 4; }
+
+int64_t scan_ids(int64_t rows, int n_seq, int shift) { return (rows >> shift) + n_seq + 1; }
+
+// V channels a thread: wide loads where every row allows them and the chip stays full
+int scan_width(const ScanArgs& a, int size, std::initializer_list<std::pair<const void*, int64_t>> tensors, int64_t ids) {
+  int v = 4;
+  for (; v > 1; v >>= 1) {
+    bool ok = a.channels % v == 0 && ids * (a.channels / v) >= 256 * 256;
+    for (auto& t : tensors) ok = ok && t.second % v == 0 && (uintptr_t)t.first % (size_t)(v * size) == 0;
+    if (ok) break;
+  }
+  return v;
+}
+
+template <typename T, int V, int L>
+void scan_forward_launch(const ScanArgs& a, hipStream_t s) {
+  const unsigned blocks = blocks_for(a.threads);
+  scan_run_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
+  scan_carry_kernel<Log2<L>::value, false><<<dim3((a.channels + kCarryChannels - 1) / kCarryChannels, a.n_seq),
+      kCarryChannels * kSegments, 0, s>>>(a);
+  scan_apply_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
+}
+
+template <typename T, int V, int L>
+void scan_backward_launch(const ScanArgs& a, hipStream_t s) {
+  const unsigned blocks = blocks_for(a.threads);
+  scan_run_back_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
+  scan_carry_kernel<Log2<L>::value, true><<<dim3((a.channels + kCarryChannels - 1) / kCarryChannels, a.n_seq),
+      kCarryChannels * kSegments, 0, s>>>(a);
+  scan_apply_back_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
+}
+
+template <typename F> void by_width(int v, F f) {
+  if (v == 4) f(std::integral_constant<int, 4>());
+  else if (v == 2) f(std::integral_constant<int, 2>());
+  else f(std::integral_constant<int, 1>());
+}
+
+}  // namespace
+}  // namespace ocnn
+
+using namespace ocnn;
+
+extern "C" {
+
+int ocnn_octree_offsets(int* offsets, const void* octree_dev, const void* info, int depth, int nempty,
+    ocnn_stream_t stream) {
+  OCNN_REQUIRE(offsets && octree_dev && info, OCNN_E_BADARG, "null pointer");
+  int rc = ocnn_info_check(info);
+  if (rc) return rc;
+  const Info* in = as_info(info);
+  OCNN_REQUIRE(depth >= 1 && depth <= in->depth, OCNN_E_BADARG, "depth %d outside 1 .. %d", depth, in->depth);
+  OCNN_REQUIRE(in->has(OCNN_KEY) && in->channel(OCNN_KEY) == 1 && in->location(OCNN_KEY) == -1, OCNN_E_UNSUPPORTED,
+      "the octree holds no 64-bit key per node");
+  OCNN_REQUIRE(!nempty || in->has(OCNN_CHILD), OCNN_E_FORMAT, "the octree holds no children");
+  const char* blob = (const char*)octree_dev;
+  octree_offsets_kernel<<<in->batch_size + 1, 64, 0, as_stream(stream)>>>(offsets,
+      (const uint64_t*)(blob + in->ptr_dis(OCNN_KEY, depth)),
+      nempty ? (const int*)(blob + in->ptr_dis(OCNN_CHILD, depth)) : nullptr, in->nnum[depth], in->nnum_nempty[depth],
+      in->batch_size, nempty != 0);
+  OCNN_LAUNCH_OK("octree_offsets");
+  return OCNN_OK;
+}
+
+int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void* data, int64_t row, int64_t head,
+    int rows, int heads, int dim, const void* positions, int position_kind, int64_t position_row,
+    const double* frequencies, const int* pairs, int axes, int interleaved, int inverse, int dtype,
+    ocnn_stream_t stream) {
+  OCNN_REQUIRE(rows >= 0 && heads > 0 && dim > 0, OCNN_E_BADARG, "rows %d, heads %d, dim %d", rows, heads, dim);
+  OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
+  OCNN_REQUIRE(position_kind >= OCNN_POS_INT32 && position_kind <= OCNN_POS_XYZ, OCNN_E_BADARG, "position kind %d",
+      position_kind);
+  OCNN_REQUIRE(pairs && axes >= 1 && axes <= 4 && (position_kind != OCNN_POS_XYZ || axes <= 3), OCNN_E_BADARG,
+      "%d axes: at most 4 (3 with packed coordinates)", axes);
+  int64_t total = 0;
+  int ends[4] = {0, 0, 0, 0};
+  for (int i = 0; i < 4; ++i) {
+    if (i < axes) {
+      OCNN_REQUIRE(pairs[i] >= 0, OCNN_E_BADARG, "axis %d: %d pairs", i, pairs[i]);
+      total += pairs[i];
+    }
+    ends[i] = i < axes ? (int)(total > 2048 ? 2048 : total) : 1 << 30;
+  }
+  for (int i = axes - 1; i < 4; ++i) ends[i] = 1 << 30;       // the last axis is open
+  OCNN_REQUIRE(2 * total <= dim, OCNN_E_SHAPE, "%lld pairs need %lld channels, a head has %d", (long long)total,
+      (long long)(2 * total), dim);
+  OCNN_REQUIRE(dim <= 1024 && heads <= 1024, OCNN_E_UNSUPPORTED, "%d heads of %d channels: at most 1024 of 1024", heads, dim);
+  if (rows == 0) return OCNN_OK;
+  OCNN_REQUIRE(out && data && (total == 0 || (positions && frequencies)), OCNN_E_BADARG, "null pointer");
+  const int size = dtype == OCNN_F32 ? 4 : 2, V = 16 / size;
+  RotaryArgs a = {};
+  a.out = out; a.data = data; a.out_row = out_row; a.out_head = out_head; a.row = row; a.head = head;
+  a.pos = positions; a.pos_row = position_row; a.freq = frequencies;
+  a.rows = rows; a.heads = heads; a.dim = dim; a.pairs = (int)total;
+  for (int i = 0; i < 3; ++i) a.axis_end[i] = ends[i];
+  a.pair_items = (a.pairs + V - 1) / V;
+  const bool in_place = out == data && out_row == row && out_head == head;
+  a.items_head = a.pair_items + (in_place ? 0 : (dim - 2 * a.pairs + V - 1) / V);
+  if (a.items_head == 0) return OCNN_OK;
+  const int items = heads * a.items_head;
+  // rows of a workgroup: about 1024 items of 32 bytes (60001 rows of 12 x 48 channels bf16), fewer where that
+  // would leave compute units without work
+  int r = 1024 / items;
+  r = r < 1 ? 1 : r > 16 ? 16 : r;
+  while (r > 1 && rows / r < 2048) r >>= 1;
+  if (a.pairs && r > kRotaryAngles / a.pairs) r = kRotaryAngles / a.pairs;
+  a.block_rows = r;
+  a.div_pairs = reciprocal(a.pairs); a.div_row = r == 1 ? 1u : reciprocal(items);   // (1: every item is of row 0)
+  a.div_head = reciprocal(a.items_head);
+  a.inverse = inverse != 0;
+  const unsigned blocks = blocks_for(rows, r);
+  hipStream_t s = as_stream(stream);
+  auto launch = [&](auto type, auto kind) {
+    if (interleaved) rotary_kernel<decltype(type), kind.value, true><<<blocks, kBlock, 0, s>>>(a);
+    else rotary_kernel<decltype(type), kind.value, false><<<blocks, kBlock, 0, s>>>(a);
+  };
+  auto by_kind = [&](auto type) {
+    if (position_kind == OCNN_POS_INT32) launch(type, std::integral_constant<int, OCNN_POS_INT32>());
+    else if (position_kind == OCNN_POS_F32) launch(type, std::integral_constant<int, OCNN_POS_F32>());
+    else launch(type, std::integral_constant<int, OCNN_POS_XYZ>());
+  };
+  if (dtype == OCNN_F32) by_kind(float()); else by_kind(uint16_t());
+  OCNN_LAUNCH_OK("octree_rotary");
+  return OCNN_OK;
+}
+
+int ocnn_recurrence_shape(int rows, int channels, int n_seq, int64_t* carry_rows, size_t* workspace_bytes,
+    size_t* grad_workspace_bytes) {
+  OCNN_REQUIRE(rows >= 0 && channels > 0 && n_seq >= 1 && n_seq <= 65535, OCNN_E_BADARG, "rows %d, channels %d, sequences %d",
+      rows, channels, n_seq);
+  const int64_t ids = scan_ids(rows, n_seq, scan_shift(rows, channels));
+  const size_t one = (size_t)ids * channels * sizeof(float);
+  if (carry_rows) *carry_rows = ids;
+  if (workspace_bytes) *workspace_bytes = 3 * one;
+  if (grad_workspace_bytes) *grad_workspace_bytes = 2 * one;
+  return OCNN_OK;
+}
+
+int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carries, const void* gate, int64_t gate_row,
+    const void* data, int64_t data_row, const float* state, const int* offsets, int n_seq, int rows, int channels,
+    int reverse, int fill_rest, int dtype, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream) {
+  size_t need = 0;
+  int rc = ocnn_recurrence_shape(rows, channels, n_seq, nullptr, &need, nullptr);
+  if (rc) return rc;
+  OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
+  OCNN_REQUIRE(offsets && (rows == 0 || (out && gate && data)), OCNN_E_BADARG, "null pointer");
+  ScanArgs a = {};
+  a.out = out; a.gate = gate; a.data = data; a.out_row = out_row; a.gate_row = gate_row; a.data_row = data_row;
+  a.state = state; a.last = last; a.offsets = offsets;
+  a.n_seq = n_seq; a.rows = rows; a.channels = channels; a.reverse = reverse != 0; a.fill = fill_rest != 0;
+  hipStream_t s = as_stream(stream);
+  const int size = dtype == OCNN_F32 ? 4 : 2;
+  // sequences of 16 rows and fewer on average: one launch that walks them
+  const bool walk = !carries && rows <= 16 * (int64_t)n_seq;
+  const int shift = scan_shift(rows, channels);
+  const int64_t ids = walk ? (int64_t)n_seq + 1 : scan_ids(rows, n_seq, shift);
+  const int v = scan_width(a, size, {{out, out_row}, {gate, gate_row}, {data, data_row}}, ids);
+  a.groups = (channels + v - 1) / v;
+  a.threads = ids * a.groups;
+  if (walk) {
+    by_width(v, [&](auto w) {
+      if (dtype == OCNN_F32) scan_walk_kernel<float, w.value><<<blocks_for(a.threads, 64), 64, 0, s>>>(a);
+      else scan_walk_kernel<uint16_t, w.value><<<blocks_for(a.threads, 64), 64, 0, s>>>(a);
+    });
+    OCNN_LAUNCH_OK("octree_recurrence");
+    return OCNN_OK;
+  }
+  OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence needs %zu bytes, got %zu", need,
+      workspace_bytes);
+  const size_t one = (size_t)ids * channels;
+  a.run_a = (float*)workspace_dev;
+  a.run_h = a.run_a + one;
+  a.carry = carries ? carries : a.run_h + one;
+  by_width(v, [&](auto w) {
+    if (shift == 6) {
+      if (dtype == OCNN_F32) scan_forward_launch<float, w.value, 64>(a, s);
+      else scan_forward_launch<uint16_t, w.value, 64>(a, s);
+    } else {
+      if (dtype == OCNN_F32) scan_forward_launch<float, w.value, 16>(a, s);
+      else scan_forward_launch<uint16_t, w.value, 16>(a, s);
+    }
+  });
+  OCNN_LAUNCH_OK("octree_recurrence");
+  return OCNN_OK;
+}
+
+int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* grad_data, int64_t grad_data_row,
+    float* grad_state, const void* grad_out, int64_t grad_out_row, const float* grad_last, const void* gate,
+    int64_t gate_row, const void* data, int64_t data_row, const float* state, const float* carries, const int* offsets,
+    int n_seq, int rows, int channels, int reverse, int dtype, void* workspace_dev, size_t workspace_bytes,
+    ocnn_stream_t stream) {
+  size_t need = 0;
+  int rc = ocnn_recurrence_shape(rows, channels, n_seq, nullptr, nullptr, &need);
+  if (rc) return rc;
+  OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
+  OCNN_REQUIRE(offsets && carries && (rows == 0 || (grad_gate && grad_data && grad_out && gate && data)), OCNN_E_BADARG,
+      "null pointer");
+  OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence_grad needs %zu bytes, got %zu",
+      need, workspace_bytes);
+  ScanArgs a = {};
+  a.gate = gate; a.data = data; a.grad = grad_out; a.grad_gate = grad_gate; a.grad_data = grad_data;
+  a.gate_row = gate_row; a.data_row = data_row; a.grad_row = grad_out_row; a.grad_gate_row = grad_gate_row;
+  a.grad_data_row = grad_data_row;
+  a.state = state; a.grad_last = grad_last; a.grad_state = grad_state; a.offsets = offsets;
+  a.n_seq = n_seq; a.rows = rows; a.channels = channels; a.reverse = reverse != 0;
+  a.carry = const_cast<float*>(carries);
+  hipStream_t s = as_stream(stream);
+  const int size = dtype == OCNN_F32 ? 4 : 2, shift = scan_shift(rows, channels);
+  const int64_t ids = scan_ids(rows, n_seq, shift);
+  int v = scan_width(a, size, {{grad_gate, grad_gate_row}, {grad_data, grad_data_row}, {grad_out, grad_out_row},
+                               {gate, gate_row}, {data, data_row}}, ids);
+  v = v > 2 ? 2 : v;                 // (a group of rows is held in registers: p, q, before and the three loads)
+  a.groups = (channels + v - 1) / v;
+  a.threads = ids * a.groups;
+  a.run_a = (float*)workspace_dev;
+  a.run_h = a.run_a + (size_t)ids * channels;
+  by_width(v, [&](auto w) {
+    if constexpr (w.value <= 2) {
+      if (shift == 6) {
+        if (dtype == OCNN_F32) scan_backward_launch<float, w.value, 64>(a, s);
+        else scan_backward_launch<uint16_t, w.value, 64>(a, s);
+      } else {
+        if (dtype == OCNN_F32) scan_backward_launch<float, w.value, 16>(a, s);
+        else scan_backward_launch<uint16_t, w.value, 16>(a, s);
+      }
+    }
+  });
+  OCNN_LAUNCH_OK("octree_recurrence_grad");
+  return OCNN_OK;
+}
+
+}  // extern "C"

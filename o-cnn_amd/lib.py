@@ -32,6 +32,14 @@ class BuildParams(C.Structure):
               ("bbmax", C.c_float * 3)]
 
 
+class AttentionParams(C.Structure):
+  _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] + \
+             [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+             [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_lengths", "key_mask")] + \
+             [(n, C.c_int) for n in ("n_seq", "rows_q", "rows_k", "heads", "kv_heads", "dim", "left", "right", "sinks",
+                                     "dtype")] + [("scale", C.c_float)]
+
+
 _lib = None
 _aten = None
 ATEN_PATH = os.path.join(HERE, "binding", "ocnn_aten.so")

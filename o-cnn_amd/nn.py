@@ -1431,3 +1431,10 @@ def octree_update(octree_in, label_in, depth, split, inplace=False):
             C.c_void_p(base), C.c_size_t(sb), _stream())
   out._ocnn_info = _Info(info.raw)
   return out
+
+
+# ---- operators along the node order of a level ----------------------------------------------------------
+from . import sequence as _sequence  # noqa: E402  (it takes the helpers above)
+from .sequence import *  # noqa: E402,F401,F403
+
+__all__ += _sequence.__all__
