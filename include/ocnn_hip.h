@@ -663,10 +663,10 @@ int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void*
  * from the first row to the last (reverse != 0: from the last to the first).  out = h; last (may be NULL)
  * [n_seq, channels] = the state behind the last step (of an empty sequence: the state it began with).
  * States are fp32.  carries: [carry_rows, channels] fp32 as ocnn_recurrence_shape says, kept for the
- * gradient; NULL where none is wanted.  `out` may be neither `gate` nor `data`.
+ * gradient; NULL where none is wanted (ocnn_recurrence_shape with carries = 0).  `out` may be neither `gate` nor `data`.
  * The gradient takes that of `out` and of `last` (grad_last, may be NULL) and writes those of gate, data
  * and state (grad_state, may be NULL).  Results do not change from run to run. */
-int ocnn_recurrence_shape(int rows, int channels, int n_seq, int64_t* carry_rows, size_t* workspace_bytes,
+int ocnn_recurrence_shape(int rows, int channels, int n_seq, int carries, int64_t* carry_rows, size_t* workspace_bytes,
     size_t* grad_workspace_bytes);
 int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carries, const void* gate, int64_t gate_row,
     const void* data, int64_t data_row, const float* state, const int* offsets, int n_seq, int rows, int channels,

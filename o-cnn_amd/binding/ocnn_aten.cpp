@@ -12,8 +12,10 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
 #include <cstring>
 #include <mutex>
+#include <optional>
 #include <unordered_map>
 #include <vector>
 
@@ -21,6 +23,7 @@
 
 namespace {
 
+using std::optional;
 using std::string;
 using std::vector;
 using torch::Tensor;
@@ -898,6 +901,211 @@ Tensor octree_align_grad(Tensor des_grad, Tensor idx_tensor) {
   return out;
 }
 
+// ---- operators along the node order of an octree level (no counterpart in the reference) -----------------------------------
+// Each comes in two parts: `try_*` runs the call where its tensors are ready for the library as they are (on the
+// current GPU, types and shapes as documented, rows where the kernels read them) and returns nothing otherwise,
+// and the registered operator demands that.  The Python mirror (sequence.py) tries first, which costs a few
+// microseconds, and otherwise makes copies, takes a caller's output or says what is wrong.
+namespace {
+
+bool ready(const Tensor& t, int64_t ndim, at::ScalarType type, const at::Device& device) {
+  return t.defined() && t.dim() == ndim && t.scalar_type() == type && t.device() == device && !(ndim && t.size(ndim - 1) > 1 && t.stride(ndim - 1) != 1);
+}
+bool feature(const Tensor& t, int64_t ndim) {
+  return t.defined() && t.is_cuda() && t.dim() == ndim && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
+      !(t.size(ndim - 1) > 1 && t.stride(ndim - 1) != 1) && t.get_device() == c10::hip::current_device();
+}
+bool aligned_rows(const Tensor& t) {
+  const int64_t e = 16 / (int64_t)t.element_size();
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % e == 0 && t.stride(1) % e == 0;
+}
+bool table(const Tensor& t, at::ScalarType type, const Tensor& like, int64_t numel) {
+  return t.defined() && t.dim() == 1 && t.scalar_type() == type && t.device() == like.device() && (numel < 0 || t.numel() == numel) &&
+      (t.numel() <= 1 || t.stride(0) == 1);
+}
+bool state_ok(const optional<Tensor>& t, int64_t n, int64_t c, const Tensor& like) {
+  return !t || (t->dim() == 2 && t->scalar_type() == at::kFloat && t->size(0) == n && t->size(1) == c && t->device() == like.device() &&
+      t->is_contiguous());
+}
+template <typename T> T* ptr_or_null(const optional<Tensor>& t) { return t ? static_cast<T*>(t->data_ptr()) : nullptr; }
+
+optional<Tensor> try_rotary(const Tensor& data, const Tensor& positions, const Tensor& frequencies, const vector<int>& pairs,
+    bool interleaved, bool inverse) {
+  if (!feature(data, 3) || pairs.empty() || pairs.size() > 4) return {};
+  int64_t total = 0;
+  for (int n : pairs) {
+    if (n < 0) return {};
+    total += n;
+  }
+  if (2 * total > data.size(2) || !table(frequencies, at::kDouble, data, total) || positions.device() != data.device()) return {};
+  int kind;
+  int64_t stride = 1;
+  if (positions.scalar_type() == at::kLong) {
+    if (!table(positions, at::kLong, data, data.size(0)) || pairs.size() > 3) return {};
+    kind = OCNN_POS_XYZ;
+  } else {
+    const bool whole = positions.scalar_type() == at::kInt;
+    if (!ready(positions, 2, whole ? at::kInt : at::kFloat, data.device()) || positions.size(0) != data.size(0) ||
+        positions.size(1) < (int64_t)pairs.size())
+      return {};
+    kind = whole ? OCNN_POS_INT32 : OCNN_POS_F32;
+    stride = positions.stride(0);
+  }
+  Tensor out = at::empty(data.sizes(), data.options());
+  if (ocnn_octree_rotary(out.data_ptr(), out.stride(0), out.stride(1), data.data_ptr(), data.stride(0), data.stride(1),
+      (int)data.size(0), (int)data.size(1), (int)data.size(2), positions.data_ptr(), kind, stride,
+      frequencies.data_ptr<double>(), pairs.data(), (int)pairs.size(), interleaved, inverse, dtype_of(data), current_stream()) != OCNN_OK) return {};
+  return out;
+}
+
+// the parameters of an attention call, false where something is not ready
+bool attention_params(ocnn_attention_params* p, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+    const optional<Tensor>& k_offsets, const optional<Tensor>& k_lengths, int64_t left, int64_t right, int64_t sinks,
+    const optional<double>& scale, const optional<Tensor>& key_mask) {
+  if (!feature(q, 3) || !ready(k, 3, q.scalar_type(), q.device()) || !ready(v, 3, q.scalar_type(), q.device())) return false;
+  if (k.sizes() != v.sizes() || k.size(2) != q.size(2) || !aligned_rows(q) || !aligned_rows(k) || !aligned_rows(v)) return false;
+  const Tensor& ko = k_offsets ? *k_offsets : q_offsets;
+  if (!k_offsets && k.size(0) != q.size(0)) return false;
+  if (!table(q_offsets, at::kInt, q, -1) || q_offsets.numel() < 2 || !table(ko, at::kInt, q, q_offsets.numel())) return false;
+  const int64_t n = q_offsets.numel() - 1;
+  if ((k_lengths && !table(*k_lengths, at::kInt, q, n)) || (key_mask && !table(*key_mask, at::kBool, q, k.size(0)))) return false;
+  const int64_t most = INT32_MAX;
+  if (left < -1 || right < -1 || sinks < 0 || left > most || right > most || sinks > 64 || n > 65535 || q.size(0) > most ||
+      k.size(0) > most || q.size(1) > most || q.size(2) > 128)
+    return false;
+  const double s = scale ? *scale : 1.0 / std::sqrt((double)std::max<int64_t>(q.size(2), 1));
+  if (!std::isfinite(s)) return false;
+  *p = ocnn_attention_params{q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+      v.stride(0), v.stride(1), q_offsets.data_ptr<int>(), ko.data_ptr<int>(), ptr_or_null<const int>(k_lengths),
+      ptr_or_null<const unsigned char>(key_mask), (int)n, (int)q.size(0), (int)k.size(0), (int)q.size(1), (int)k.size(1),
+      (int)q.size(2), (int)left, (int)right, (int)sinks, dtype_of(q), (float)s};
+  return ocnn_attention_workspace_bytes(p, nullptr, nullptr) == OCNN_OK;
+}
+optional<Tensor> scratch(size_t bytes, const Tensor& like) {
+  if (!bytes) return {};
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+// {out} or {out, lse}; empty where something is not ready
+vector<Tensor> try_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+    const optional<Tensor>& k_offsets, const optional<Tensor>& k_lengths, int64_t left, int64_t right, int64_t sinks,
+    const optional<double>& scale, const optional<Tensor>& key_mask, bool return_lse) {
+  ocnn_attention_params p;
+  if (!attention_params(&p, q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask)) return {};
+  size_t need = 0;
+  if (ocnn_attention_workspace_bytes(&p, &need, nullptr) != OCNN_OK) return {};
+  Tensor out = at::empty(q.sizes(), q.options());
+  vector<Tensor> result{out};
+  if (return_lse) result.push_back(at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)));
+  const optional<Tensor> ws = scratch(need, q);
+  if (ocnn_octree_attention(out.data_ptr(), out.stride(0), out.stride(1), return_lse ? result[1].data_ptr<float>() : nullptr, &p, 1,
+      ptr_or_null<void>(ws), need, current_stream()) != OCNN_OK) return {};
+  return result;
+}
+
+vector<Tensor> try_attention_grad(const Tensor& grad_out, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+    const Tensor& lse, const Tensor& q_offsets, const optional<Tensor>& k_offsets, const optional<Tensor>& k_lengths, int64_t left,
+    int64_t right, int64_t sinks, const optional<double>& scale, const optional<Tensor>& key_mask) {
+  ocnn_attention_params p;
+  if (!attention_params(&p, q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask)) return {};
+  if (!ready(out, 3, q.scalar_type(), q.device()) || !ready(grad_out, 3, q.scalar_type(), q.device()) || out.sizes() != q.sizes() ||
+      grad_out.sizes() != q.sizes() || !aligned_rows(out) || !aligned_rows(grad_out) ||
+      !state_ok(lse, q.size(0), q.size(1), q))
+    return {};
+  size_t need = 0;
+  if (ocnn_attention_workspace_bytes(&p, nullptr, &need) != OCNN_OK) return {};
+  Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()), dv = at::empty(k.sizes(), q.options());
+  const optional<Tensor> ws = scratch(need, q);
+  if (ocnn_octree_attention_grad(dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1),
+      dv.data_ptr(), dv.stride(0), dv.stride(1), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1), out.data_ptr(),
+      out.stride(0), out.stride(1), lse.data_ptr<float>(), &p, ptr_or_null<void>(ws), need, current_stream()) != OCNN_OK) return {};
+  return {dq, dk, dv};
+}
+
+bool recurrence_ready(const Tensor& gate, const Tensor& data, const Tensor& offsets, const optional<Tensor>& state) {
+  return feature(data, 2) && ready(gate, 2, data.scalar_type(), data.device()) && gate.sizes() == data.sizes() && data.size(1) > 0 &&
+      data.size(0) <= INT32_MAX && data.size(1) <= INT32_MAX && table(offsets, at::kInt, data, -1) && offsets.numel() >= 2 &&
+      offsets.numel() <= 65536 && state_ok(state, offsets.numel() - 1, data.size(1), data);
+}
+
+// {h, last} or {h, last, carries}; empty where something is not ready
+vector<Tensor> try_recurrence(const Tensor& gate, const Tensor& data, const Tensor& offsets, const optional<Tensor>& state,
+    bool reverse, bool return_carries) {
+  if (!recurrence_ready(gate, data, offsets, state)) return {};
+  const int rows = (int)data.size(0), channels = (int)data.size(1), n = (int)offsets.numel() - 1;
+  int64_t carry_rows = 0;
+  size_t need = 0;
+  if (ocnn_recurrence_shape(rows, channels, n, return_carries, &carry_rows, &need, nullptr) != OCNN_OK) return {};
+  Tensor out = at::empty(data.sizes(), data.options()), last = at::empty({n, channels}, data.options().dtype(at::kFloat));
+  vector<Tensor> result{out, last};
+  if (return_carries) result.push_back(at::empty({carry_rows, channels}, last.options()));
+  const optional<Tensor> ws = scratch(need, data);
+  if (ocnn_octree_recurrence(out.data_ptr(), out.stride(0), last.data_ptr<float>(),
+      return_carries ? result[2].data_ptr<float>() : nullptr, gate.data_ptr(), gate.stride(0), data.data_ptr(), data.stride(0),
+      ptr_or_null<const float>(state), offsets.data_ptr<int>(), n, rows, channels, reverse, 1, dtype_of(data),
+      ptr_or_null<void>(ws), need, current_stream()) != OCNN_OK) return {};
+  return result;
+}
+
+vector<Tensor> try_recurrence_grad(const Tensor& grad_out, const Tensor& gate, const Tensor& data, const Tensor& offsets,
+    const Tensor& carries, const optional<Tensor>& state, const optional<Tensor>& grad_last, bool reverse) {
+  if (!recurrence_ready(gate, data, offsets, state) || !ready(grad_out, 2, data.scalar_type(), data.device()) ||
+      grad_out.sizes() != data.sizes())
+    return {};
+  const int rows = (int)data.size(0), channels = (int)data.size(1), n = (int)offsets.numel() - 1;
+  int64_t carry_rows = 0;
+  size_t need = 0;
+  if (ocnn_recurrence_shape(rows, channels, n, 1, &carry_rows, nullptr, &need) != OCNN_OK) return {};
+  if (!state_ok(carries, carry_rows, channels, data) || !state_ok(grad_last, n, channels, data)) return {};
+  Tensor dgate = at::empty(data.sizes(), data.options()), ddata = at::empty(data.sizes(), data.options());
+  Tensor dstate = at::empty({n, channels}, carries.options());
+  const optional<Tensor> ws = scratch(need, data);
+  if (ocnn_octree_recurrence_grad(dgate.data_ptr(), dgate.stride(0), ddata.data_ptr(), ddata.stride(0), dstate.data_ptr<float>(),
+      grad_out.data_ptr(), grad_out.stride(0), ptr_or_null<const float>(grad_last), gate.data_ptr(), gate.stride(0),
+      data.data_ptr(), data.stride(0), ptr_or_null<const float>(state), carries.data_ptr<float>(), offsets.data_ptr<int>(), n, rows,
+      channels, reverse, dtype_of(data), ptr_or_null<void>(ws), need, current_stream()) != OCNN_OK) return {};
+  return {dgate, ddata, dstate};
+}
+
+const char* kNotReady = "the tensors must be on the current GPU, fp32 or bf16 alike, with the documented shapes, contiguous innermost "
+    "axes and (attention) rows at multiples of 16 bytes";
+vector<Tensor> demand(vector<Tensor> r, const char* name) {
+  TORCH_CHECK(!r.empty(), name, ": ", kNotReady, " (the library's last message: ", ocnn_last_error(), ")");
+  return r;
+}
+
+}  // namespace
+
+Tensor octree_offsets(Tensor octree, int depth, bool nempty) {
+  Info info(octree);
+  Tensor out = torch::empty({ocnn_info_batch_size(info.p()) + 1}, octree.options().dtype(torch::kInt32));
+  check(ocnn_octree_offsets(out.data_ptr<int>(), octree.data_ptr(), info.p(), depth, nempty, current_stream()));
+  return out;
+}
+Tensor octree_rotary(Tensor data, Tensor positions, Tensor frequencies, vector<int> pairs, bool interleaved, bool inverse) {
+  const optional<Tensor> out = try_rotary(data, positions, frequencies, pairs, interleaved, inverse);
+  TORCH_CHECK(out.has_value(), "octree_rotary: ", kNotReady);
+  return *out;
+}
+vector<Tensor> octree_attention(Tensor q, Tensor k, Tensor v, Tensor q_offsets, optional<Tensor> k_offsets, optional<Tensor> k_lengths,
+    int64_t left, int64_t right, int64_t sinks, optional<double> scale, optional<Tensor> key_mask, bool return_lse) {
+  return demand(try_attention(q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask, return_lse),
+      "octree_attention");
+}
+vector<Tensor> octree_attention_grad(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor q_offsets,
+    optional<Tensor> k_offsets, optional<Tensor> k_lengths, int64_t left, int64_t right, int64_t sinks, optional<double> scale,
+    optional<Tensor> key_mask) {
+  return demand(try_attention_grad(grad_out, q, k, v, out, lse, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask),
+      "octree_attention_grad");
+}
+vector<Tensor> octree_recurrence(Tensor gate, Tensor data, Tensor offsets, optional<Tensor> state, bool reverse, bool return_carries) {
+  return demand(try_recurrence(gate, data, offsets, state, reverse, return_carries), "octree_recurrence");
+}
+vector<Tensor> octree_recurrence_grad(Tensor grad_out, Tensor gate, Tensor data, Tensor offsets, Tensor carries, optional<Tensor> state,
+    optional<Tensor> grad_last, bool reverse) {
+  return demand(try_recurrence_grad(grad_out, gate, data, offsets, carries, state, grad_last, reverse), "octree_recurrence_grad");
+}
+
 // Test hooks for the header copies: the bytes this file would use for `octree`, and how many
 // copies are alive (entries of dead tensors are dropped first).
 Tensor octree_header(Tensor octree) {
@@ -958,6 +1166,29 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("points_property", &points_property, "a property of a point cloud");
   m.def("points_set_property", &points_set_property, "a copy of a point cloud with one property replaced");
   m.def("points_new", &points_new, "a serialized point cloud from its arrays");
+  m.def("octree_offsets", &octree_offsets, "where the nodes of each octree of a level begin", py::arg("octree"), py::arg("depth"),
+      py::arg("nempty") = false);
+  m.def("octree_rotary", &octree_rotary, "rotary positions with several axes", py::arg("data"), py::arg("positions"),
+      py::arg("frequencies"), py::arg("pairs"), py::arg("interleaved") = false, py::arg("inverse") = false);
+  m.def("octree_attention", &octree_attention, "attention inside each sequence: [out] or [out, lse]", py::arg("q"), py::arg("k"),
+      py::arg("v"), py::arg("q_offsets"), py::arg("k_offsets") = py::none(), py::arg("k_lengths") = py::none(),
+      py::arg("left") = -1, py::arg("right") = -1, py::arg("sinks") = 0, py::arg("scale") = py::none(),
+      py::arg("key_mask") = py::none(), py::arg("return_lse") = false);
+  m.def("octree_attention_grad", &octree_attention_grad, "gradients of octree_attention", py::arg("grad_out"), py::arg("q"),
+      py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("q_offsets"), py::arg("k_offsets") = py::none(),
+      py::arg("k_lengths") = py::none(), py::arg("left") = -1, py::arg("right") = -1, py::arg("sinks") = 0,
+      py::arg("scale") = py::none(), py::arg("key_mask") = py::none());
+  m.def("octree_recurrence", &octree_recurrence, "gated linear recurrence: [h, last] or [h, last, carries]", py::arg("gate"),
+      py::arg("data"), py::arg("offsets"), py::arg("state") = py::none(), py::arg("reverse") = false,
+      py::arg("return_carries") = false);
+  m.def("octree_recurrence_grad", &octree_recurrence_grad, "gradients of octree_recurrence", py::arg("grad_out"), py::arg("gate"),
+      py::arg("data"), py::arg("offsets"), py::arg("carries"), py::arg("state") = py::none(), py::arg("grad_last") = py::none(),
+      py::arg("reverse") = false);
+  m.def("try_rotary", &try_rotary, "octree_rotary, or None where a tensor is not ready for it");
+  m.def("try_attention", &try_attention, "octree_attention, or [] where a tensor is not ready for it");
+  m.def("try_attention_grad", &try_attention_grad, "octree_attention_grad, or [] where a tensor is not ready for it");
+  m.def("try_recurrence", &try_recurrence, "octree_recurrence, or [] where a tensor is not ready for it");
+  m.def("try_recurrence_grad", &try_recurrence_grad, "octree_recurrence_grad, or [] where a tensor is not ready for it");
   m.def("octree_header", &octree_header, "the host copy of an octree's header (test hook)");
   m.def("octree_header_copies", &octree_header_copies, "live header copies (test hook)");
 }

@@ -559,38 +559,60 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
   }
 }
 
-// o = sum_s exp(m_s - m) o_s / sum_s exp(m_s - m) l_s, a wavefront a row
+// o = sum_s exp(m_s - m) o_s / sum_s exp(m_s - m) l_s.  A workgroup joins one row: its 256 threads weigh the (at
+// most 256) shares, then 8 groups of 32 lanes, 4 channels each, add theirs up and are added in order.
+constexpr int kMaxSplits = 256;
 template <typename T>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs a) {
+  __shared__ float weight[kMaxSplits];
+  __shared__ float part[4];
+  __shared__ floatx4 sums[8][32];
   const ocnn_attention_params& p = a.p;
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)p.rows_q * p.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int64_t token = row / p.heads;
-  const int head = (int)(row - token * p.heads);
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int64_t rows = (int64_t)p.rows_q * p.heads, row = blockIdx.x;
+  const int token = (int)(row / p.heads), head = (int)(row - (int64_t)token * p.heads);
   float m = -__builtin_inff(), l = 0.0f;
-  bool none = false;
-  for (int s = 0; s < a.splits; ++s) {
-    m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
-    none = none || a.part_ml[(s * rows + row) * 2 + 1] == -1.0f;
+  if (t < a.splits) {
+    const float2 ml = *(const float2*)(a.part_ml + (t * rows + row) * 2);
+    m = ml.x;
+    l = ml.y;
   }
+  const bool none = __syncthreads_or(l == -1.0f);       // a row of no sequence
   if (none && !a.fill) return;
-  const float base = m == -__builtin_inff() ? 0.0f : m;
-  float o0 = 0.0f, o1 = 0.0f;
-  if (!none)
-    for (int s = 0; s < a.splits; ++s) {
-      const float ls = a.part_ml[(s * rows + row) * 2 + 1];
-      if (ls == 0.0f) continue;               // (a share without a visible key: its values do not count)
-      const float w = __builtin_amdgcn_exp2f(a.part_ml[(s * rows + row) * 2] - base);
-      l += w * ls;
-      const float* po = a.part_o + (s * rows + row) * p.dim;
-      if (lane < p.dim) o0 = fmaf(w, po[lane], o0);
-      if (lane + 64 < p.dim) o1 = fmaf(w, po[lane + 64], o1);
+  const float wm = wave_max(m);
+  if (lane == 0) part[wave] = wm;
+  __syncthreads();
+  const float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), base = top == -__builtin_inff() ? 0.0f : top;
+  // (a share without a visible key does not count, whatever its values are)
+  const float w = none || l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+  weight[t] = w;
+  l = wave_sum(w == 0.0f ? 0.0f : w * l);
+  __syncthreads();
+  if (lane == 0) part[wave] = l;
+  __syncthreads();
+  l = part[0] + part[1] + part[2] + part[3];
+  const int group = t >> 5, c = (t & 31) * 4;
+  floatx4 o = {0, 0, 0, 0};
+  if (c < p.dim)
+#pragma unroll 8
+    for (int s = group; s < a.splits; s += 8) {
+      const floatx4 x = *(const floatx4*)(a.part_o + (s * rows + row) * p.dim + c);
+      const float ws = weight[s];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = ws == 0.0f ? o[e] : fmaf(ws, x[e], o[e]);
     }
-  T* out = (T*)a.out + token * a.out_row + head * a.out_head;
-  if (lane < p.dim) out[lane] = from_f32<T>(l == 0.0f ? 0.0f : o0 / l);
-  if (lane + 64 < p.dim) out[lane + 64] = from_f32<T>(l == 0.0f ? 0.0f : o1 / l);
-  if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  sums[group][t & 31] = o;
+  __syncthreads();
+  if (group || c >= p.dim) return;
+#pragma unroll
+  for (int g = 1; g < 8; ++g)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += sums[g][t & 31][e];
+  Pack<T, 4> y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y.v[e] = from_f32<T>(l == 0.0f ? 0.0f : o[e] / l);
+  y.store((T*)a.out + (int64_t)token * a.out_row + (int64_t)head * a.out_head + c);
+  if (a.lse && t == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---- gradient of the queries ---------------------------------------------------------------------------
@@ -1120,7 +1142,7 @@ Plan plan_of(const ocnn_attention_params& p) {
   if (p.left >= 0 && p.right >= 0) keys = std::min<int64_t>(keys, (int64_t)p.left + p.right + p.rows_q / p.n_seq + p.sinks);
   const int64_t blocks = std::max<int64_t>((packed + (n.few ? 31 : 127)) / (n.few ? 32 : 128), n.few ? p.n_seq : 1) * p.kv_heads;
   const int64_t most = n.few ? keys / 512 : keys / 1024;
-  n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, 256}));
+  n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, kMaxSplits}));
   return n;
 }
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -1164,7 +1186,7 @@ template <typename T, int DP> void forward_launch(const AttnArgs& a, const Plan&
     if (n.splits > 1) attention_kernel<T, DP, 4, true><<<grid, 256, 0, s>>>(a);
     else attention_kernel<T, DP, 4, false><<<grid, 256, 0, s>>>(a);
   }
-  if (n.splits > 1) attention_join_kernel<T><<<blocks_for((int64_t)a.p.rows_q * a.p.heads, 4), 256, 0, s>>>(a);
+  if (n.splits > 1) attention_join_kernel<T><<<(unsigned)((int64_t)a.p.rows_q * a.p.heads), 256, 0, s>>>(a);
 }
 
 template <typename T, int DP> void backward_launch(const AttnArgs& a, hipStream_t s) {

@@ -41,7 +41,7 @@ __global__ void octree_offsets_kernel(int* __restrict__ offsets, const uint64_t*
 // position 2^20 a 32-bit product is off by 2^-5 rad, the fraction by 2^-25 of a turn.  One angle
 // serves all heads of a row, so the sines (a 64-bit product, a reduction and a polynomial) are computed
 // once a row into LDS and the streaming part is two fused multiply-adds per channel: bound by HBM.
-// A thread takes 16 bytes of the first channels of V pairs and 16 of the second ones (interleaved: 32
+// A thread takes 16 bytes of the first channels of V pairs and 16 of the second ones (interleaved: 16
 // neighbouring bytes) and writes them back in the same places, so `out` may be `data`.
 constexpr int kRotaryAngles = 2048;   // (rows of a workgroup) x (pairs): 16 KiB of LDS
 
@@ -52,7 +52,7 @@ struct RotaryArgs {
   const double* freq;
   int rows, heads, dim, pairs, axis_end[3], block_rows, items_head, pair_items, copy;
   uint32_t div_pairs, div_row, div_head;   // reciprocals: see fast_div
-  int inverse;
+  int inverse, in_place;
 };
 
 // n / d for n * d < 2^32, by a multiplication with m = floor(2^32 / d) + 1 (m = 0 stands for d = 1)
@@ -62,6 +62,12 @@ template <int KIND> __device__ inline double rotary_position(const void* pos, in
   if (KIND == OCNN_POS_INT32) return (double)((const int*)pos)[row * stride + axis];
   if (KIND == OCNN_POS_F32) return (double)((const float*)pos)[row * stride + axis];
   return (double)(int)((((const uint64_t*)pos)[row] >> (16 * axis)) & 0xffffu);
+}
+
+template <typename T> __device__ inline void turn_pair(T& x, T& y, const float2 k) {
+  const float a = to_f32(x), b = to_f32(y);
+  x = from_f32<T>(fmaf(a, k.x, -(b * k.y)));
+  y = from_f32<T>(fmaf(a, k.y, b * k.x));
 }
 
 template <typename T, int KIND, bool INTERLEAVED>
@@ -88,46 +94,68 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryArgs a) {
     const int h = (int)fast_div((uint32_t)in_row, a.div_head), item = in_row - h * a.items_head;
     const T* src = data + (int64_t)r * a.row + (int64_t)h * a.head;
     T* dst = out + (int64_t)r * a.out_row + (int64_t)h * a.out_head;
+    const float2* cs = turn + r * a.pairs;
+    if (INTERLEAVED) {
+      // V neighbouring channels; those from 2 P on turn by nothing
+      const int c = item * V, n = min(V, a.dim - c);
+      Pack<T, V> x;
+      if (n == V) {
+        x.load(src + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x.v[j] = j < n ? src[c + j] : (T)0;
+      }
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        const int p = c / 2 + j / 2;
+        if (p < a.pairs) turn_pair(x.v[j], x.v[j + 1], cs[p]);
+      }
+      if (n == V) {
+        x.store(dst + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < n) dst[c + j] = x.v[j];
+      }
+      continue;
+    }
     if (item >= a.pair_items) {                       // channels that carry no position
-      const int c = 2 * a.pairs + (item - a.pair_items) * V, n = min(V, a.dim - c);
+      int c = 2 * a.pairs + (item - a.pair_items) * V;
+      if (c + V > a.dim && a.dim - 2 * a.pairs >= V) c = a.dim - V;     // (copies: overlapping ones are the same)
+      const int n = min(V, a.dim - c);
       if (n == V) { Pack<T, V> x; x.load(src + c); x.store(dst + c); }
       else for (int j = 0; j < n; ++j) dst[c + j] = src[c + j];
       continue;
     }
-    const int p = item * V, n = min(V, a.pairs - p);
-    const float2* cs = turn + r * a.pairs + p;
-    const int c0 = INTERLEAVED ? 2 * p : p, c1 = INTERLEAVED ? 2 * p + V : a.pairs + p;
+    int p = item * V;
+    // the last pairs of a head, where they fill no whole vector: one vector back, together with pairs of the item
+    // before, whose results are the same -- unless the input is overwritten meanwhile
+    if (p + V > a.pairs && a.pairs >= V && !a.in_place) p = a.pairs - V;
+    const int n = min(V, a.pairs - p);
     Pack<T, V> u, w;
     if (n == V) {
-      u.load(src + c0);
-      w.load(src + c1);
+      u.load(src + p);
+      w.load(src + a.pairs + p);
     } else {
-      u.fill(0);
-      w.fill(0);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if ((INTERLEAVED ? j < 2 * n : j < n)) u.v[j] = src[c0 + j];
-        if ((INTERLEAVED ? j + V < 2 * n : j < n)) w.v[j] = src[c1 + j];
+        u.v[j] = j < n ? src[p + j] : (T)0;
+        w.v[j] = j < n ? src[a.pairs + p + j] : (T)0;
       }
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 k = j < n ? cs[j] : make_float2(1.0f, 0.0f);
-      T& first = INTERLEAVED ? (2 * j < V ? u.v[(2 * j) % V] : w.v[(2 * j) % V]) : u.v[j];
-      T& second = INTERLEAVED ? (2 * j < V ? u.v[(2 * j + 1) % V] : w.v[(2 * j + 1) % V]) : w.v[j];
-      const float x = to_f32(first), y = to_f32(second);
-      first = from_f32<T>(fmaf(x, k.x, -(y * k.y)));
-      second = from_f32<T>(fmaf(x, k.y, y * k.x));
-    }
+    for (int j = 0; j < V; ++j)
+      if (j < n) turn_pair(u.v[j], w.v[j], cs[p + j]);
     if (n == V) {
-      u.store(dst + c0);
-      w.store(dst + c1);
+      u.store(dst + p);
+      w.store(dst + a.pairs + p);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if ((INTERLEAVED ? j < 2 * n : j < n)) dst[c0 + j] = u.v[j];
-        if ((INTERLEAVED ? j + V < 2 * n : j < n)) dst[c1 + j] = w.v[j];
-      }
+      for (int j = 0; j < V; ++j)
+        if (j < n) {
+          dst[p + j] = u.v[j];
+          dst[a.pairs + p + j] = w.v[j];
+        }
     }
   }
 }
@@ -295,8 +323,10 @@ __global__ void __launch_bounds__(kBlock) scan_run_back_kernel(ScanArgs a) {
 
 // The state in front of each chunk of a sequence: kSegments threads a channel fold a share of the runs
 // each, the shares are folded in order, and each thread walks its share again writing the states.
-// A workgroup serves 16 channels of one sequence.
-constexpr int kCarryChannels = 16, kSegments = 64;
+// A workgroup serves 8 channels (32 bytes a run: the smallest piece memory moves) of one sequence, so that
+// one long sequence still has a workgroup for every 8 channels; a share of up to kHeld runs stays in
+// registers between the two walks (262147 rows of 256 channels: 16 runs of 128 rows a thread).
+constexpr int kCarryChannels = 8, kSegments = 128, kHeld = 16;
 
 template <int SHIFT, bool BACK>
 __global__ void __launch_bounds__(kCarryChannels * kSegments) scan_carry_kernel(ScanArgs a) {
@@ -309,28 +339,43 @@ __global__ void __launch_bounds__(kCarryChannels * kSegments) scan_carry_kernel(
   const int64_t id0 = first_id(a, seq, SHIFT);
   const int share = (chunks + kSegments - 1) / kSegments;
   const int from = min(seg * share, chunks), to = min(from + share, chunks);
+  const bool mine = c < a.channels;
   // chunk j in the order of the walk; the run of the walk's last chunk does not exist
   auto at = [&](int j) { return (id0 + (BACK ? chunks - 1 - j : j)) * a.channels + c; };
-  float A = 1.0f, H = 0.0f;
-  if (c < a.channels)
-    for (int j = from; j < min(to, chunks - 1); ++j) {
-      const float ra = a.run_a[at(j)], rh = a.run_h[at(j)];
-      H = fmaf(ra, H, rh);
-      A *= ra;
+  float ra[kHeld], rh[kHeld];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const bool ok = mine && j0 + i < min(to, chunks - 1);
+      ra[i] = ok ? a.run_a[at(j0 + i)] : 1.0f;
+      rh[i] = ok ? a.run_h[at(j0 + i)] : 0.0f;
     }
+  };
+  float A = 1.0f, H = 0.0f;
+  for (int j = from; j < to; j += kHeld) {
+    load(j);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      H = fmaf(ra[i], H, rh[i]);
+      A *= ra[i];
+    }
+  }
   sa[seg][lane] = A;
   sh[seg][lane] = H;
   __syncthreads();
-  if (c >= a.channels) return;
   const float* start = BACK ? a.grad_last : a.state;
-  float h = start ? start[(int64_t)seq * a.channels + c] : 0.0f;
+  float h = mine && start ? start[(int64_t)seq * a.channels + c] : 0.0f;
   for (int s = 0; s < seg; ++s) h = fmaf(sa[s][lane], h, sh[s][lane]);
+  if (!mine) return;
   float* carry = BACK ? a.run_h : a.carry;       // (back: in place, a share is read before it is written)
-  for (int j = from; j < to; ++j) {
-    float ra = 0.0f, rh = 0.0f;
-    if (j < chunks - 1) { ra = a.run_a[at(j)]; rh = a.run_h[at(j)]; }
-    carry[at(j)] = h;
-    h = fmaf(ra, h, rh);
+  for (int j = from; j < to; j += kHeld) {
+    if (share > kHeld) load(j);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (j + i < to) {
+        carry[at(j + i)] = h;
+        h = fmaf(ra[i], h, rh[i]);
+      }
   }
 }
 
@@ -532,9 +577,15 @@ __global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
     for (int v = 0; v < V; ++v) a.last[(int64_t)seq * a.channels + c0 + v] = h[v];
 }
 
-// Rows of a chunk: 64 where that leaves enough threads for the chip, else 16.  The rule sees sizes that the
+// Rows of a chunk: many where that leaves enough threads for the chip (the runs and states cost 24 bytes a
+// channel and chunk, and the carry step is short), few where it does not.  The rule sees sizes that the
 // forward and the backward call share, so their chunks are the same.
-int scan_shift(int64_t rows, int64_t channels) { return rows * channels >= (int64_t)1 << 22 ? 6 : 4; }
+int scan_shift(int64_t rows, int64_t channels) {
+  return rows * channels >= (int64_t)1 << 25 ? 7 : rows * channels >= (int64_t)1 << 22 ? 6 : 4;
+}
+
+// sequences of 16 rows and fewer on average: one launch that walks them
+bool scan_walks(int64_t rows, int64_t n_seq, bool carries) { return !carries && rows <= 16 * n_seq; }
 
 int64_t scan_ids(int64_t rows, int n_seq, int shift) { return (rows >> shift) + n_seq + 1; }
 
@@ -571,6 +622,12 @@ template <typename F> void by_width(int v, F f) {
   if (v == 4) f(std::integral_constant<int, 4>());
   else if (v == 2) f(std::integral_constant<int, 2>());
   else f(std::integral_constant<int, 1>());
+}
+
+template <typename F> void by_chunk(int shift, F f) {
+  if (shift == 7) f(std::integral_constant<int, 128>());
+  else if (shift == 6) f(std::integral_constant<int, 64>());
+  else f(std::integral_constant<int, 16>());
 }
 
 }  // namespace
@@ -630,9 +687,10 @@ int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void*
   a.pos = positions; a.pos_row = position_row; a.freq = frequencies;
   a.rows = rows; a.heads = heads; a.dim = dim; a.pairs = (int)total;
   for (int i = 0; i < 3; ++i) a.axis_end[i] = ends[i];
-  a.pair_items = (a.pairs + V - 1) / V;
-  const bool in_place = out == data && out_row == row && out_head == head;
-  a.items_head = a.pair_items + (in_place ? 0 : (dim - 2 * a.pairs + V - 1) / V);
+  a.in_place = out == data && out_row == row && out_head == head;
+  a.pair_items = interleaved ? 0 : (a.pairs + V - 1) / V;
+  if (interleaved) a.items_head = ((a.in_place ? 2 * a.pairs : dim) + V - 1) / V;
+  else a.items_head = a.pair_items + (a.in_place ? 0 : (dim - 2 * a.pairs + V - 1) / V);
   if (a.items_head == 0) return OCNN_OK;
   const int items = heads * a.items_head;
   // rows of a workgroup: about 1024 items of 32 bytes (60001 rows of 12 x 48 channels bf16), fewer where that
@@ -661,14 +719,14 @@ int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void*
   return OCNN_OK;
 }
 
-int ocnn_recurrence_shape(int rows, int channels, int n_seq, int64_t* carry_rows, size_t* workspace_bytes,
+int ocnn_recurrence_shape(int rows, int channels, int n_seq, int carries, int64_t* carry_rows, size_t* workspace_bytes,
     size_t* grad_workspace_bytes) {
   OCNN_REQUIRE(rows >= 0 && channels > 0 && n_seq >= 1 && n_seq <= 65535, OCNN_E_BADARG, "rows %d, channels %d, sequences %d",
       rows, channels, n_seq);
   const int64_t ids = scan_ids(rows, n_seq, scan_shift(rows, channels));
   const size_t one = (size_t)ids * channels * sizeof(float);
   if (carry_rows) *carry_rows = ids;
-  if (workspace_bytes) *workspace_bytes = 3 * one;
+  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) ? 0 : (carries ? 2 : 3) * one;
   if (grad_workspace_bytes) *grad_workspace_bytes = 2 * one;
   return OCNN_OK;
 }
@@ -677,7 +735,7 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
     const void* data, int64_t data_row, const float* state, const int* offsets, int n_seq, int rows, int channels,
     int reverse, int fill_rest, int dtype, void* workspace_dev, size_t workspace_bytes, ocnn_stream_t stream) {
   size_t need = 0;
-  int rc = ocnn_recurrence_shape(rows, channels, n_seq, nullptr, &need, nullptr);
+  int rc = ocnn_recurrence_shape(rows, channels, n_seq, carries != nullptr, nullptr, &need, nullptr);
   if (rc) return rc;
   OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
   OCNN_REQUIRE(offsets && (rows == 0 || (out && gate && data)), OCNN_E_BADARG, "null pointer");
@@ -687,8 +745,7 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
   a.n_seq = n_seq; a.rows = rows; a.channels = channels; a.reverse = reverse != 0; a.fill = fill_rest != 0;
   hipStream_t s = as_stream(stream);
   const int size = dtype == OCNN_F32 ? 4 : 2;
-  // sequences of 16 rows and fewer on average: one launch that walks them
-  const bool walk = !carries && rows <= 16 * (int64_t)n_seq;
+  const bool walk = scan_walks(rows, n_seq, carries != nullptr);
   const int shift = scan_shift(rows, channels);
   const int64_t ids = walk ? (int64_t)n_seq + 1 : scan_ids(rows, n_seq, shift);
   const int v = scan_width(a, size, {{out, out_row}, {gate, gate_row}, {data, data_row}}, ids);
@@ -709,13 +766,10 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
   a.run_h = a.run_a + one;
   a.carry = carries ? carries : a.run_h + one;
   by_width(v, [&](auto w) {
-    if (shift == 6) {
-      if (dtype == OCNN_F32) scan_forward_launch<float, w.value, 64>(a, s);
-      else scan_forward_launch<uint16_t, w.value, 64>(a, s);
-    } else {
-      if (dtype == OCNN_F32) scan_forward_launch<float, w.value, 16>(a, s);
-      else scan_forward_launch<uint16_t, w.value, 16>(a, s);
-    }
+    by_chunk(shift, [&](auto l) {
+      if (dtype == OCNN_F32) scan_forward_launch<float, w.value, l.value>(a, s);
+      else scan_forward_launch<uint16_t, w.value, l.value>(a, s);
+    });
   });
   OCNN_LAUNCH_OK("octree_recurrence");
   return OCNN_OK;
@@ -727,7 +781,7 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
     int n_seq, int rows, int channels, int reverse, int dtype, void* workspace_dev, size_t workspace_bytes,
     ocnn_stream_t stream) {
   size_t need = 0;
-  int rc = ocnn_recurrence_shape(rows, channels, n_seq, nullptr, nullptr, &need);
+  int rc = ocnn_recurrence_shape(rows, channels, n_seq, 1, nullptr, nullptr, &need);
   if (rc) return rc;
   OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
   OCNN_REQUIRE(offsets && carries && (rows == 0 || (grad_gate && grad_data && grad_out && gate && data)), OCNN_E_BADARG,
@@ -752,15 +806,11 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
   a.run_a = (float*)workspace_dev;
   a.run_h = a.run_a + (size_t)ids * channels;
   by_width(v, [&](auto w) {
-    if constexpr (w.value <= 2) {
-      if (shift == 6) {
-        if (dtype == OCNN_F32) scan_backward_launch<float, w.value, 64>(a, s);
-        else scan_backward_launch<uint16_t, w.value, 64>(a, s);
-      } else {
-        if (dtype == OCNN_F32) scan_backward_launch<float, w.value, 16>(a, s);
-        else scan_backward_launch<uint16_t, w.value, 16>(a, s);
-      }
-    }
+    if constexpr (w.value <= 2)
+      by_chunk(shift, [&](auto l) {
+        if (dtype == OCNN_F32) scan_backward_launch<float, w.value, l.value>(a, s);
+        else scan_backward_launch<uint16_t, w.value, l.value>(a, s);
+      });
   });
   OCNN_LAUNCH_OK("octree_recurrence_grad");
   return OCNN_OK;

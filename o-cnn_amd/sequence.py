@@ -113,6 +113,19 @@ def _i64(n):
   return C.c_int64(int(n))
 
 
+_fast = None
+
+
+def _compiled():
+  """The compiled module's try_* functions (binding/ocnn_aten.cpp): the same calls of the same library where all
+  tensors are ready as they are, for a third of the host time; None where the module is not built."""
+  global _fast
+  if _fast is None:
+    import os
+    _fast = _lib.aten() if os.path.exists(_lib.ATEN_PATH) else False
+  return _fast
+
+
 # ---- octree_offsets ---------------------------------------------------------------------------------
 def octree_offsets(octree, depth, nempty=False):
   """Where the nodes (nempty: the non-empty nodes) of each octree of a batch begin at `depth`: int32
@@ -143,6 +156,13 @@ def octree_rotary(data, positions, frequencies, pairs, interleaved=False, invers
   octree_property(octree, "xyz", depth) returns (int64 [rows], at most 3 axes).  The angle is formed in 64
   bits (frequencies: float64), so positions in the millions keep their phase.
   `out`: where the result goes; `data` itself, or a tensor that does not overlap it."""
+  if out is None and _compiled():
+    try:
+      done = _fast.try_rotary(data, positions, frequencies, pairs, interleaved, inverse)
+      if done is not None:
+        return done
+    except TypeError:        # an argument of another kind: named below
+      pass
   data = _rows(data, "data", 3)
   rows, heads, dim = data.shape
   pairs = [int(n) for n in pairs]
@@ -241,6 +261,13 @@ def octree_attention(q, k, v, q_offsets, k_offsets=None, k_lengths=None, left=-1
   `out`: where the result goes (rows of no sequence are left as they are; without `out` they are zero).
   return_lse=True returns (out, lse): lse [rows_q, heads] float32, the logarithm of each softmax's sum, which
   octree_attention_grad takes."""
+  if out is None and _compiled():
+    try:
+      done = _fast.try_attention(q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask, return_lse)
+      if done:
+        return tuple(done) if return_lse else done[0]
+    except TypeError:
+      pass
   p, need, _, q, keep = _attention_params(q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask)
   fill = out is None
   if fill:
@@ -261,6 +288,14 @@ def octree_attention_grad(grad_out, q, k, v, out, lse, q_offsets, k_offsets=None
                           sinks=0, scale=None, key_mask=None):
   """Gradients of octree_attention with respect to q, k and v; `out` and `lse` are what the forward call with the
   same arguments returned.  Rows of no sequence and key rows that are no keys get zeros."""
+  if _compiled():
+    try:
+      done = _fast.try_attention_grad(grad_out, q, k, v, out, lse, q_offsets, k_offsets, k_lengths, left, right, sinks, scale,
+                                      key_mask)
+      if done:
+        return tuple(done)
+    except TypeError:
+      pass
   p, _, need, q, keep = _attention_params(q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask)
   out, grad_out = _rows(out, "out", 3, q), _rows(grad_out, "grad_out", 3, q)
   _require(out.shape == q.shape and grad_out.shape == q.shape, "out is %s, grad_out %s, expected %s"
@@ -283,7 +318,7 @@ def _require_lse(lse, q):
 
 
 # ---- gated linear recurrence ------------------------------------------------------------------------
-def _recurrence_args(gate, data, offsets, state):
+def _recurrence_args(gate, data, offsets, state, carries):
   data = _rows(data, "data", 2)
   gate = _rows(gate, "gate", 2, data)
   _require(gate.shape == data.shape, "gate is %s, data is %s" % (tuple(gate.shape), tuple(data.shape)))
@@ -293,7 +328,7 @@ def _recurrence_args(gate, data, offsets, state):
   n_seq = offsets.numel() - 1
   state = _state(state, "state", (n_seq, data.size(1)), data)
   carry, need, grad = C.c_int64(), C.c_size_t(), C.c_size_t()
-  _lib.call("ocnn_recurrence_shape", data.size(0), data.size(1), n_seq, C.byref(carry), C.byref(need), C.byref(grad))
+  _lib.call("ocnn_recurrence_shape", data.size(0), data.size(1), n_seq, int(bool(carries)), C.byref(carry), C.byref(need), C.byref(grad))
   _on_gpu(data)
   return gate, data, offsets, state, n_seq, carry.value, need.value, grad.value
 
@@ -306,7 +341,14 @@ def octree_recurrence(gate, data, offsets, state=None, reverse=False, out=None, 
   (float32; of an empty sequence the one it began with), which the next call of a running sequence takes
   as `state`.  return_carries=True adds what octree_recurrence_grad needs: the states inside the sequences.
   `out`: where h goes (rows of no sequence are left as they are; without `out` they are zero)."""
-  gate, data, offsets, state, n_seq, carry_rows, need, _ = _recurrence_args(gate, data, offsets, state)
+  if out is None and _compiled():
+    try:
+      done = _fast.try_recurrence(gate, data, offsets, state, reverse, return_carries)
+      if done:
+        return tuple(done)
+    except TypeError:
+      pass
+  gate, data, offsets, state, n_seq, carry_rows, need, _ = _recurrence_args(gate, data, offsets, state, return_carries)
   rows, channels = data.shape
   fill = out is None
   if fill:
@@ -329,7 +371,14 @@ def octree_recurrence_grad(grad_out, gate, data, offsets, carries, state=None, g
   """Gradients of octree_recurrence with respect to gate, data and state, from those of h (`grad_out`) and of
   the last state (`grad_last`, float32, zeros where None).  `carries` is what the forward call with the same
   arguments returned.  Rows of no sequence get zeros."""
-  gate, data, offsets, state, n_seq, carry_rows, _, need = _recurrence_args(gate, data, offsets, state)
+  if _compiled():
+    try:
+      done = _fast.try_recurrence_grad(grad_out, gate, data, offsets, carries, state, grad_last, reverse)
+      if done:
+        return tuple(done)
+    except TypeError:
+      pass
+  gate, data, offsets, state, n_seq, carry_rows, _, need = _recurrence_args(gate, data, offsets, state, True)
   rows, channels = data.shape
   grad_out = _rows(grad_out, "grad_out", 2, data)
   _require(grad_out.shape == data.shape, "grad_out is %s, expected %s" % (tuple(grad_out.shape), tuple(data.shape)))
