@@ -683,10 +683,11 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
  * with -1 for a bound that is absent.  out = sum_j softmax_j(scale q . k_j) v_j over the visible keys, zeros where
  * there is none; a value of a row that is not visible has no influence, whatever it holds.  lse [rows_q, heads]
  * fp32 (may be NULL): the logarithm of the softmax's sum, -inf where no key is visible.
- *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads);
+ *   heads % kv_heads == 0, at most 64 to 1: query head h reads key head h / (heads / kv_heads);
  *   k_offsets: where the rows of each sequence begin in k and v; k_lengths (device, may be NULL): how many of
  *     them are keys -- a cache with room to grow; key_mask (device, may be NULL): one byte a key row;
- *   dim: a multiple of 8 up to 128; sinks <= 64; every row and head begins at a multiple of 16 bytes.
+ *   dim: a multiple of 8 up to 128; sinks <= 64; every row and head begins at a multiple of 16 bytes, less than
+ *     2^22 elements from the one before.
  * The gradient takes out and lse of the forward call; key rows that are no keys get zeros.  Scores, statistics
  * and sums are fp32; bf16 probabilities and score gradients are rounded to bf16 as operands of the second
  * product.  Results do not change from run to run.  Both calls need ocnn_attention_workspace_bytes bytes

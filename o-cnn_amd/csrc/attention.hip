@@ -24,6 +24,13 @@
 namespace ocnn {
 namespace {
 
+#ifndef FWD_W
+#define FWD_W 3
+#define GQ_W 2
+#endif
+// wavefronts a SIMD that the registers leave room for: `small` up to 64 channels
+template <typename T, int DP> constexpr int waves_of(int small) { return DP <= 64 ? small : sizeof(T) == 4 ? 1 : 2; }
+
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
@@ -46,7 +53,7 @@ struct AttnArgs {
   float* part_o; float* part_ml;                              // split keys: [split][row][dim], [split][row][2]
   float* sink_part;                                           // [work item][kv head][2][sinks][dim]
   int splits, fill, group;
-  float scale2;                                               // scale * log2(e)
+  float scale2;                                               // |scale| * log2(e); a negative scale turns one operand around
 };
 
 template <typename T> struct Frag;
@@ -84,7 +91,7 @@ __device__ inline floatx16 zero16() {
 // The lane's pieces of a row (a column of a B operand), straight from memory; zeros where the row or the
 // channels do not exist.
 template <typename T, int DP>
-__device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim) {
+__device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim, bool negate = false) {
   using S = Shape<T, DP>;
   const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
@@ -92,6 +99,7 @@ __device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim
     const int c = (2 * s + half) * S::kPiece;
     uintx4 v = {0, 0, 0, 0};
     if (ok && c < dim) v = *(const uintx4*)(row + c);
+    if (negate) v ^= sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
     f.v[s] = __builtin_bit_cast(typename Frag<T>::type, v);
   }
 }
@@ -153,35 +161,86 @@ __device__ inline void columns_times(floatx16 (&acc)[DP / 32], const float* tile
       acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * S::kPitch + 32 * d], w[r], acc[d], 0, 0, 0);
 }
 
+// For a branch between a matrix product and the code that reads its result.  The compiler counts the wait states
+// that an accumulator needs before it is read, but where a short block lies on one of two paths it counts along
+// that path only, and the other path reads the last registers too early (the last key of a tile came out without
+// its last channels).  So the conditions of such a branch are formed before the product (`decided`: a value
+// the compiler cannot put off), and the branch that is seldom taken waits by itself.
+__device__ inline bool decided(bool x) {
+  int v = __builtin_amdgcn_readfirstlane(x);
+  asm volatile("" : "+s"(v));
+  return v != 0;
+}
+__device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 3"); }
+
 // Row r of an accumulator register in this lane
 __device__ inline int acc_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (r & 3); }
 
 // A tile of ROWS rows on its way from memory to LDS: the loads of the next tile are issued before the current
-// one is used and wait in registers.
-template <typename T, int DP, int ROWS, int THREADS> struct Staged {
+// one is used and wait in registers.  A thread's pieces keep their byte offsets from the tile's first row, so
+// a tile costs one scalar address; a row that does not exist (or is masked) gets an offset behind the
+// buffer, for which the hardware returns zeros without reading.
+constexpr uint32_t kNowhere = 0xfffffff0u, kBufferBytes = 0x80000000u;
+
+__device__ inline __amdgpu_buffer_rsrc_t buffer_at(const void* base) {
+  const uint64_t u = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), (short)0, (int)kBufferBytes, 0x00020000);
+}
+
+// EVEN: rows a constant stride apart; the pieces of a thread are then too, and all but the first offset
+// are scalars (where the threads of a row divide the workgroup).
+template <typename T, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
   using S = Shape<T, DP>;
   static constexpr int kEach = ROWS * S::kPieces / THREADS;
   static_assert(kEach * THREADS == ROWS * S::kPieces, "whole pieces a thread");
+  static constexpr bool kScalar = EVEN && THREADS % S::kPieces == 0;
   uintx4 v[kEach];
-  // row(i): pointer to tile row i or null where there is none
-  template <typename Row> __device__ inline void load(int tid, int dim, Row row) {
+  uint32_t at[kScalar ? 1 : kEach];
+  uint32_t apart;
+  __device__ static inline int row_of(int tid, int i) {
+    return kScalar ? tid / S::kPieces + i * (THREADS / S::kPieces) : (tid + i * THREADS) / S::kPieces;
+  }
+  // offset(r): elements from the tile's first row to row r
+  template <typename Offset> __device__ inline void init(int tid, int dim, Offset offset) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = tid + i * THREADS, r = at / S::kPieces, c = (at % S::kPieces) * S::kPiece;
-      const T* p = row(r);
-      uintx4 x = {0, 0, 0, 0};
-      if (p && c < dim) x = *(const uintx4*)(p + c);
-      v[i] = x;
+    for (int i = 0; i < (kScalar ? 1 : kEach); ++i) {
+      const int n = tid + i * THREADS, r = n / S::kPieces, c = (n % S::kPieces) * S::kPiece;
+      at[i] = c < dim ? (uint32_t)(offset(r) + c) * (uint32_t)sizeof(T) : kNowhere;
     }
+    apart = kScalar ? (uint32_t)offset(THREADS / S::kPieces) * (uint32_t)sizeof(T) : 0;
+  }
+  __device__ inline uintx4 piece(__amdgpu_buffer_rsrc_t buf, int i, bool ok) const {
+    const uint32_t o = at[kScalar ? 0 : i];
+    return __builtin_amdgcn_raw_buffer_load_b128(buf, ok ? o : kNowhere, kScalar ? i * apart : 0, 0);
+  }
+  // the tile's first `rows` rows
+  __device__ inline void load(const T* base, int tid, int rows) {
+    const __amdgpu_buffer_rsrc_t buf = buffer_at(base);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) v[i] = piece(buf, i, row_of(tid, i) < rows);
+  }
+  __device__ inline void load_live(const T* base, int tid, uint64_t live) {
+    const __amdgpu_buffer_rsrc_t buf = buffer_at(base);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) v[i] = piece(buf, i, live >> row_of(tid, i) & 1);
   }
   __device__ inline void store(T* tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int at = tid + i * THREADS, r = at / S::kPieces, c = (at % S::kPieces) * S::kPiece;
-      *(uintx4*)(tile + r * S::kPitch + c) = v[i];
+      const int c = (kScalar ? tid : tid + i * THREADS) % S::kPieces * S::kPiece;
+      *(uintx4*)(tile + row_of(tid, i) * S::kPitch + c) = v[i];
     }
   }
 };
+
+// The keys of a tile that exist and are not masked, bit i for key j0 + i: the same in every wavefront
+template <int KEYS> __device__ inline uint64_t live_keys(const unsigned char* mask, int j0, int keys) {
+  const int n = keys - j0, lane = threadIdx.x & 63;
+  uint64_t live = n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0;
+  if (mask) live &= __ballot(lane < KEYS && lane < n && mask[j0 + lane] != 0);
+  return live;
+}
 
 __device__ inline float wave_max(float x) {
 #pragma unroll
@@ -240,10 +299,11 @@ struct Softmax { float m, l; };
 
 // One row again, visible terms only: for rows whose result is not finite.  The products above multiply the
 // values of keys that a row does not see by a probability of zero, which is no zero where such a value is
-// infinite or NaN.  `tiles` (first tile, last tile, sink tiles, keys a tile) are those of this workgroup.
-template <typename T, int DP>
-__device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& s, int kv, int row, int v0, int v1, int sink_tiles,
-    int t0, int key_tile, Softmax* st, float (&o)[(DP + 63) / 64]) {
+// infinite or NaN.
+template <typename T, int DP, int QW>
+__device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& s, int kv, int row, int split, int tiles, int sink_tiles,
+    int t0, Softmax* st, float (&o)[(DP + 63) / 64]) {
+  constexpr int key_tile = QW == 4 ? 64 : 32, kWays = QW == 4 ? 1 : 4;
   const ocnn_attention_params& p = a.p;
   const int lane = threadIdx.x & 63;
   const int token = row / a.group, head = kv * a.group + row % a.group;
@@ -252,7 +312,10 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
   float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
   for (int i = 0; i < (DP + 63) / 64; ++i) o[i] = 0.0f;
-  for (int v = v0; v < v1; ++v) {
+  for (int n = 0;; ++n) {
+    const int v = (n / kWays * a.splits + split) * kWays + n % kWays;      // the tiles of this workgroup in turn
+    if (v - n % kWays >= tiles) break;
+    if (v >= tiles) continue;
     const int j0 = (v < sink_tiles ? v : t0 + v - sink_tiles) * key_tile;
     const int j = j0 + lane;
     bool see = lane < key_tile && j < hi && (j >= lo || j < p.sinks);
@@ -262,7 +325,7 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
       const T* k = (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head;
       float dot = 0.0f;
       for (int c = 0; c < p.dim; ++c) dot = fmaf(to_f32(q[c]), to_f32(k[c]), dot);
-      x = dot * a.scale2;
+      x = dot * (p.scale < 0.0f ? -a.scale2 : a.scale2);
     }
     uint64_t left = __ballot(see);
     if (!left) continue;
@@ -288,14 +351,14 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
 }
 
 template <typename T, int DP, int QW, bool SPLIT>
-__global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? FWD_W : 2))) attention_kernel(AttnArgs a) {
   using S = Shape<T, DP>;
   using F = ForwardShape<T, DP, QW>;
   constexpr int kRows = 32 * QW, kShift = Log2<kRows>::value;
   __shared__ __attribute__((aligned(16))) char lds[F::kLds];
   __shared__ Softmax stats[4][32];
   const ocnn_attention_params& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y, split = SPLIT ? blockIdx.z : 0;
   const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, blockIdx.x, kShift, a.group);
   const int q_begin = clamped(p.q_offsets, b, p.rows_q);
@@ -353,12 +416,10 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
   // tiles of the sinks in front of the window's: their keys are visible up to what causality allows
   const int sink_tiles = min((min(p.sinks, b_hi) + KT - 1) / KT, t0);
   const int tiles = sink_tiles + t1 - t0;
-  const int v0 = SPLIT ? (int)((int64_t)tiles * split / a.splits) : 0;
-  const int v1 = SPLIT ? (int)((int64_t)tiles * (split + 1) / a.splits) : tiles;
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
 
   Column<T, DP> q;
-  load_row<T, DP>(q, (const T*)p.q + out_at * p.q_row + head * p.q_head, have, p.dim);
+  load_row<T, DP>(q, (const T*)p.q + out_at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   floatx16 o[S::kBlocks];
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d) o[d] = zero16();
@@ -368,29 +429,37 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
   const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
   const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
 
-  // scores of 32 keys from j0 on against this wavefront's rows -> probabilities -> o
-  auto subtile = [&](const T* kt, const T* vt, int j0) {
-    const bool reach = (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi);
-    if (!reach) return;
-    floatx16 x = rows_times<T, DP>(kt, q, zero16());
-    const bool whole = j0 >= all_lo && j0 + 32 <= all_hi && !mask;
-    if (!whole) {
-      uint32_t live = ~0u;
-      if (mask) live = (uint32_t)__ballot(j0 + col < s.keys && mask[min(j0 + col, s.keys - 1)] != 0);
+  // N x 32 keys from j0 on against this wavefront's rows: scores -> probabilities -> o.  The base of the
+  // exponentials follows the running maximum only when that has grown by more than 8 (a factor of 2^8, which 32-bit
+  // sums and bf16 weights hold without loss): the values kept are rescaled a few times a row instead of in
+  // most tiles, and lanes compare without exchanging their maxima.
+  auto keys = [&](auto n, const T* kt, const T* vt, int j0, uint64_t live) {
+    constexpr int N = n.value;
+    floatx16 x[N];
+    const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
+    const bool masked = decided((j0 < all_lo) | (j0 + 32 * N > all_hi) | ((live & all) != all));
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = j0 + acc_row(r);
-        const bool see = j < hi && (j >= lo || j < sinks) && (live >> acc_row(r) & 1);
-        x[r] = see ? x[r] : -__builtin_inff();
-      }
+    for (int i = 0; i < N; ++i) x[i] = rows_times<T, DP>(kt + i * 32 * S::kPitch, q, zero16());
+    if (masked) {
+      settle();
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + 32 * i + acc_row(r);
+          const bool see = (j < hi) & ((j >= lo) | (j < sinks)) & (int)(live >> (32 * i + acc_row(r)) & 1);
+          x[i][r] = see ? x[i][r] : -__builtin_inff();
+        }
     }
-    float top = x[0];
+    float top = x[0][0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale2;
-    const float to = fmaxf(m, top), base = to == -__builtin_inff() ? 0.0f : to;
-    if (__any(to != m)) {
-      const float shrink = __builtin_amdgcn_exp2f(m - base);
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, x[i][r]);
+    top *= a.scale2;
+    if (__any(top > m + 8.0f)) {
+      const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      const float shrink = __builtin_amdgcn_exp2f(m - (to == -__builtin_inff() ? 0.0f : to));
       l *= shrink;
 #pragma unroll
       for (int d = 0; d < S::kBlocks; ++d)
@@ -398,64 +467,85 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
         for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
       m = to;
     }
+    const float base = m == -__builtin_inff() ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -base));
-      sum += x[r];
-    }
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], a.scale2, -base));
+        sum += x[i][r];
+      }
     l += sum;
-    columns_times<DP>(o, vt, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) columns_times<DP>(o, vt + i * 32 * S::kPitch, x[i]);
   };
+  auto reach = [&](int j0) { return (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi); };
 
   if constexpr (QW == 4) {
-    Staged<T, DP, KT, 256> sk, sv;
+    Staged<T, DP, KT, 256, true> sk, sv;
+    sk.init(tid, p.dim, [&](int r) { return r * (int)p.k_row; });
+    sv.init(tid, p.dim, [&](int r) { return r * (int)p.v_row; });
+    uint64_t next = 0;
     auto fetch = [&](int v) {
       const int j0 = tile_key(v);
-      sk.load(tid, p.dim, [&](int r) -> const T* {
-        const int j = j0 + r;
-        return j < s.keys && (!mask || mask[j]) ? kbase + (int64_t)j * p.k_row : nullptr;
-      });
-      sv.load(tid, p.dim, [&](int r) -> const T* {
-        const int j = j0 + r;
-        return j < s.keys && (!mask || mask[j]) ? vbase + (int64_t)j * p.v_row : nullptr;
-      });
+      next = live_keys<KT>(mask, j0, s.keys);
+      if (mask) {
+        sk.load_live(kbase + (int64_t)j0 * p.k_row, tid, next);
+        sv.load_live(vbase + (int64_t)j0 * p.v_row, tid, next);
+      } else {
+        sk.load(kbase + (int64_t)j0 * p.k_row, tid, s.keys - j0);
+        sv.load(vbase + (int64_t)j0 * p.v_row, tid, s.keys - j0);
+      }
     };
-    if (v0 < v1) fetch(v0);
-    for (int v = v0; v < v1; ++v) {
-      T* kt = (T*)lds + (v & 1) * 2 * F::kTile;
+    const int step = SPLIT ? a.splits : 1;
+    if (split < tiles) fetch(split);
+    int buf = 0;
+    for (int v = split; v < tiles; v += step, buf ^= 1) {
+      T* kt = (T*)lds + buf * 2 * F::kTile;
       T* vt = kt + F::kTile;
       sk.store(kt, tid);
       sv.store(vt, tid);
+      const uint64_t live = next;
       __syncthreads();                        // (the other buffer's readers are done: they passed the last barrier)
-      if (v + 1 < v1) fetch(v + 1);
+      if (v + step < tiles) fetch(v + step);
       const int j0 = tile_key(v);
-      subtile(kt, vt, j0);
-      subtile(kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32);
+      const bool first = reach(j0), second = reach(j0 + 32);
+      if (first && second) keys(std::integral_constant<int, 2>(), kt, vt, j0, live);
+      else if (first) keys(std::integral_constant<int, 1>(), kt, vt, j0, live);
+      else if (second) keys(std::integral_constant<int, 1>(), kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32, live >> 32);
     }
   } else {
-    Staged<T, DP, KT, 64> sk, sv;
+    Staged<T, DP, KT, 64, true> sk, sv;
+    sk.init(lane, p.dim, [&](int r) { return r * (int)p.k_row; });
+    sv.init(lane, p.dim, [&](int r) { return r * (int)p.v_row; });
+    uint64_t next = 0;
     auto fetch = [&](int v) {
       const int j0 = tile_key(v);
-      sk.load(lane, p.dim, [&](int r) -> const T* {
-        const int j = j0 + r;
-        return j < s.keys && (!mask || mask[j]) ? kbase + (int64_t)j * p.k_row : nullptr;
-      });
-      sv.load(lane, p.dim, [&](int r) -> const T* {
-        const int j = j0 + r;
-        return j < s.keys && (!mask || mask[j]) ? vbase + (int64_t)j * p.v_row : nullptr;
-      });
+      next = live_keys<KT>(mask, j0, s.keys);
+      if (mask) {
+        sk.load_live(kbase + (int64_t)j0 * p.k_row, lane, next);
+        sv.load_live(vbase + (int64_t)j0 * p.v_row, lane, next);
+      } else {
+        sk.load(kbase + (int64_t)j0 * p.k_row, lane, s.keys - j0);
+        sv.load(vbase + (int64_t)j0 * p.v_row, lane, s.keys - j0);
+      }
     };
     T* kt = (T*)lds + wave * 2 * F::kTile;
     T* vt = kt + F::kTile;
-    if (v0 + wave < v1) fetch(v0 + wave);
-    for (int v = v0 + wave; v < v1; v += 4) {
+    // (the splits take turns: at any time the workgroups together read one stretch of the keys, which spreads
+    // over all memory channels; shares of their own, a power of two apart, met on a few of them)
+    const int first = split * 4 + wave, step = 4 * (SPLIT ? a.splits : 1);
+    if (first < tiles) fetch(first);
+    for (int v = first; v < tiles; v += step) {
       wave_lds_fence();
       sk.store(kt, lane);
       sv.store(vt, lane);
+      const uint64_t live = next;
       wave_lds_fence();
-      if (v + 4 < v1) fetch(v + 4);
-      subtile(kt, vt, tile_key(v));
+      if (v + step < tiles) fetch(v + step);
+      const int j0 = tile_key(v);
+      if (reach(j0)) keys(std::integral_constant<int, 1>(), kt, vt, j0, live);
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -537,7 +627,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
     const int r = __shfl(row, c, 64);
     Softmax st;
     float oo[(DP + 63) / 64];
-    forward_row_again<T, DP>(a, s, kv, r, v0, v1, sink_tiles, t0, KT, &st, oo);
+    forward_row_again<T, DP, QW>(a, s, kv, r, split, tiles, sink_tiles, t0, &st, oo);
     const int tk = r / a.group, hd = kv * a.group + r % a.group;
     const int64_t at = (int64_t)(s.q0 + tk) * p.heads + hd;
 #pragma unroll
@@ -643,7 +733,7 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
         dot = fmaf(to_f32(q[c]), to_f32(k[c]), dot);
         dp = fmaf(to_f32(go[c]), to_f32(vr[c]), dp);
       }
-      ds = exp2f(fmaf(dot, a.scale2, -lse2)) * (dp - delta);
+      ds = exp2f(fmaf(dot, p.scale < 0.0f ? -a.scale2 : a.scale2, -lse2)) * (dp - delta);
     }
     uint64_t left = __ballot(see);
     while (left) {
@@ -659,12 +749,12 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) attention_grad_q_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? GQ_W : 2))) attention_grad_q_kernel(AttnArgs a) {
   using S = Shape<T, DP>;
   constexpr int KT = 64, kTile = KT * S::kPitch, kRows = 128, kShift = 7;
   __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
   const ocnn_attention_params& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y;
   const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, blockIdx.x, kShift, a.group);
   const int q_begin = clamped(p.q_offsets, b, p.rows_q);
@@ -716,7 +806,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
 #pragma unroll
     for (int e = 0; e < S::kPiece; ++e) delta = fmaf((float)q.v[i][e], (float)go.v[i][e], delta);
   delta += __shfl_xor(delta, 32, 64);
-  load_row<T, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim);
+  load_row<T, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   const int64_t at_row = at * p.heads + head;
   const float lse = have ? a.lse[at_row] : -__builtin_inff();
   const float lse2 = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
@@ -729,37 +819,47 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
   const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
   const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
 
-  auto subtile = [&](const T* kt, const T* vt, int j0) {
-    const bool reach = (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi);
-    if (!reach) return;
-    floatx16 x = rows_times<T, DP>(kt, q, zero16());
-    const floatx16 dp = rows_times<T, DP>(vt, go, zero16());
+  auto reach = [&](int j0) { return (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi); };
+  auto keys = [&](auto n, const T* kt, const T* vt, int j0, uint64_t live) {
+    constexpr int N = n.value;
+    floatx16 x[N];
+    const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
+    const bool masked = decided((j0 < all_lo) | (j0 + 32 * N > all_hi) | ((live & all) != all));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -lse2)) * (dp[r] - delta);
-    if (!(j0 >= all_lo && j0 + 32 <= all_hi && !mask)) {
-      uint32_t live = ~0u;
-      if (mask) live = (uint32_t)__ballot(j0 + col < s.keys && mask[min(j0 + col, s.keys - 1)] != 0);
+    for (int i = 0; i < N; ++i) {
+      x[i] = rows_times<T, DP>(kt + i * 32 * S::kPitch, q, zero16());
+      const floatx16 dp = rows_times<T, DP>(vt + i * 32 * S::kPitch, go, zero16());
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = j0 + acc_row(r);
-        const bool see = j < hi && (j >= lo || j < sinks) && (live >> acc_row(r) & 1);
-        x[r] = see ? x[r] : 0.0f;
-      }
+      for (int r = 0; r < 16; ++r) x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], a.scale2, -lse2)) * (dp[r] - delta);
     }
-    columns_times<DP>(dq, kt, x);
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + 32 * i + acc_row(r);
+          const bool see = (j < hi) & ((j >= lo) | (j < sinks)) & (int)(live >> (32 * i + acc_row(r)) & 1);
+          x[i][r] = see ? x[i][r] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) columns_times<DP>(dq, kt + i * 32 * S::kPitch, x[i]);
   };
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
-  Staged<T, DP, KT, 256> sk, sv;
+  Staged<T, DP, KT, 256, true> sk, sv;
+  sk.init(tid, p.dim, [&](int r) { return r * (int)p.k_row; });
+  sv.init(tid, p.dim, [&](int r) { return r * (int)p.v_row; });
+  uint64_t next = 0;
   auto fetch = [&](int v) {
     const int j0 = tile_key(v);
-    sk.load(tid, p.dim, [&](int r) -> const T* {
-      const int j = j0 + r;
-      return j < s.keys && (!mask || mask[j]) ? kbase + (int64_t)j * p.k_row : nullptr;
-    });
-    sv.load(tid, p.dim, [&](int r) -> const T* {
-      const int j = j0 + r;
-      return j < s.keys && (!mask || mask[j]) ? vbase + (int64_t)j * p.v_row : nullptr;
-    });
+    next = live_keys<KT>(mask, j0, s.keys);
+    if (mask) {
+      sk.load_live(kbase + (int64_t)j0 * p.k_row, tid, next);
+      sv.load_live(vbase + (int64_t)j0 * p.v_row, tid, next);
+    } else {
+      sk.load(kbase + (int64_t)j0 * p.k_row, tid, s.keys - j0);
+      sv.load(vbase + (int64_t)j0 * p.v_row, tid, s.keys - j0);
+    }
   };
   if (tiles > 0) fetch(0);
   for (int v = 0; v < tiles; ++v) {
@@ -767,11 +867,14 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 && DP > 64) ? 1 : 2) atte
     T* vt = kt + kTile;
     sk.store(kt, tid);
     sv.store(vt, tid);
+    const uint64_t live = next;
     __syncthreads();
     if (v + 1 < tiles) fetch(v + 1);
     const int j0 = tile_key(v);
-    subtile(kt, vt, j0);
-    subtile(kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32);
+    const bool first = reach(j0), second = reach(j0 + 32);
+    if (first && second) keys(std::integral_constant<int, 2>(), kt, vt, j0, live);
+    else if (first) keys(std::integral_constant<int, 1>(), kt, vt, j0, live);
+    else if (second) keys(std::integral_constant<int, 1>(), kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32, live >> 32);
   }
   float worst = 0.0f;
 #pragma unroll
@@ -843,7 +946,7 @@ __device__ __forceinline__ void grad_k_row_again(const AttnArgs& a, const Seq& s
         dp = fmaf(to_f32(go[c]), to_f32(v[c]), dp);
       }
       const float lse = a.lse[at * p.heads + head];
-      w = exp2f(fmaf(dot, a.scale2, lse == -__builtin_inff() ? 0.0f : -lse * kLog2e));
+      w = exp2f(fmaf(dot, p.scale < 0.0f ? -a.scale2 : a.scale2, lse == -__builtin_inff() ? 0.0f : -lse * kLog2e));
       ds = w * (dp - a.delta[at * p.heads + head]);
     }
     for (int i = 0; i < min(64, to - r0); ++i) {
@@ -870,7 +973,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
   __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
   __shared__ float row_lse[2][RT], row_delta[2][RT];
   const ocnn_attention_params& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y;
   const bool far = (int)blockIdx.x >= near_items;
   int b, j0 = 0;
@@ -937,14 +1040,16 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
     }
   }
   Column<T, DP> k, vv;
-  load_row<T, DP>(k, (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head, key, p.dim);
+  load_row<T, DP>(k, (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head, key, p.dim, p.scale < 0.0f);
   load_row<T, DP>(vv, (const T*)p.v + (int64_t)(s.k0 + j) * p.v_row + kv * p.v_head, key, p.dim);
   floatx16 dk[S::kBlocks], dv[S::kBlocks];
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d) dk[d] = dv[d] = zero16();
 
-  auto subtile = [&](const T* qt, const T* gt, const float* lse2, const float* delta, int r0) {
-    if (r0 + 32 <= w_lo || r0 >= w_hi) return;
+  // 32 packed rows from r0 on, those before `end`
+  auto subtile = [&](const T* qt, const T* gt, const float* lse2, const float* delta, int r0, int end) {
+    if (r0 + 32 <= w_lo || r0 >= min(w_hi, end)) return;
+    const bool masked = decided((r0 < all_lo) | (r0 + 32 > min(all_hi, end)));
     floatx16 x = rows_times<T, DP>(qt, k, zero16());
     floatx16 dp = rows_times<T, DP>(gt, vv, zero16());
     floatx4 ls[4], de[4];
@@ -953,17 +1058,17 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
       ls[i] = *(const floatx4*)(lse2 + 8 * i + 4 * half);
       de[i] = *(const floatx4*)(delta + 8 * i + 4 * half);
     }
-    const bool whole = r0 >= all_lo && r0 + 32 <= all_hi;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -ls[r >> 2][r & 3]));
       dp[r] = x[r] * (dp[r] - de[r >> 2][r & 3]);
     }
-    if (!whole) {
+    if (masked) {
+      const int upto = min(hi, end);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = r0 + acc_row(r);
-        const bool see = row >= lo && row < hi;
+        const bool see = (row >= lo) & (row < upto);
         x[r] = see ? x[r] : 0.0f;
         dp[r] = see ? dp[r] : 0.0f;
       }
@@ -972,28 +1077,27 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
     columns_times<DP>(dk, qt, dp);
   };
 
-  const int ra = ta * a.group, rb = tb * a.group, tiles = s.keys > 0 ? max(rb - ra + RT - 1, 0) / RT : 0;
-  Staged<T, DP, RT, 256> sq, sg;
+  // a tile holds whole tokens: `step` of them, group rows each, so that a thread's rows keep their offsets
+  const int step = RT / a.group, used = step * a.group;
+  const int tiles = s.keys > 0 && tb > ta ? (tb - ta + step - 1) / step : 0;
+  const T* qbase = (const T*)p.q + (int64_t)(s.q0 + ta) * p.q_row + (int64_t)kv * a.group * p.q_head;
+  const T* gbase = (const T*)a.grad + (int64_t)(s.q0 + ta) * a.grad_row + (int64_t)kv * a.group * a.grad_head;
+  Staged<T, DP, RT, 256, false> sq, sg;
+  sq.init(tid, p.dim, [&](int i) { const int t = i / a.group; return t * (int)p.q_row + (i - t * a.group) * (int)p.q_head; });
+  sg.init(tid, p.dim, [&](int i) { const int t = i / a.group; return t * (int)a.grad_row + (i - t * a.group) * (int)a.grad_head; });
+  const int my_token = tid / a.group;
+  const int64_t my_stat = (int64_t)(s.q0 + ta + my_token) * p.heads + kv * a.group + tid - my_token * a.group;
   float one_lse = 0.0f, one_delta = 0.0f;
   auto fetch = [&](int v) {
-    const int r0 = ra + v * RT;
-    sq.load(tid, p.dim, [&](int i) -> const T* {
-      const int r = r0 + i, token = a.group == 1 ? r : r / a.group;
-      return r < rb ? (const T*)p.q + (int64_t)(s.q0 + token) * p.q_row + (kv * a.group + r - token * a.group) * p.q_head : nullptr;
-    });
-    sg.load(tid, p.dim, [&](int i) -> const T* {
-      const int r = r0 + i, token = a.group == 1 ? r : r / a.group;
-      return r < rb ? (const T*)a.grad + (int64_t)(s.q0 + token) * a.grad_row + (kv * a.group + r - token * a.group) * a.grad_head
-                    : nullptr;
-    });
+    const int t = v * step, rows = min(tb - ta - t, step) * a.group;
+    sq.load(qbase + (int64_t)t * p.q_row, tid, used < RT ? min(rows, used) : rows);
+    sg.load(gbase + (int64_t)t * a.grad_row, tid, used < RT ? min(rows, used) : rows);
     if (tid < RT) {
-      const int r = r0 + tid, token = r / a.group;
       one_lse = one_delta = 0.0f;
-      if (r < rb) {
-        const int64_t at = (int64_t)(s.q0 + token) * p.heads + kv * a.group + r - token * a.group;
-        const float lse = a.lse[at];
+      if (tid < rows) {
+        const float lse = a.lse[my_stat + (int64_t)t * p.heads];
         one_lse = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
-        one_delta = a.delta[at];
+        one_delta = a.delta[my_stat + (int64_t)t * p.heads];
       }
     }
   };
@@ -1010,9 +1114,9 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
     }
     __syncthreads();
     if (v + 1 < tiles) fetch(v + 1);
-    const int r0 = ra + v * RT;
-    subtile(qt, gt, row_lse[buf], row_delta[buf], r0);
-    subtile(qt + 32 * S::kPitch, gt + 32 * S::kPitch, row_lse[buf] + 32, row_delta[buf] + 32, r0 + 32);
+    const int r0 = (ta + v * step) * a.group, end = r0 + used;
+    subtile(qt, gt, row_lse[buf], row_delta[buf], r0, end);
+    if (used > 32) subtile(qt + 32 * S::kPitch, gt + 32 * S::kPitch, row_lse[buf] + 32, row_delta[buf] + 32, r0 + 32, end);
   }
 
   float worst = 0.0f;
@@ -1111,6 +1215,7 @@ int check_params(const ocnn_attention_params* p) {
       "%d queries, %d keys, %d sequences (1 .. 65535)", p->rows_q, p->rows_k, p->n_seq);
   OCNN_REQUIRE(p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0 && p->kv_heads <= 65535, OCNN_E_SHAPE,
       "%d query heads over %d key heads", p->heads, p->kv_heads);
+  OCNN_REQUIRE(p->heads / p->kv_heads <= 64, OCNN_E_UNSUPPORTED, "%d query heads a key head: at most 64", p->heads / p->kv_heads);
   OCNN_REQUIRE(p->dim > 0 && p->dim <= 128 && p->dim % 8 == 0, OCNN_E_UNSUPPORTED,
       "%d channels a head: multiples of 8 up to 128", p->dim);
   OCNN_REQUIRE(p->left >= -1 && p->right >= -1, OCNN_E_BADARG, "window %d, %d: -1 for no bound", p->left, p->right);
@@ -1123,8 +1228,11 @@ int check_params(const ocnn_attention_params* p) {
 }
 
 // 16-byte rows: pointers and strides of every row tensor
+// and 64 rows of a group of heads lie within 2^30 elements
 int check_rows(int dtype, const char* name, const void* at, int64_t row, int64_t head) {
   const int64_t piece = dtype == OCNN_F32 ? 4 : 8;
+  OCNN_REQUIRE(row >= 0 && row < (1 << 22) && head >= 0 && head < (1 << 22), OCNN_E_UNSUPPORTED,
+      "%s: strides %lld, %lld: below 2^22 elements", name, (long long)row, (long long)head);
   OCNN_REQUIRE((uintptr_t)at % 16 == 0 && row % piece == 0 && head % piece == 0, OCNN_E_BADARG,
       "%s: rows and heads must begin at multiples of 16 bytes", name);
   return OCNN_OK;
@@ -1141,7 +1249,7 @@ Plan plan_of(const ocnn_attention_params& p) {
   int64_t keys = p.rows_k / p.n_seq;
   if (p.left >= 0 && p.right >= 0) keys = std::min<int64_t>(keys, (int64_t)p.left + p.right + p.rows_q / p.n_seq + p.sinks);
   const int64_t blocks = std::max<int64_t>((packed + (n.few ? 31 : 127)) / (n.few ? 32 : 128), n.few ? p.n_seq : 1) * p.kv_heads;
-  const int64_t most = n.few ? keys / 512 : keys / 1024;
+  const int64_t most = n.few ? keys / 256 : keys / 1024;
   n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, kMaxSplits}));
   return n;
 }
@@ -1166,7 +1274,7 @@ AttnArgs args_of(const ocnn_attention_params& p) {
   a.p.left = std::min(p.left, 1 << 30);
   a.p.right = std::min(p.right, 1 << 30);
   a.group = p.heads / p.kv_heads;
-  a.scale2 = p.scale * kLog2e;
+  a.scale2 = fabsf(p.scale) * kLog2e;
   return a;
 }
 
@@ -1233,8 +1341,8 @@ int ocnn_octree_attention(void* out, int64_t out_row, int64_t out_head, float* l
   OCNN_REQUIRE(need == 0 || (workspace_dev && workspace_bytes >= need && (uintptr_t)workspace_dev % 16 == 0), OCNN_E_WORKSPACE,
       "octree_attention needs %zu bytes, 16-byte aligned, got %zu", need, workspace_bytes);
   AttnArgs a = args_of(p);
-  a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.fill = fill_rest != 0;
   a.splits = n.splits;
+  a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse; a.fill = fill_rest != 0;
   if (n.splits > 1) {
     a.part_o = (float*)workspace_dev;
     a.part_ml = (float*)((char*)workspace_dev + round256((size_t)n.splits * p.rows_q * p.heads * p.dim * 4));

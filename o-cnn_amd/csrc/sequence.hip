@@ -164,19 +164,25 @@ uint32_t reciprocal(uint32_t d) { return d <= 1 ? 0u : (uint32_t)((1ull << 32) /
 
 // ---- gated linear recurrence ----------------------------------------------------------------------
 //   h_t = a_t h_{t-1} + b_t x_t,  a = sigmoid(g), b = 1 - a = sigmoid(-g)
-// The map of a run of rows is (A, H): h -> A h + H, and runs compose.  Three launches:
-//   run    every chunk of L rows of a sequence: its (A, H)           reads g, x
-//   carry  per sequence: the state in front of each chunk            reads and writes 8 bytes / L rows
-//   apply  every chunk again from its state: h                       reads g, x, writes h
-// The chunks' states are folded in a fixed order, so results do not change from run to run (a
-// single pass that takes whatever prefix its predecessors have published would not give that).
+// The map of a run of rows is (A, H): h -> A h + H, and runs compose.  Four launches:
+//   run    every chunk of L rows of a sequence: its (A, H)               reads g, x
+//   group  every 32 chunks: the run in front of each, and of all of them
+//   top    the state in front of every group
+//   apply  every chunk again from its state: h                           reads g, x, writes h
+// The chunks of all sequences are scanned as one list: a run that begins a sequence starts from the caller's
+// state and forgets what came before (A = kReset; no product with it, so a NaN stays in its sequence).
+// group and top move 16 bytes a channel and chunk; they are two launches because one compute unit has too few
+// loads in flight to fetch a long list by itself (262147 rows of 256 channels: 4097 chunks, 69 us in one launch
+// of a workgroup for every 8 channels).
+// States are folded in a fixed order, so results do not change from run to run (a single pass that takes
+// whatever prefix its predecessors have published would not give that).
 // Threads enumerate (chunk, channels) with the channels innermost.  The state is 32 bits throughout.
 // Sequences of a few rows (a step of a running sequence) take one launch, a thread per (sequence,
 // channels) that walks the rows.
 //
 // The gradient, with L_t = dh_t + a_{t+1} L_{t+1} (L_end += the gradient of the last state):
 //   dx = b L,  dg = a b L (h_{t-1} - x),  d state = a_1 L_1
-// runs the same three steps from the other end on (a, dh).  h_{t-1} is computed again from the
+// runs the same steps from the other end on (a, dh).  h_{t-1} is computed again from the
 // chunk's state (kept from the forward pass, 32 bits): the stored h of a bf16 call is rounded, and
 // h_{t-1} - x cancels where a sequence hardly changes.
 
@@ -204,13 +210,24 @@ struct ScanArgs {
   void* grad_gate; void* grad_data;
   int64_t out_row, gate_row, data_row, grad_row, grad_gate_row, grad_data_row;
   const float* state; float* last; const float* grad_last; float* grad_state;
-  float* run_a; float* run_h; float* carry;      // [ids][channels]
+  float* run_a; float* run_h;                     // [ids][channels]
+  float* group_a; float* group_h;                 // [groups of ids][channels]; group_h: then the state in front
+  float* carry;                                   // [ids][channels], kept for the gradient
+  int64_t ids;
   const int* offsets;
   int n_seq, rows, channels, groups, reverse, fill;
   int64_t threads;                                // ids x groups
 };
 
 constexpr int kScanRows = 8;   // rows whose loads are in flight together
+constexpr int kGroupShift = 5, kGroup = 1 << kGroupShift;
+constexpr float kReset = -1.0f;   // (products of sigmoids are not negative)
+
+// the run (A, H) behind the run (a, h)
+__device__ inline void compose(float& A, float& H, float a, float h) {
+  H = a < 0.0f ? h : fmaf(a, H, h);
+  A = a < 0.0f || A < 0.0f ? kReset : A * a;
+}
 
 // The rows of chunk `id`: their sequence, where they begin and how many there are.
 struct Chunk {
@@ -235,9 +252,20 @@ template <int L> __device__ inline Chunk chunk_of(const ScanArgs& a, int64_t id)
   return c;
 }
 
-// ids whose chunk is the first one of its sequence's chunk ids
-__device__ inline int64_t first_id(const ScanArgs& a, int seq, int shift) {
-  return (int64_t)(clamped(a.offsets, seq, a.rows) >> shift) + seq;
+template <int V> __device__ inline void put_run(const ScanArgs& a, int64_t id, int c0, const float* A, const float* H) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    a.run_a[id * a.channels + c0 + v] = A[v];
+    a.run_h[id * a.channels + c0 + v] = H[v];
+  }
+}
+// the state in front of a chunk that does not begin its sequence (back: behind one that does not end it)
+template <int V> __device__ inline void state_at(const ScanArgs& a, int64_t id, int c0, float* h) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float A = a.run_a[id * a.channels + c0 + v], H = a.run_h[id * a.channels + c0 + v];
+    h[v] = A < 0.0f ? H : fmaf(A, a.group_h[(id >> kGroupShift) * a.channels + c0 + v], H);
+  }
 }
 
 template <typename T, int V, int L>
@@ -247,13 +275,16 @@ __global__ void __launch_bounds__(kBlock) scan_run_kernel(ScanArgs a) {
   const int64_t id = i / a.groups;
   const int c0 = (int)(i - id * a.groups) * V;
   const Chunk ch = chunk_of<L>(a, id);
-  // (the run of a sequence's last chunk is not needed by anything)
-  if (!ch.live || ch.seq >= a.n_seq || (int64_t)(ch.index + 1) * L >= ch.length) return;
   const T* gate = (const T*)a.gate + c0;
   const T* data = (const T*)a.data + c0;
   float A[V], H[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) { A[v] = 1.0f; H[v] = 0.0f; }
+  // (what a sequence's last chunk does to the state matters to no other chunk)
+  if (!ch.live || ch.seq >= a.n_seq || (int64_t)(ch.index + 1) * L >= ch.length) {
+    put_run<V>(a, id, c0, A, H);
+    return;
+  }
   for (int t = 0; t < L; t += kScanRows) {       // the chunk is full: it is not its sequence's last
     Pack<T, V> g[kScanRows], x[kScanRows];
 #pragma unroll
@@ -272,11 +303,13 @@ __global__ void __launch_bounds__(kBlock) scan_run_kernel(ScanArgs a) {
         A[v] *= p;
       }
   }
+  if (ch.index == 0)
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    a.run_a[id * a.channels + c0 + v] = A[v];
-    a.run_h[id * a.channels + c0 + v] = H[v];
-  }
+    for (int v = 0; v < V; ++v) {
+      if (a.state) H[v] = fmaf(A[v], a.state[(int64_t)ch.seq * a.channels + c0 + v], H[v]);
+      A[v] = kReset;
+    }
+  put_run<V>(a, id, c0, A, H);
 }
 
 // The same from the other end for the gradient: m = a (dh + m'), m' from the row behind.  Runs of the chunks
@@ -288,12 +321,15 @@ __global__ void __launch_bounds__(kBlock) scan_run_back_kernel(ScanArgs a) {
   const int64_t id = i / a.groups;
   const int c0 = (int)(i - id * a.groups) * V;
   const Chunk ch = chunk_of<L>(a, id);
-  if (!ch.live || ch.seq >= a.n_seq || ch.index == 0) return;
   const T* gate = (const T*)a.gate + c0;
   const T* grad = (const T*)a.grad + c0;
   float A[V], M[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) { A[v] = 1.0f; M[v] = 0.0f; }
+  if (!ch.live || ch.seq >= a.n_seq || ch.index == 0) {
+    put_run<V>(a, id, c0, A, M);
+    return;
+  }
   for (int t = L - kScanRows; t >= 0; t -= kScanRows) {
     if (t >= ch.count) continue;
     Pack<T, V> g[kScanRows], d[kScanRows];
@@ -314,67 +350,99 @@ __global__ void __launch_bounds__(kBlock) scan_run_back_kernel(ScanArgs a) {
           A[v] *= p;
         }
   }
+  if ((int64_t)(ch.index + 1) * L >= ch.length)
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    a.run_a[id * a.channels + c0 + v] = A[v];
-    a.run_h[id * a.channels + c0 + v] = M[v];
-  }
+    for (int v = 0; v < V; ++v) {
+      if (a.grad_last) M[v] = fmaf(A[v], a.grad_last[(int64_t)ch.seq * a.channels + c0 + v], M[v]);
+      A[v] = kReset;
+    }
+  put_run<V>(a, id, c0, A, M);
 }
 
-// The state in front of each chunk of a sequence: kSegments threads a channel fold a share of the runs
-// each, the shares are folded in order, and each thread walks its share again writing the states.
-// A workgroup serves 8 channels (32 bytes a run: the smallest piece memory moves) of one sequence, so that
-// one long sequence still has a workgroup for every 8 channels; a share of up to kHeld runs stays in
-// registers between the two walks (262147 rows of 256 channels: 16 runs of 128 rows a thread).
-constexpr int kCarryChannels = 8, kSegments = 128, kHeld = 16;
+// In place: the run of each chunk -> the run of the chunks of its group in front of it (back: behind it).
+template <bool BACK>
+__global__ void __launch_bounds__(64) scan_group_kernel(ScanArgs a) {
+  const int64_t id0 = (int64_t)blockIdx.x << kGroupShift;
+  const int n = (int)min((int64_t)kGroup, a.ids - id0);
+  const int c = blockIdx.y * 64 + threadIdx.x;
+  if (c >= a.channels) return;
+  float ra[kGroup], rh[kGroup];
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {             // (no branch a load: they are in flight together)
+    const int64_t o = (id0 + min(i, n - 1)) * a.channels + c;
+    ra[i] = a.run_a[o];
+    rh[i] = a.run_h[o];
+  }
+  float A = 1.0f, H = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kGroup; ++k) {
+    const int i = BACK ? kGroup - 1 - k : k;
+    if (i >= n) continue;
+    const int64_t o = (id0 + i) * a.channels + c;
+    a.run_a[o] = A;
+    a.run_h[o] = H;
+    compose(A, H, ra[i], rh[i]);
+  }
+  a.group_a[blockIdx.x * (int64_t)a.channels + c] = A;
+  a.group_h[blockIdx.x * (int64_t)a.channels + c] = H;
+}
 
-template <int SHIFT, bool BACK>
-__global__ void __launch_bounds__(kCarryChannels * kSegments) scan_carry_kernel(ScanArgs a) {
-  __shared__ float sa[kSegments][kCarryChannels], sh[kSegments][kCarryChannels];
-  const int seq = blockIdx.y, lane = threadIdx.x % kCarryChannels, seg = threadIdx.x / kCarryChannels;
-  const int c = blockIdx.x * kCarryChannels + lane;
-  const int begin = clamped(a.offsets, seq, a.rows), end = clamped(a.offsets, seq + 1, a.rows);
-  const int chunks = (max(end - begin, 0) + (1 << SHIFT) - 1) >> SHIFT;
-  if (chunks < 2) return;                       // its only chunk starts from the caller's state
-  const int64_t id0 = first_id(a, seq, SHIFT);
-  const int share = (chunks + kSegments - 1) / kSegments;
-  const int from = min(seg * share, chunks), to = min(from + share, chunks);
+// group_h: the run of each group -> the state in front of it (back: behind it).  32 threads a channel fold a
+// share of the groups each, the shares are combined by doubling, and each thread walks its share again.
+constexpr int kTopChannels = 32, kTopShares = 32, kHeld = 8;
+
+template <bool BACK>
+__global__ void __launch_bounds__(kTopChannels * kTopShares) scan_top_kernel(ScanArgs a) {
+  __shared__ float sa[kTopShares][kTopChannels], sh[kTopShares][kTopChannels];
+  const int lane = threadIdx.x % kTopChannels, seg = threadIdx.x / kTopChannels;
+  const int c = blockIdx.x * kTopChannels + lane;
+  const int groups = (int)((a.ids + kGroup - 1) >> kGroupShift);
+  const int share = (groups + kTopShares - 1) / kTopShares;
+  const int from = min(seg * share, groups), to = min(from + share, groups);
   const bool mine = c < a.channels;
-  // chunk j in the order of the walk; the run of the walk's last chunk does not exist
-  auto at = [&](int j) { return (id0 + (BACK ? chunks - 1 - j : j)) * a.channels + c; };
+  auto at = [&](int j) { return (int64_t)(BACK ? groups - 1 - j : j) * a.channels + c; };
   float ra[kHeld], rh[kHeld];
   auto load = [&](int j0) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-      const bool ok = mine && j0 + i < min(to, chunks - 1);
-      ra[i] = ok ? a.run_a[at(j0 + i)] : 1.0f;
-      rh[i] = ok ? a.run_h[at(j0 + i)] : 0.0f;
+      const int64_t o = at(min(j0 + i, to - 1));
+      ra[i] = a.group_a[o];
+      rh[i] = a.group_h[o];
     }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (j0 + i >= to) { ra[i] = 1.0f; rh[i] = 0.0f; }
   };
   float A = 1.0f, H = 0.0f;
-  for (int j = from; j < to; j += kHeld) {
-    load(j);
+  if (mine)
+    for (int j = from; j < to; j += kHeld) {
+      load(j);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      H = fmaf(ra[i], H, rh[i]);
-      A *= ra[i];
+      for (int i = 0; i < kHeld; ++i) compose(A, H, ra[i], rh[i]);
     }
-  }
   sa[seg][lane] = A;
   sh[seg][lane] = H;
+  for (int d = 1; d < kTopShares; d <<= 1) {
+    __syncthreads();
+    float fa = 1.0f, fh = 0.0f;
+    if (seg >= d) { fa = sa[seg - d][lane]; fh = sh[seg - d][lane]; }
+    __syncthreads();
+    compose(fa, fh, A, H);
+    A = fa;
+    H = fh;
+    sa[seg][lane] = A;
+    sh[seg][lane] = H;
+  }
   __syncthreads();
-  const float* start = BACK ? a.grad_last : a.state;
-  float h = mine && start ? start[(int64_t)seq * a.channels + c] : 0.0f;
-  for (int s = 0; s < seg; ++s) h = fmaf(sa[s][lane], h, sh[s][lane]);
   if (!mine) return;
-  float* carry = BACK ? a.run_h : a.carry;       // (back: in place, a share is read before it is written)
+  float h = seg ? sh[seg - 1][lane] : 0.0f;       // (the list begins with a sequence: nothing comes before it)
   for (int j = from; j < to; j += kHeld) {
     if (share > kHeld) load(j);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
       if (j + i < to) {
-        carry[at(j + i)] = h;
-        h = fmaf(ra[i], h, rh[i]);
+        a.group_h[at(j + i)] = h;
+        h = ra[i] < 0.0f ? rh[i] : fmaf(ra[i], h, rh[i]);
       }
   }
 }
@@ -401,10 +469,15 @@ __global__ void __launch_bounds__(kBlock) scan_apply_kernel(ScanArgs a) {
   const T* gate = (const T*)a.gate + c0;
   const T* data = (const T*)a.data + c0;
   float h[V];
+  if (ch.index) {
+    state_at<V>(a, id, c0, h);
+    if (a.carry)
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    h[v] = ch.index ? a.carry[id * a.channels + c0 + v]
-                    : a.state ? a.state[(int64_t)ch.seq * a.channels + c0 + v] : 0.0f;
+      for (int v = 0; v < V; ++v) a.carry[id * a.channels + c0 + v] = h[v];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = a.state ? a.state[(int64_t)ch.seq * a.channels + c0 + v] : 0.0f;
+  }
   for (int t = 0; t < ch.count; t += kScanRows) {
     Pack<T, V> g[kScanRows], x[kScanRows];
 #pragma unroll
@@ -459,8 +532,9 @@ __global__ void __launch_bounds__(kBlock) scan_apply_back_kernel(ScanArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     h[v] = ch.index ? a.carry[id * a.channels + c0 + v] : a.state ? a.state[at_seq + v] : 0.0f;
-    m[v] = !is_last ? a.run_h[id * a.channels + c0 + v] : a.grad_last ? a.grad_last[at_seq + v] : 0.0f;
+    m[v] = is_last && a.grad_last ? a.grad_last[at_seq + v] : 0.0f;
   }
+  if (!is_last) state_at<V>(a, id, c0, m);
 #pragma unroll
   for (int s = 0; s < kGroups; ++s) {
 #pragma unroll
@@ -581,13 +655,23 @@ __global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
 // channel and chunk, and the carry step is short), few where it does not.  The rule sees sizes that the
 // forward and the backward call share, so their chunks are the same.
 int scan_shift(int64_t rows, int64_t channels) {
-  return rows * channels >= (int64_t)1 << 25 ? 7 : rows * channels >= (int64_t)1 << 22 ? 6 : 4;
+  return rows * channels >= (int64_t)1 << 22 ? 6 : 4;
 }
 
 // sequences of 16 rows and fewer on average: one launch that walks them
 bool scan_walks(int64_t rows, int64_t n_seq, bool carries) { return !carries && rows <= 16 * n_seq; }
 
 int64_t scan_ids(int64_t rows, int n_seq, int shift) { return (rows >> shift) + n_seq + 1; }
+
+// the lists of runs in a workspace
+void scan_lists(ScanArgs* a, int64_t ids, void* workspace) {
+  const size_t one = (size_t)ids * a->channels, groups = (size_t)((ids + kGroup - 1) >> kGroupShift) * a->channels;
+  a->ids = ids;
+  a->run_a = (float*)workspace;
+  a->run_h = a->run_a + one;
+  a->group_a = a->run_h + one;
+  a->group_h = a->group_a + groups;
+}
 
 // V channels a thread: wide loads where every row allows them and the chip stays full
 int scan_width(const ScanArgs& a, int size, std::initializer_list<std::pair<const void*, int64_t>> tensors, int64_t ids) {
@@ -600,12 +684,17 @@ int scan_width(const ScanArgs& a, int size, std::initializer_list<std::pair<cons
   return v;
 }
 
+template <bool BACK> void scan_lists_launch(const ScanArgs& a, hipStream_t s) {
+  const unsigned groups = (unsigned)((a.ids + kGroup - 1) >> kGroupShift);
+  scan_group_kernel<BACK><<<dim3(groups, (a.channels + 63) / 64), 64, 0, s>>>(a);
+  scan_top_kernel<BACK><<<(a.channels + kTopChannels - 1) / kTopChannels, kTopChannels * kTopShares, 0, s>>>(a);
+}
+
 template <typename T, int V, int L>
 void scan_forward_launch(const ScanArgs& a, hipStream_t s) {
   const unsigned blocks = blocks_for(a.threads);
   scan_run_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
-  scan_carry_kernel<Log2<L>::value, false><<<dim3((a.channels + kCarryChannels - 1) / kCarryChannels, a.n_seq),
-      kCarryChannels * kSegments, 0, s>>>(a);
+  scan_lists_launch<false>(a, s);
   scan_apply_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
 }
 
@@ -613,8 +702,7 @@ template <typename T, int V, int L>
 void scan_backward_launch(const ScanArgs& a, hipStream_t s) {
   const unsigned blocks = blocks_for(a.threads);
   scan_run_back_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
-  scan_carry_kernel<Log2<L>::value, true><<<dim3((a.channels + kCarryChannels - 1) / kCarryChannels, a.n_seq),
-      kCarryChannels * kSegments, 0, s>>>(a);
+  scan_lists_launch<true>(a, s);
   scan_apply_back_kernel<T, V, L><<<blocks, kBlock, 0, s>>>(a);
 }
 
@@ -625,8 +713,7 @@ template <typename F> void by_width(int v, F f) {
 }
 
 template <typename F> void by_chunk(int shift, F f) {
-  if (shift == 7) f(std::integral_constant<int, 128>());
-  else if (shift == 6) f(std::integral_constant<int, 64>());
+  if (shift == 6) f(std::integral_constant<int, 64>());
   else f(std::integral_constant<int, 16>());
 }
 
@@ -724,10 +811,11 @@ int ocnn_recurrence_shape(int rows, int channels, int n_seq, int carries, int64_
   OCNN_REQUIRE(rows >= 0 && channels > 0 && n_seq >= 1 && n_seq <= 65535, OCNN_E_BADARG, "rows %d, channels %d, sequences %d",
       rows, channels, n_seq);
   const int64_t ids = scan_ids(rows, n_seq, scan_shift(rows, channels));
-  const size_t one = (size_t)ids * channels * sizeof(float);
+  const size_t lists = 2 * (size_t)(ids + ((ids + kGroup - 1) >> kGroupShift)) * channels * sizeof(float);
+  OCNN_REQUIRE(ids < (1ll << 31) && (channels + 63) / 64 <= 65535, OCNN_E_UNSUPPORTED, "%d rows of %d channels", rows, channels);
   if (carry_rows) *carry_rows = ids;
-  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) ? 0 : (carries ? 2 : 3) * one;
-  if (grad_workspace_bytes) *grad_workspace_bytes = 2 * one;
+  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) ? 0 : lists;
+  if (grad_workspace_bytes) *grad_workspace_bytes = lists;
   return OCNN_OK;
 }
 
@@ -761,10 +849,8 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
   }
   OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence needs %zu bytes, got %zu", need,
       workspace_bytes);
-  const size_t one = (size_t)ids * channels;
-  a.run_a = (float*)workspace_dev;
-  a.run_h = a.run_a + one;
-  a.carry = carries ? carries : a.run_h + one;
+  a.carry = carries;
+  scan_lists(&a, ids, workspace_dev);
   by_width(v, [&](auto w) {
     by_chunk(shift, [&](auto l) {
       if (dtype == OCNN_F32) scan_forward_launch<float, w.value, l.value>(a, s);
@@ -803,8 +889,7 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
   v = v > 2 ? 2 : v;                 // (a group of rows is held in registers: p, q, before and the three loads)
   a.groups = (channels + v - 1) / v;
   a.threads = ids * a.groups;
-  a.run_a = (float*)workspace_dev;
-  a.run_h = a.run_a + (size_t)ids * channels;
+  scan_lists(&a, ids, workspace_dev);
   by_width(v, [&](auto w) {
     if constexpr (w.value <= 2)
       by_chunk(shift, [&](auto l) {

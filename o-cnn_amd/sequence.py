@@ -45,9 +45,9 @@ def _rows(t, name, ndim, like=None):
 
 
 def _aligned(t):
-  """rows and heads at multiples of 16 bytes, copied where they are not"""
+  """rows and heads at multiples of 16 bytes and not too far apart for the kernels' offsets, copied where they are not"""
   e = 16 // t.element_size()
-  if t.data_ptr() % 16 or t.stride(0) % e or t.stride(1) % e or (t.size(-1) > 1 and t.stride(-1) != 1):
+  if t.stride(0) >= 1 << 22 or t.stride(1) >= 1 << 22 or t.data_ptr() % 16 or t.stride(0) % e or t.stride(1) % e or (t.size(-1) > 1 and t.stride(-1) != 1):
     t = t.contiguous()
     if t.data_ptr() % 16:
       t = t.clone()
@@ -257,7 +257,7 @@ def octree_attention(q, k, v, q_offsets, k_offsets=None, k_lengths=None, left=-1
   visible to it when j <= p + right and (j >= p - left or j < sinks), -1 for a bound that is absent
   (right=0: causal), and key_mask[row of j] (bool [rows_k]) holds.  A query that sees no key gets zeros; what
   invisible keys and values hold does not matter.
-  dim: a multiple of 8 up to 128; sinks: at most 64; scale: 1 / sqrt(dim) where None.
+  dim: a multiple of 8 up to 128; heads // kv_heads and sinks: at most 64; scale: 1 / sqrt(dim) where None.
   `out`: where the result goes (rows of no sequence are left as they are; without `out` they are zero).
   return_lse=True returns (out, lse): lse [rows_q, heads] float32, the logarithm of each softmax's sum, which
   octree_attention_grad takes."""
