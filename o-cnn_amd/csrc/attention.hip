@@ -24,10 +24,6 @@
 namespace ocnn {
 namespace {
 
-#ifndef FWD_W
-#define FWD_W 3
-#define GQ_W 2
-#endif
 // wavefronts a SIMD that the registers leave room for: `small` up to 64 channels
 template <typename T, int DP> constexpr int waves_of(int small) { return DP <= 64 ? small : sizeof(T) == 4 ? 1 : 2; }
 
@@ -173,8 +169,15 @@ __device__ inline bool decided(bool x) {
 }
 __device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 3"); }
 
-// Row r of an accumulator register in this lane
-__device__ inline int acc_row(int r) { return 8 * (r >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (r & 3); }
+// Bits 0 .. n - 1
+__device__ inline uint32_t first_bits(int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; }
+// x where the lane's bit of accumulator row r is set, `other` (as bits) elsewhere; `bits` has been moved right by 4 in the
+// upper half of the wavefront.  Two integer instructions, and a NaN in x does not come through.
+__device__ inline float where_seen(uint32_t bits, int r, float x, uint32_t other) {
+  const int n = 8 * (r >> 2) + (r & 3);
+  const uint32_t keep = (uint32_t)(((int32_t)(bits << (31 - n))) >> 31);
+  return __uint_as_float((__float_as_uint(x) & keep) | (other & ~keep));
+}
 
 // A tile of ROWS rows on its way from memory to LDS: the loads of the next tile are issued before the current
 // one is used and wait in registers.  A thread's pieces keep their byte offsets from the tile's first row, so
@@ -234,12 +237,10 @@ template <typename T, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
   }
 };
 
-// The keys of a tile that exist and are not masked, bit i for key j0 + i: the same in every wavefront
+// The keys of a tile that exist and that `mask` keeps, bit i for key j0 + i: the same in every wavefront
 template <int KEYS> __device__ inline uint64_t live_keys(const unsigned char* mask, int j0, int keys) {
-  const int n = keys - j0, lane = threadIdx.x & 63;
-  uint64_t live = n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0;
-  if (mask) live &= __ballot(lane < KEYS && lane < n && mask[j0 + lane] != 0);
-  return live;
+  const int lane = threadIdx.x & 63;
+  return __ballot(lane < KEYS && j0 + lane < keys && mask[j0 + lane] != 0);
 }
 
 __device__ inline float wave_max(float x) {
@@ -260,6 +261,13 @@ __device__ inline void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+
+// Work items in an order that keeps neighbours on one XCD: workgroups go round the 8 XCDs in turn, so of every 64
+// items each XCD takes 8 in a row, whose windows overlap in its L2.  (Not an eighth of all items: the tiles of a
+// causal sequence grow towards its end.)  Grids are padded to whole sets of 64.
+__device__ inline int near_item(int x) { return (x & ~63) + (x & 7) * 8 + ((x >> 3) & 7); }
+inline int64_t whole_sets(int64_t n) { return n <= 64 ? n : (n + 63) & ~(int64_t)63; }
+__device__ inline int item_of(int x, int n) { return n <= 64 ? x : near_item(x); }
 
 // One sequence as the kernels see it
 struct Seq {
@@ -351,7 +359,7 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
 }
 
 template <typename T, int DP, int QW, bool SPLIT>
-__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? FWD_W : 2))) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))) attention_kernel(AttnArgs a) {
   using S = Shape<T, DP>;
   using F = ForwardShape<T, DP, QW>;
   constexpr int kRows = 32 * QW, kShift = Log2<kRows>::value;
@@ -359,10 +367,11 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? FWD_W :
   __shared__ Softmax stats[4][32];
   const ocnn_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
-  const int kv = blockIdx.y, split = SPLIT ? blockIdx.z : 0;
-  const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, blockIdx.x, kShift, a.group);
+  // (splits first: workgroups go round the XCDs in turn, and work items that no sequence owns must not be every second one)
+  const int kv = blockIdx.y, split = SPLIT ? blockIdx.x : 0, work_id = SPLIT ? (int)blockIdx.z : item_of(blockIdx.x, gridDim.x);
+  const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, work_id, kShift, a.group);
   const int q_begin = clamped(p.q_offsets, b, p.rows_q);
-  const int64_t tile = (int64_t)blockIdx.x - (((int64_t)q_begin * a.group >> kShift) + b);
+  const int64_t tile = (int64_t)work_id - (((int64_t)q_begin * a.group >> kShift) + b);
   Seq s;
   if (b >= p.n_seq) {
     s.q0 = q_begin; s.queries = p.rows_q - q_begin; s.k0 = 0; s.keys = 0; s.room = 0;
@@ -429,108 +438,122 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? FWD_W :
   const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
   const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
 
-  // N x 32 keys from j0 on against this wavefront's rows: scores -> probabilities -> o.  The base of the
-  // exponentials follows the running maximum only when that has grown by more than 8 (a factor of 2^8, which 32-bit
-  // sums and bf16 weights hold without loss): the values kept are rescaled a few times a row instead of in
-  // most tiles, and lanes compare without exchanging their maxima.
-  auto keys = [&](auto n, const T* kt, const T* vt, int j0, uint64_t live) {
-    constexpr int N = n.value;
-    floatx16 x[N];
+  // the keys j0 .. j0 + 31 that this lane's row sees, as bits for where_seen
+  auto seen_bits = [&](int j0, uint32_t live) {
+    return (live & first_bits(hi - j0) & (~first_bits(lo - j0) | first_bits(sinks - j0))) >> (4 * half);
+  };
+  auto rebase = [&](float to) {
+    const float shrink = __builtin_amdgcn_exp2f(m - (to == -__builtin_inff() ? 0.0f : to));
+    l *= shrink;
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
+    m = to;
+  };
+  // The tile's keys, from j0 on, against this wavefront's rows: scores -> probabilities -> o.  The exponentials are
+  // taken against a base that follows the row's running maximum from behind: it is set by the first keys a
+  // row sees, and raised after a tile whose sum has passed 2^10.  32-bit sums and bf16 weights hold larger
+  // powers without loss, so most tiles need neither a maximum nor a rescaling, and the second product does
+  // not wait for a vote.  Only a weight beyond 2^100 of the base is too much: the tile says so, and the
+  // workgroup takes all its tiles again, with the maximum of each (careful).
+  bool careful = QW == 1, over = false;       // (QW = 1 waits for memory: careful from the start)
+  auto keys = [&](const T* kt, const T* vt, int j0, uint64_t live) {
+    constexpr int N = KT / 32;
     const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
-    const bool masked = decided((j0 < all_lo) | (j0 + 32 * N > all_hi) | ((live & all) != all));
+    const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | ((live & all) != all));
+    const bool measure = careful || decided(__any(m == -__builtin_inff()));
+    floatx16 x[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = rows_times<T, DP>(kt + i * 32 * S::kPitch, q, zero16());
     if (masked) {
       settle();
 #pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t seen = seen_bits(j0 + 32 * i, (uint32_t)(live >> (32 * i)));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[i][r] = where_seen(seen, r, x[i][r], 0xff800000u);
+      }
+    }
+    if (measure) {
+      settle();
+      float top = x[0][0];
+#pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + 32 * i + acc_row(r);
-          const bool see = (j < hi) & ((j >= lo) | (j < sinks)) & (int)(live >> (32 * i + acc_row(r)) & 1);
-          x[i][r] = see ? x[i][r] : -__builtin_inff();
-        }
-    }
-    float top = x[0][0];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, x[i][r]);
-    top *= a.scale2;
-    if (__any(top > m + 8.0f)) {
-      const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-      const float shrink = __builtin_amdgcn_exp2f(m - (to == -__builtin_inff() ? 0.0f : to));
-      l *= shrink;
-#pragma unroll
-      for (int d = 0; d < S::kBlocks; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= shrink;
-      m = to;
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, x[i][r]);
+      top *= a.scale2;
+      rebase(fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))));
     }
     const float base = m == -__builtin_inff() ? 0.0f : m;
-    float sum = 0.0f;
+    float sums[2 * N];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) {
+      sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], a.scale2, -base));
-        sum += x[i][r];
+        sums[2 * i + (r & 1)] += x[i][r];
       }
-    l += sum;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) columns_times<DP>(o, vt + i * 32 * S::kPitch, x[i]);
+    float sum = sums[0] + sums[1];
+    if (N == 2) sum += sums[2] + sums[3];
+    l += sum;
+    if (QW == 4 && __any(!(sum <= 1024.0f))) {
+      settle();
+      over = over || !(sum <= 1.2676506e30f);
+      const float most = fmaxf(sum, __shfl_xor(sum, 32, 64));
+      rebase(most > 1024.0f && most <= 1.2676506e30f ? m + rintf(__builtin_amdgcn_logf(most)) : m);
+    }
   };
-  auto reach = [&](int j0) { return (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi); };
+  auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + KT > w_lo) | (j0 < p.sinks)); };
+  if (!have) m = 0.0f;                        // (does not ask for a maximum)
 
-  if constexpr (QW == 4) {
-    Staged<T, DP, KT, 256, true> sk, sv;
-    sk.init(tid, p.dim, [&](int r) { return r * (int)p.k_row; });
-    sv.init(tid, p.dim, [&](int r) { return r * (int)p.v_row; });
-    uint64_t next = 0;
-    auto fetch = [&](int v) {
-      const int j0 = tile_key(v);
+  constexpr int kThreads = QW == 4 ? 256 : 64;
+  const int mine = QW == 4 ? tid : lane;
+  Staged<T, DP, KT, kThreads, true> sk, sv;
+  sk.init(mine, p.dim, [&](int r) { return r * (int)p.k_row; });
+  sv.init(mine, p.dim, [&](int r) { return r * (int)p.v_row; });
+  uint64_t next = ~0ull;
+  auto fetch = [&](int v) {
+    const int j0 = tile_key(v);
+    if (mask) {
       next = live_keys<KT>(mask, j0, s.keys);
-      if (mask) {
-        sk.load_live(kbase + (int64_t)j0 * p.k_row, tid, next);
-        sv.load_live(vbase + (int64_t)j0 * p.v_row, tid, next);
-      } else {
-        sk.load(kbase + (int64_t)j0 * p.k_row, tid, s.keys - j0);
-        sv.load(vbase + (int64_t)j0 * p.v_row, tid, s.keys - j0);
-      }
-    };
+      sk.load_live(kbase + (int64_t)j0 * p.k_row, mine, next);
+      sv.load_live(vbase + (int64_t)j0 * p.v_row, mine, next);
+    } else {
+      sk.load(kbase + (int64_t)j0 * p.k_row, mine, s.keys - j0);
+      sv.load(vbase + (int64_t)j0 * p.v_row, mine, s.keys - j0);
+    }
+  };
+  if constexpr (QW == 4) {
     const int step = SPLIT ? a.splits : 1;
-    if (split < tiles) fetch(split);
-    int buf = 0;
-    for (int v = split; v < tiles; v += step, buf ^= 1) {
-      T* kt = (T*)lds + buf * 2 * F::kTile;
-      T* vt = kt + F::kTile;
-      sk.store(kt, tid);
-      sv.store(vt, tid);
-      const uint64_t live = next;
-      __syncthreads();                        // (the other buffer's readers are done: they passed the last barrier)
-      if (v + step < tiles) fetch(v + step);
-      const int j0 = tile_key(v);
-      const bool first = reach(j0), second = reach(j0 + 32);
-      if (first && second) keys(std::integral_constant<int, 2>(), kt, vt, j0, live);
-      else if (first) keys(std::integral_constant<int, 1>(), kt, vt, j0, live);
-      else if (second) keys(std::integral_constant<int, 1>(), kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32, live >> 32);
+#pragma unroll 1
+    for (;;) {
+      if (split < tiles) fetch(split);
+      T* kt = (T*)lds;
+#pragma unroll 1
+      for (int v = split; v < tiles; v += step) {
+        T* vt = kt + F::kTile;
+        sk.store(kt, tid);
+        sv.store(vt, tid);
+        const uint64_t live = next;
+        __syncthreads();                      // (the other buffer's readers are done: they passed the last barrier)
+        if (v + step < tiles) fetch(v + step);
+        const int j0 = tile_key(v);
+        if (reach(j0)) keys(kt, vt, j0, live);
+        kt = kt == (T*)lds ? (T*)lds + 2 * F::kTile : (T*)lds;
+      }
+      if (careful || !__syncthreads_or(over)) break;
+      careful = true;
+      m = have ? -__builtin_inff() : 0.0f;
+      l = 0.0f;
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d) o[d] = zero16();
     }
   } else {
-    Staged<T, DP, KT, 64, true> sk, sv;
-    sk.init(lane, p.dim, [&](int r) { return r * (int)p.k_row; });
-    sv.init(lane, p.dim, [&](int r) { return r * (int)p.v_row; });
-    uint64_t next = 0;
-    auto fetch = [&](int v) {
-      const int j0 = tile_key(v);
-      next = live_keys<KT>(mask, j0, s.keys);
-      if (mask) {
-        sk.load_live(kbase + (int64_t)j0 * p.k_row, lane, next);
-        sv.load_live(vbase + (int64_t)j0 * p.v_row, lane, next);
-      } else {
-        sk.load(kbase + (int64_t)j0 * p.k_row, lane, s.keys - j0);
-        sv.load(vbase + (int64_t)j0 * p.v_row, lane, s.keys - j0);
-      }
-    };
     T* kt = (T*)lds + wave * 2 * F::kTile;
     T* vt = kt + F::kTile;
     // (the splits take turns: at any time the workgroups together read one stretch of the keys, which spreads
@@ -545,9 +568,10 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? FWD_W :
       wave_lds_fence();
       if (v + step < tiles) fetch(v + step);
       const int j0 = tile_key(v);
-      if (reach(j0)) keys(std::integral_constant<int, 1>(), kt, vt, j0, live);
+      if (reach(j0)) keys(kt, vt, j0, live);
     }
   }
+  if (!have) m = -__builtin_inff();
   l += __shfl_xor(l, 32, 64);
 
   if constexpr (QW == 1) {                    // the wavefronts' shares, joined in the first one
@@ -749,16 +773,17 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? GQ_W : 2))) attention_grad_q_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))) attention_grad_q_kernel(AttnArgs a) {
   using S = Shape<T, DP>;
   constexpr int KT = 64, kTile = KT * S::kPitch, kRows = 128, kShift = 7;
   __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
   const ocnn_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y;
-  const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, blockIdx.x, kShift, a.group);
+  const int work_id = item_of(blockIdx.x, gridDim.x);
+  const int b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, work_id, kShift, a.group);
   const int q_begin = clamped(p.q_offsets, b, p.rows_q);
-  const int64_t tile = (int64_t)blockIdx.x - (((int64_t)q_begin * a.group >> kShift) + b);
+  const int64_t tile = (int64_t)work_id - (((int64_t)q_begin * a.group >> kShift) + b);
   Seq s;
   if (b >= p.n_seq) {
     s.q0 = q_begin; s.queries = p.rows_q - q_begin; s.k0 = 0; s.keys = 0; s.room = 0;
@@ -819,14 +844,16 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? GQ_W : 
   const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
   const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
 
-  auto reach = [&](int j0) { return (j0 < w_hi && j0 + 32 > w_lo) || (j0 < p.sinks && j0 < w_hi); };
-  auto keys = [&](auto n, const T* kt, const T* vt, int j0, uint64_t live) {
-    constexpr int N = n.value;
-    floatx16 x[N];
-    const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
-    const bool masked = decided((j0 < all_lo) | (j0 + 32 * N > all_hi) | ((live & all) != all));
+  // the keys j0 .. j0 + 31 that this lane's row sees, as bits for where_seen
+  auto seen_bits = [&](int j0, uint32_t live) {
+    return (live & first_bits(hi - j0) & (~first_bits(lo - j0) | first_bits(sinks - j0))) >> (4 * half);
+  };
+  auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + KT > w_lo) | (j0 < p.sinks)); };
+  auto keys = [&](const T* kt, const T* vt, int j0, uint64_t live) {
+    const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | (live != ~0ull));
+    floatx16 x[2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < 2; ++i) {
       x[i] = rows_times<T, DP>(kt + i * 32 * S::kPitch, q, zero16());
       const floatx16 dp = rows_times<T, DP>(vt + i * 32 * S::kPitch, go, zero16());
 #pragma unroll
@@ -834,26 +861,24 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? GQ_W : 
     }
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t seen = seen_bits(j0 + 32 * i, (uint32_t)(live >> (32 * i)));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = j0 + 32 * i + acc_row(r);
-          const bool see = (j < hi) & ((j >= lo) | (j < sinks)) & (int)(live >> (32 * i + acc_row(r)) & 1);
-          x[i][r] = see ? x[i][r] : 0.0f;
-        }
+        for (int r = 0; r < 16; ++r) x[i][r] = where_seen(seen, r, x[i][r], 0u);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) columns_times<DP>(dq, kt + i * 32 * S::kPitch, x[i]);
+    for (int i = 0; i < 2; ++i) columns_times<DP>(dq, kt + i * 32 * S::kPitch, x[i]);
   };
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
   Staged<T, DP, KT, 256, true> sk, sv;
   sk.init(tid, p.dim, [&](int r) { return r * (int)p.k_row; });
   sv.init(tid, p.dim, [&](int r) { return r * (int)p.v_row; });
-  uint64_t next = 0;
+  uint64_t next = ~0ull;
   auto fetch = [&](int v) {
     const int j0 = tile_key(v);
-    next = live_keys<KT>(mask, j0, s.keys);
     if (mask) {
+      next = live_keys<KT>(mask, j0, s.keys);
       sk.load_live(kbase + (int64_t)j0 * p.k_row, tid, next);
       sv.load_live(vbase + (int64_t)j0 * p.v_row, tid, next);
     } else {
@@ -862,8 +887,8 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? GQ_W : 
     }
   };
   if (tiles > 0) fetch(0);
+  T* kt = lds;
   for (int v = 0; v < tiles; ++v) {
-    T* kt = lds + (v & 1) * 2 * kTile;
     T* vt = kt + kTile;
     sk.store(kt, tid);
     sv.store(vt, tid);
@@ -871,10 +896,8 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? GQ_W : 
     __syncthreads();
     if (v + 1 < tiles) fetch(v + 1);
     const int j0 = tile_key(v);
-    const bool first = reach(j0), second = reach(j0 + 32);
-    if (first && second) keys(std::integral_constant<int, 2>(), kt, vt, j0, live);
-    else if (first) keys(std::integral_constant<int, 1>(), kt, vt, j0, live);
-    else if (second) keys(std::integral_constant<int, 1>(), kt + 32 * S::kPitch, vt + 32 * S::kPitch, j0 + 32, live >> 32);
+    if (reach(j0)) keys(kt, vt, j0, live);
+    kt = kt == lds ? lds + 2 * kTile : lds;
   }
   float worst = 0.0f;
 #pragma unroll
@@ -1064,13 +1087,11 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
       dp[r] = x[r] * (dp[r] - de[r >> 2][r & 3]);
     }
     if (masked) {
-      const int upto = min(hi, end);
+      const uint32_t seen = (first_bits(min(hi, end) - r0) & ~first_bits(lo - r0)) >> (4 * half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = r0 + acc_row(r);
-        const bool see = (row >= lo) & (row < upto);
-        x[r] = see ? x[r] : 0.0f;
-        dp[r] = see ? dp[r] : 0.0f;
+        x[r] = where_seen(seen, r, x[r], 0u);
+        dp[r] = where_seen(seen, r, dp[r], 0u);
       }
     }
     columns_times<DP>(dv, gt, x);
@@ -1250,7 +1271,7 @@ Plan plan_of(const ocnn_attention_params& p) {
   if (p.left >= 0 && p.right >= 0) keys = std::min<int64_t>(keys, (int64_t)p.left + p.right + p.rows_q / p.n_seq + p.sinks);
   const int64_t blocks = std::max<int64_t>((packed + (n.few ? 31 : 127)) / (n.few ? 32 : 128), n.few ? p.n_seq : 1) * p.kv_heads;
   const int64_t most = n.few ? keys / 256 : keys / 1024;
-  n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, kMaxSplits}));
+  n.splits = n.tiles > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, kMaxSplits}));
   return n;
 }
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -1286,7 +1307,7 @@ template <typename F> void by_dim(int dim, F f) {
 }
 
 template <typename T, int DP> void forward_launch(const AttnArgs& a, const Plan& n, hipStream_t s) {
-  const dim3 grid((unsigned)n.tiles, a.p.kv_heads, n.splits);
+  const dim3 grid = n.splits > 1 ? dim3(n.splits, a.p.kv_heads, (unsigned)n.tiles) : dim3((unsigned)whole_sets(n.tiles), a.p.kv_heads);
   if (n.few) {
     if (n.splits > 1) attention_kernel<T, DP, 1, true><<<grid, 256, 0, s>>>(a);
     else attention_kernel<T, DP, 1, false><<<grid, 256, 0, s>>>(a);
@@ -1301,7 +1322,7 @@ template <typename T, int DP> void backward_launch(const AttnArgs& a, hipStream_
   const ocnn_attention_params& p = a.p;
   if (p.rows_q > 0) {
     const int64_t tiles = ((int64_t)p.rows_q * a.group >> 7) + p.n_seq + 1;
-    attention_grad_q_kernel<T, DP><<<dim3((unsigned)tiles, p.kv_heads), 256, 0, s>>>(a);
+    attention_grad_q_kernel<T, DP><<<dim3((unsigned)whole_sets(tiles), p.kv_heads), 256, 0, s>>>(a);
   }
   if (p.rows_k > 0) {
     const int64_t near_items = (p.rows_k >> 7) + p.n_seq + 1;

@@ -13,7 +13,7 @@ __device__ inline float to_f32(float v) { return v; }
 __device__ inline float to_f32(uint16_t v) { return bf16_to_f32(v); }
 template <typename T> __device__ inline T from_f32(float v);
 template <> __device__ inline float from_f32<float>(float v) { return v; }
-template <> __device__ inline uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16(v); }
+template <> __device__ inline uint16_t from_f32<uint16_t>(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest even
 
 // N neighbouring elements in registers; loads and stores need the alignment of one element only
 template <typename T, int N> struct Pack {
