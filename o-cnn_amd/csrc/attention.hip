@@ -35,7 +35,7 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxSinks = 64;
-constexpr int kFarRows = 256;   // tokens of a work item of the sinks' gradient
+constexpr int kFarRows = 512;   // tokens of a work item of the sinks' gradient
 
 struct AttnArgs {
   ocnn_attention_params p;
@@ -936,8 +936,9 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))
 // A workgroup owns 128 keys of a key head, 32 a wavefront, in registers; the packed rows that see them go
 // through LDS 64 at a time, so the query heads that share the key head are summed where they are
 // accumulated.  The first keys (sinks) are seen by every later row: the rows beyond the window of
-// their tile ("far") are dealt out in items of kFarRows tokens to workgroups of their own, whose sums over
-// the sinks go to memory in 32 bits and are added in order by attention_sink_kernel.
+// their tile ("far") are dealt out in items of kFarRows tokens to workgroups of their own, in which all four
+// wavefronts hold the same 32 sinks and share the rows (with a wavefront for every 32 keys, three of them had
+// nothing to do).  Their sums go to memory in 32 bits and are added in order by attention_sink_kernel.
 struct FarRange { int first; bool any; };        // tokens [first, queries) see the sinks only
 __device__ inline FarRange far_tokens(const ocnn_attention_params& p, const Seq& s) {
   FarRange f;
@@ -999,13 +1000,17 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y;
   const bool far = (int)blockIdx.x >= near_items;
-  int b, j0 = 0;
+  const int sink_blocks = p.sinks > 32 ? 2 : 1;    // of 32
+  int b, j0 = 0, far_id = 0;
   int64_t item;
   if (!far) {
-    b = locate_packed(p.k_offsets, p.n_seq, p.rows_k, blockIdx.x, 7, 1);
-    item = (int64_t)blockIdx.x - ((clamped(p.k_offsets, b, p.rows_k) >> 7) + b);
+    const int id = item_of(blockIdx.x, near_items);
+    b = locate_packed(p.k_offsets, p.n_seq, p.rows_k, id, 7, 1);
+    item = (int64_t)id - ((clamped(p.k_offsets, b, p.rows_k) >> 7) + b);
   } else {
-    const int id = (int)blockIdx.x - near_items;
+    far_id = ((int)blockIdx.x - near_items) / sink_blocks;
+    j0 = (((int)blockIdx.x - near_items) % sink_blocks) * 32;
+    const int id = far_id;
     b = locate_packed(p.q_offsets, p.n_seq, p.rows_q, id, Log2<kFarRows>::value, 1);
     item = (int64_t)id - ((clamped(p.q_offsets, b, p.rows_q) >> Log2<kFarRows>::value) + b);
     if (b >= p.n_seq) return;
@@ -1039,8 +1044,8 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
     tb = (int)min((item + 1) * kFarRows, (int64_t)s.queries);
     if (ta >= tb) return;
   }
-  const bool sink_tile = j0 == 0 && fr.any;        // its first keys' sums go to memory
-  const int j = j0 + wave * 32 + col;
+  const bool sink_tile = (far || j0 == 0) && fr.any;   // its first keys' sums go to memory
+  const int jw = far ? j0 : j0 + wave * 32, j = jw + col;
   bool key = j < s.keys && (!far || j < p.sinks);
   if (key && p.key_mask) key = p.key_mask[s.k0 + j] != 0;
   // this key's packed rows: [lo, hi), and what some / every key of the wavefront has
@@ -1051,7 +1056,6 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
     lo = max(lo, ta) * a.group;
     hi = min(hi, tb) * a.group;
   }
-  const int jw = j0 + wave * 32;
   int w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
   if (jw < s.keys && (!far || jw < p.sinks)) {
     const bool any_sink = jw < p.sinks;
@@ -1122,22 +1126,64 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
       }
     }
   };
-  if (tiles > 0) fetch(0);
-  for (int v = 0; v < tiles; ++v) {
-    const int buf = v & 1;
-    T* qt = lds + buf * 2 * kTile;
-    T* gt = qt + kTile;
-    sq.store(qt, tid);
-    sg.store(gt, tid);
+  auto put = [&](int buf) {
+    sq.store(lds + buf * 2 * kTile, tid);
+    sg.store(lds + (buf * 2 + 1) * kTile, tid);
     if (tid < RT) {
       row_lse[buf][tid] = one_lse;
       row_delta[buf][tid] = one_delta;
     }
-    __syncthreads();
-    if (v + 1 < tiles) fetch(v + 1);
-    const int r0 = (ta + v * step) * a.group, end = r0 + used;
-    subtile(qt, gt, row_lse[buf], row_delta[buf], r0, end);
-    if (used > 32) subtile(qt + 32 * S::kPitch, gt + 32 * S::kPitch, row_lse[buf] + 32, row_delta[buf] + 32, r0 + 32, end);
+  };
+  auto half_tile = [&](int buf, int h, int v) {
+    const int r0 = (ta + v * step) * a.group;
+    if (32 * h < used)
+      subtile(lds + buf * 2 * kTile + h * 32 * S::kPitch, lds + (buf * 2 + 1) * kTile + h * 32 * S::kPitch,
+          row_lse[buf] + 32 * h, row_delta[buf] + 32 * h, r0 + 32 * h, r0 + used);
+  };
+  if (!far) {
+    if (tiles > 0) fetch(0);
+    for (int v = 0; v < tiles; ++v) {
+      put(v & 1);
+      __syncthreads();
+      if (v + 1 < tiles) fetch(v + 1);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) half_tile(v & 1, h, v);
+    }
+  } else {
+#pragma unroll 1
+    for (int v = 0; v < tiles; v += 2) {             // two tiles, a half for each wavefront
+      fetch(v);
+      __syncthreads();
+      put(0);
+      if (v + 1 < tiles) {
+        fetch(v + 1);
+        put(1);
+      }
+      __syncthreads();
+      if (v + (wave >> 1) < tiles) half_tile(wave >> 1, wave & 1, v + (wave >> 1));
+    }
+    // the four shares, added in order by the first wavefront
+    float* join = (float*)lds;
+    auto add_up = [&](floatx16 (&x)[S::kBlocks]) {
+      __syncthreads();
+      if (wave)
+#pragma unroll
+        for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) join[(((wave - 1) * S::kBlocks + d) * 16 + r) * 64 + lane] = x[d][r];
+      __syncthreads();
+      if (!wave)
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+          for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[d][r] += join[((w * S::kBlocks + d) * 16 + r) * 64 + lane];
+    };
+    settle();
+    add_up(dk);
+    add_up(dv);
+    if (wave) return;
   }
 
   float worst = 0.0f;
@@ -1148,7 +1194,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
   worst += __shfl_xor(worst, 32, 64);
   const bool good = finite(worst), mine = j < s.room;
   const bool to_memory = sink_tile && j < min(p.sinks, s.keys);
-  const int64_t slot = far ? (int64_t)p.n_seq + ((int)blockIdx.x - near_items) : b;
+  const int64_t slot = far ? (int64_t)p.n_seq + far_id : b;
   float* part = a.sink_part + (slot * p.kv_heads + kv) * 2 * p.sinks * p.dim + (int64_t)(to_memory ? j : 0) * p.dim;
   const int64_t part_dv = (int64_t)p.sinks * p.dim;
   T* dk_row = (T*)a.dk + (int64_t)(s.k0 + j) * a.dk_row + kv * a.dk_head;
@@ -1325,8 +1371,8 @@ template <typename T, int DP> void backward_launch(const AttnArgs& a, hipStream_
     attention_grad_q_kernel<T, DP><<<dim3((unsigned)whole_sets(tiles), p.kv_heads), 256, 0, s>>>(a);
   }
   if (p.rows_k > 0) {
-    const int64_t near_items = (p.rows_k >> 7) + p.n_seq + 1;
-    const int64_t all = near_items + (has_far(p) ? far_items(p) : 0);
+    const int64_t near_items = whole_sets((p.rows_k >> 7) + p.n_seq + 1);
+    const int64_t all = near_items + (has_far(p) ? far_items(p) * (p.sinks > 32 ? 2 : 1) : 0);
     attention_grad_kv_kernel<T, DP><<<dim3((unsigned)all, p.kv_heads), 256, 0, s>>>(a, (int)near_items);
     if (has_far(p)) attention_sink_kernel<T><<<dim3(p.sinks, p.kv_heads, p.n_seq), 1024, 0, s>>>(a);
   }
