@@ -24,8 +24,10 @@
 namespace ocnn {
 namespace {
 
-// wavefronts a SIMD that the registers leave room for: `small` up to 64 channels
-template <typename T, int DP> constexpr int waves_of(int small) { return DP <= 64 ? small : sizeof(T) == 4 ? 1 : 2; }
+// wavefronts a SIMD that the registers leave room for, by the bytes of a row
+constexpr int forward_waves(int row) { return row <= 128 ? 3 : row <= 256 ? 2 : 1; }
+constexpr int grad_q_waves(int row) { return row <= 64 ? 3 : row <= 192 ? 2 : 1; }
+constexpr int grad_kv_waves(int row) { return row <= 128 ? 2 : 1; }
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -100,16 +102,36 @@ __device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim
   }
 }
 
-// acc[row of the tile][column] += tile rows . column
-template <typename T, int DP>
-__device__ inline floatx16 rows_times(const T* tile, const Column<T, DP>& col, floatx16 acc) {
+// Keeps the compiler from moving instructions across.  It otherwise reads each fragment right in front of the
+// matrix instruction that uses it (fewer registers) and waits for LDS every time: eight times 130 cycles in
+// front of 256 cycles of products.
+__device__ inline void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// The fragments of 32 rows of a tile as the left operand of tile rows . column
+template <typename T, int DP> struct RowFrags {
   using S = Shape<T, DP>;
-  const int lane = threadIdx.x & 63;
-  const T* at = tile + (lane & 31) * S::kPitch + (lane >> 5) * S::kPiece;
+  typename Frag<T>::type v[S::kSteps];
+  __device__ inline void load(const T* tile) {
+    const int lane = threadIdx.x & 63;
+    const T* at = tile + (lane & 31) * S::kPitch + (lane >> 5) * S::kPiece;
 #pragma unroll
-  for (int s = 0; s < S::kSteps; ++s)
-    acc = mma(*(const typename Frag<T>::type*)(at + 2 * s * S::kPiece), col.v[s], acc);
-  return acc;
+    for (int s = 0; s < S::kSteps; ++s) v[s] = *(const typename Frag<T>::type*)(at + 2 * s * S::kPiece);
+  }
+};
+// two products whose steps alternate, so that none waits for the one before it
+template <typename T, int DP>
+__device__ inline void rows_times(const RowFrags<T, DP>& a, const Column<T, DP>& x, floatx16& ax, const RowFrags<T, DP>& b,
+    const Column<T, DP>& y, floatx16& by) {
+#pragma unroll
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) {
+    ax = mma(a.v[s], x.v[s], ax);
+    by = mma(b.v[s], y.v[s], by);
+  }
+}
+template <typename T, int DP>
+__device__ inline void rows_times(const RowFrags<T, DP>& a, const Column<T, DP>& x, floatx16& ax) {
+#pragma unroll
+  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) ax = mma(a.v[s], x.v[s], ax);
 }
 
 __device__ inline shortx4 read_transposed(const uint16_t* p) {
@@ -122,40 +144,56 @@ __device__ inline uint32_t pack_bf16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// acc[block][channel][column] += sum over the 32 rows of the tile: tile[row][channel] * w[row][column], w as an
-// accumulator of rows_times holds it.  bf16: w is rounded to bf16 (2^-9 of each weight at most, the same
-// as the tile's own elements carry); statistics and sums stay in 32 bits.
-template <int DP>
-__device__ inline void columns_times(floatx16 (&acc)[DP / 32], const uint16_t* tile, const floatx16& w) {
+// The fragments of 32 rows of a tile, by channel, for  acc[block][channel][column] += sum over the rows of
+// tile[row][channel] * w[row][column], w as an accumulator of rows_times holds it.  bf16: w is rounded to bf16 (2^-8 of
+// each weight at most, as the tile's own elements are); statistics and sums stay in 32 bits.
+template <typename T, int DP> struct ColumnFrags;
+template <int DP> struct ColumnFrags<uint16_t, DP> {
   using S = Shape<uint16_t, DP>;
-  const int lane = threadIdx.x & 63;
-  // 16 lanes read 4 rows of 16 channels and get them back by channel
-  const uint16_t* at = tile + ((lane >> 5) * 4 + ((lane >> 2) & 3)) * S::kPitch + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  bf16x8 v[2][S::kBlocks];
+  __device__ inline void load(const uint16_t* tile) {
+    const int lane = threadIdx.x & 63;
+    // 16 lanes read 4 rows of 16 channels and get them back by channel
+    const uint16_t* at = tile + ((lane >> 5) * 4 + ((lane >> 2) & 3)) * S::kPitch + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    uintx4 b;
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = pack_bf16(w[8 * s + 2 * i], w[8 * s + 2 * i + 1]);
-    const bf16x8 bw = __builtin_bit_cast(bf16x8, b);
+      for (int d = 0; d < S::kBlocks; ++d) {
+        struct { shortx4 lo, hi; } a = {read_transposed(at + 16 * s * S::kPitch + 32 * d),
+                                        read_transposed(at + (16 * s + 8) * S::kPitch + 32 * d)};
+        v[s][d] = __builtin_bit_cast(bf16x8, a);
+      }
+  }
+  __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
 #pragma unroll
-    for (int d = 0; d < S::kBlocks; ++d) {
-      struct { shortx4 lo, hi; } a = {read_transposed(at + 16 * s * S::kPitch + 32 * d),
-                                      read_transposed(at + (16 * s + 8) * S::kPitch + 32 * d)};
-      acc[d] = mma(__builtin_bit_cast(bf16x8, a), bw, acc[d]);
+    for (int s = 0; s < 2; ++s) {
+      uintx4 b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = pack_bf16(w[8 * s + 2 * i], w[8 * s + 2 * i + 1]);
+      const bf16x8 bw = __builtin_bit_cast(bf16x8, b);
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[s][d], bw, acc[d]);
     }
   }
-}
-template <int DP>
-__device__ inline void columns_times(floatx16 (&acc)[DP / 32], const float* tile, const floatx16& w) {
+};
+template <int DP> struct ColumnFrags<float, DP> {
   using S = Shape<float, DP>;
-  const int lane = threadIdx.x & 63;
-  const float* at = tile + (lane >> 5) * 4 * S::kPitch + (lane & 31);
+  float v[16][S::kBlocks];
+  __device__ inline void load(const float* tile) {
+    const int lane = threadIdx.x & 63;
+    const float* at = tile + (lane >> 5) * 4 * S::kPitch + (lane & 31);
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-    for (int d = 0; d < S::kBlocks; ++d)
-      acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (r >> 2) + (r & 3)) * S::kPitch + 32 * d], w[r], acc[d], 0, 0, 0);
-}
+      for (int d = 0; d < S::kBlocks; ++d) v[r][d] = at[(8 * (r >> 2) + (r & 3)) * S::kPitch + 32 * d];
+  }
+  __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int d = 0; d < S::kBlocks; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][d], w[r], acc[d], 0, 0, 0);
+  }
+};
 
 // For a branch between a matrix product and the code that reads its result.  The compiler counts the wait states
 // that an accumulator needs before it is read, but where a short block lies on one of two paths it counts along
@@ -211,7 +249,7 @@ template <typename T, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
       const int n = tid + i * THREADS, r = n / S::kPieces, c = (n % S::kPieces) * S::kPiece;
       at[i] = c < dim ? (uint32_t)(offset(r) + c) * (uint32_t)sizeof(T) : kNowhere;
     }
-    apart = kScalar ? (uint32_t)offset(THREADS / S::kPieces) * (uint32_t)sizeof(T) : 0;
+    apart = __builtin_amdgcn_readfirstlane(kScalar ? offset(THREADS / S::kPieces) * (int)sizeof(T) : 0);
   }
   __device__ inline uintx4 piece(__amdgpu_buffer_rsrc_t buf, int i, bool ok) const {
     const uint32_t o = at[kScalar ? 0 : i];
@@ -264,8 +302,9 @@ __device__ inline void wave_lds_fence() {
 
 // Work items in an order that keeps neighbours on one XCD: workgroups go round the 8 XCDs in turn, so of every 64
 // items each XCD takes 8 in a row, whose windows overlap in its L2.  (Not an eighth of all items: the tiles of a
-// causal sequence grow towards its end.)  Grids are padded to whole sets of 64.
-__device__ inline int near_item(int x) { return (x & ~63) + (x & 7) * 8 + ((x >> 3) & 7); }
+// causal sequence grow towards its end.)  Which XCD begins changes with the head, so that what the last set
+// lacks is spread.  Grids are padded to whole sets of 64.
+__device__ inline int near_item(int x) { return (x & ~63) + ((x + blockIdx.y) & 7) * 8 + ((x >> 3) & 7); }
 inline int64_t whole_sets(int64_t n) { return n <= 64 ? n : (n + 63) & ~(int64_t)63; }
 __device__ inline int item_of(int x, int n) { return n <= 64 ? x : near_item(x); }
 
@@ -359,7 +398,7 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
 }
 
 template <typename T, int DP, int QW, bool SPLIT>
-__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) attention_kernel(AttnArgs a) {
   using S = Shape<T, DP>;
   using F = ForwardShape<T, DP, QW>;
   constexpr int kRows = 32 * QW, kShift = Log2<kRows>::value;
@@ -464,8 +503,20 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))
     const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | ((live & all) != all));
     const bool measure = careful || decided(__any(m == -__builtin_inff()));
     floatx16 x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = rows_times<T, DP>(kt + i * 32 * S::kPitch, q, zero16());
+    if constexpr (N == 2) {
+      RowFrags<T, DP> ka, kb;
+      ka.load(kt);
+      kb.load(kt + 32 * S::kPitch);
+      in_order();
+      x[0] = x[1] = zero16();
+      rows_times<T, DP>(ka, q, x[0], kb, q, x[1]);
+    } else {
+      RowFrags<T, DP> ka;
+      ka.load(kt);
+      in_order();
+      x[0] = zero16();
+      rows_times<T, DP>(ka, q, x[0]);
+    }
     if (masked) {
       settle();
 #pragma unroll
@@ -487,8 +538,12 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))
     }
     const float base = m == -__builtin_inff() ? 0.0f : m;
     float sums[2 * N];
+    ColumnFrags<T, DP> vf[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; ++i) {             // the values of one half arrive while the other half's weights are formed
+      vf[i].load(vt + i * 32 * S::kPitch);
+      in_order();
+      if (i) vf[0].times(o, x[0]);
       sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -496,8 +551,7 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))
         sums[2 * i + (r & 1)] += x[i][r];
       }
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) columns_times<DP>(o, vt + i * 32 * S::kPitch, x[i]);
+    vf[N - 1].times(o, x[N - 1]);
     float sum = sums[0] + sums[1];
     if (N == 2) sum += sums[2] + sums[3];
     l += sum;
@@ -773,7 +827,7 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))) attention_grad_q_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attention_grad_q_kernel(AttnArgs a) {
   using S = Shape<T, DP>;
   constexpr int KT = 64, kTile = KT * S::kPitch, kRows = 128, kShift = 7;
   __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
@@ -854,11 +908,18 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))
     floatx16 x[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x[i] = rows_times<T, DP>(kt + i * 32 * S::kPitch, q, zero16());
-      const floatx16 dp = rows_times<T, DP>(vt + i * 32 * S::kPitch, go, zero16());
+      RowFrags<T, DP> kf, vf;
+      kf.load(kt + i * 32 * S::kPitch);
+      vf.load(vt + i * 32 * S::kPitch);
+      in_order();
+      floatx16 dp = zero16();
+      x[i] = zero16();
+      rows_times<T, DP>(kf, q, x[i], vf, go, dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], a.scale2, -lse2)) * (dp[r] - delta);
     }
+    ColumnFrags<T, DP> cf[2];
+    cf[0].load(kt);
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -867,8 +928,10 @@ __global__ void __launch_bounds__(256, (waves_of<T, DP>(sizeof(T) == 2 ? 3 : 2))
         for (int r = 0; r < 16; ++r) x[i][r] = where_seen(seen, r, x[i][r], 0u);
       }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) columns_times<DP>(dq, kt + i * 32 * S::kPitch, x[i]);
+    cf[1].load(kt + 32 * S::kPitch);
+    in_order();
+    cf[0].times(dq, x[0]);
+    cf[1].times(dq, x[1]);
   };
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
   Staged<T, DP, KT, 256, true> sk, sv;
@@ -990,7 +1053,7 @@ __device__ __forceinline__ void grad_k_row_again(const AttnArgs& a, const Seq& s
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 : 2) attention_grad_kv_kernel(AttnArgs a,
+__global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) attention_grad_kv_kernel(AttnArgs a,
     int near_items) {
   using S = Shape<T, DP>;
   constexpr int RT = 64, kTile = RT * S::kPitch;
@@ -1077,18 +1140,29 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
   auto subtile = [&](const T* qt, const T* gt, const float* lse2, const float* delta, int r0, int end) {
     if (r0 + 32 <= w_lo || r0 >= min(w_hi, end)) return;
     const bool masked = decided((r0 < all_lo) | (r0 + 32 > min(all_hi, end)));
-    floatx16 x = rows_times<T, DP>(qt, k, zero16());
-    floatx16 dp = rows_times<T, DP>(gt, vv, zero16());
-    floatx4 ls[4], de[4];
+    RowFrags<T, DP> qf, gf;
+    qf.load(qt);
+    gf.load(gt);
+    // the products start from -lse and -dO . o of their rows, in the units of the scores
+    floatx16 x, dp;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      ls[i] = *(const floatx4*)(lse2 + 8 * i + 4 * half);
-      de[i] = *(const floatx4*)(delta + 8 * i + 4 * half);
+      const floatx4 ls = *(const floatx4*)(lse2 + 8 * i + 4 * half), de = *(const floatx4*)(delta + 8 * i + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[4 * i + e] = ls[e];
+        dp[4 * i + e] = de[e];
+      }
     }
+    in_order();
+    rows_times<T, DP>(qf, k, x, gf, vv, dp);
+    ColumnFrags<T, DP> gc, qc;
+    gc.load(gt);
+    in_order();
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -ls[r >> 2][r & 3]));
-      dp[r] = x[r] * (dp[r] - de[r >> 2][r & 3]);
+      x[r] = __builtin_amdgcn_exp2f(x[r] * a.scale2);
+      dp[r] *= x[r];
     }
     if (masked) {
       const uint32_t seen = (first_bits(min(hi, end) - r0) & ~first_bits(lo - r0)) >> (4 * half);
@@ -1098,8 +1172,10 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
         dp[r] = where_seen(seen, r, dp[r], 0u);
       }
     }
-    columns_times<DP>(dv, gt, x);
-    columns_times<DP>(dk, qt, dp);
+    qc.load(qt);
+    in_order();
+    gc.times(dv, x);
+    qc.times(dk, dp);
   };
 
   // a tile holds whole tokens: `step` of them, group rows each, so that a thread's rows keep their offsets
@@ -1112,26 +1188,25 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 
   sg.init(tid, p.dim, [&](int i) { const int t = i / a.group; return t * (int)a.grad_row + (i - t * a.group) * (int)a.grad_head; });
   const int my_token = tid / a.group;
   const int64_t my_stat = (int64_t)(s.q0 + ta + my_token) * p.heads + kv * a.group + tid - my_token * a.group;
+  const float lse_unit = kLog2e / a.scale2;
   float one_lse = 0.0f, one_delta = 0.0f;
   auto fetch = [&](int v) {
     const int t = v * step, rows = min(tb - ta - t, step) * a.group;
     sq.load(qbase + (int64_t)t * p.q_row, tid, used < RT ? min(rows, used) : rows);
     sg.load(gbase + (int64_t)t * a.grad_row, tid, used < RT ? min(rows, used) : rows);
-    if (tid < RT) {
+    if (tid < rows && tid < RT) {              // (as they are: nothing here may wait for a load)
+      one_lse = a.lse[my_stat + (int64_t)t * p.heads];
+      one_delta = a.delta[my_stat + (int64_t)t * p.heads];
+    } else {
       one_lse = one_delta = 0.0f;
-      if (tid < rows) {
-        const float lse = a.lse[my_stat + (int64_t)t * p.heads];
-        one_lse = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
-        one_delta = a.delta[my_stat + (int64_t)t * p.heads];
-      }
     }
   };
   auto put = [&](int buf) {
     sq.store(lds + buf * 2 * kTile, tid);
     sg.store(lds + (buf * 2 + 1) * kTile, tid);
     if (tid < RT) {
-      row_lse[buf][tid] = one_lse;
-      row_delta[buf][tid] = one_delta;
+      row_lse[buf][tid] = one_lse == -__builtin_inff() ? 0.0f : -one_lse * lse_unit;
+      row_delta[buf][tid] = -one_delta;
     }
   };
   auto half_tile = [&](int buf, int h, int v) {
@@ -1341,7 +1416,7 @@ AttnArgs args_of(const ocnn_attention_params& p) {
   a.p.left = std::min(p.left, 1 << 30);
   a.p.right = std::min(p.right, 1 << 30);
   a.group = p.heads / p.kv_heads;
-  a.scale2 = fabsf(p.scale) * kLog2e;
+  a.scale2 = std::max(fabsf(p.scale) * kLog2e, 0x1p-100f);   // (not zero: statistics are divided by it)
   return a;
 }
 
