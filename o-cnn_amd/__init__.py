@@ -21,4 +21,5 @@ from .nn import *  # noqa: F401,F403
 from .layers import (OctreeConvolution, OctreeConv, OctreeDeconv, OctreeConvFast,  # noqa: F401
                      OctreeDeconvFast, OctreeMaxPool, OctreeMaxUnpool, OctreeAvgPool, OctreePad,
                      OctreeDepad, OctreeTrilinear, OctreeInterp, OctreeAlign, octree_nearest_pts,
-                     octree_trilinear_pts, octree_trilinear, Octree2Col, Col2Octree)
+                     octree_trilinear_pts, octree_trilinear, Octree2Col, Col2Octree, OctreeRotary,
+                     OctreeAttention, OctreeRecurrence)

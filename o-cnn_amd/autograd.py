@@ -2,9 +2,11 @@
 pytorch/ocnn/octree_conv.py:15-68, octree_pool.py:7-61, octree_pad.py:7-41 and
 octree2col.py: each backward is the reference's choice of adjoint operator
 (conv <-> conv_grad, pool <-> unpool, unpool <-> mask_pool, pad <-> depad, octree2col <-> col2octree).
-Gradients are fp32, like every reference operator."""
+Gradients are fp32, like every reference operator; the operators along the node order of a level
+(rotary positions, attention, gated recurrence) also train in bf16."""
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import nn as F
 
@@ -177,6 +179,70 @@ class OctreeInterpFunction(Function):
     return (F.octree_interp_pts_grad(grad_out.contiguous(), idx, weight, H, method),) + (None,) * 5
 
 
+# The three below may be captured into a graph with their backward.  As with every torch function, an eager graph of the
+# same leaves must be gone by then: torch accumulates a leaf's gradient on the stream on which its oldest living graph was
+# made, and a capture that is pulled onto another stream does not end well.  torch.autograd.grad accumulates nothing.
+class OctreeRotaryFunction(Function):
+  """Rotary positions; the gradient is the turn back.  Positions and frequencies take none."""
+
+  @staticmethod
+  def forward(ctx, data, positions, frequencies, pairs, interleaved=False):
+    if any(ctx.needs_input_grad[1:3]):
+      raise F.OcnnError(-3, "positions and frequencies take no gradient")
+    ctx.save_for_backward(positions, frequencies)
+    ctx.cfg = (tuple(pairs), interleaved)
+    return F.octree_rotary(data, positions, frequencies, pairs, interleaved)
+
+  @staticmethod
+  @once_differentiable
+  def backward(ctx, grad):
+    positions, frequencies = ctx.saved_tensors
+    pairs, interleaved = ctx.cfg
+    return F.octree_rotary(grad, positions, frequencies, pairs, interleaved, inverse=True), None, None, None, None
+
+
+class OctreeAttentionFunction(Function):
+  """octree_attention, differentiable in q, k and v."""
+
+  @staticmethod
+  def forward(ctx, q, k, v, q_offsets, k_offsets=None, k_lengths=None, left=-1, right=-1, sinks=0, scale=None, key_mask=None):
+    out, lse = F.octree_attention(q, k, v, q_offsets, k_offsets, k_lengths, left, right, sinks, scale, key_mask, return_lse=True)
+    ctx.save_for_backward(q, k, v, out, lse, q_offsets, k_offsets, k_lengths, key_mask)
+    ctx.cfg = (left, right, sinks, scale)
+    return out
+
+  @staticmethod
+  @once_differentiable
+  def backward(ctx, grad):
+    q, k, v, out, lse, q_offsets, k_offsets, k_lengths, key_mask = ctx.saved_tensors
+    left, right, sinks, scale = ctx.cfg
+    return F.octree_attention_grad(grad, q, k, v, out, lse, q_offsets, k_offsets, k_lengths, left, right, sinks, scale,
+                                   key_mask) + (None,) * 8
+
+
+class OctreeRecurrenceFunction(Function):
+  """octree_recurrence -> (h, last), differentiable in gate, data and state."""
+
+  @staticmethod
+  def forward(ctx, gate, data, offsets, state=None, reverse=False):
+    out, last, carries = F.octree_recurrence(gate, data, offsets, state, reverse, return_carries=True)
+    ctx.save_for_backward(gate, data, offsets, state, carries)
+    ctx.reverse = reverse
+    ctx.set_materialize_grads(False)
+    return out, last
+
+  @staticmethod
+  @once_differentiable
+  def backward(ctx, grad, grad_last):
+    gate, data, offsets, state, carries = ctx.saved_tensors
+    if grad is None:
+      if grad_last is None:
+        return (None,) * 5
+      grad = torch.zeros_like(data)
+    g, x, s = F.octree_recurrence_grad(grad, gate, data, offsets, carries, state, grad_last, ctx.reverse)
+    return g, x, None, s if state is not None else None, None
+
+
 octree_conv = OctreeConvFunction.apply
 octree_deconv = OctreeDeconvFunction.apply
 octree_max_pool = OctreeMaxPoolFunction.apply
@@ -188,3 +254,6 @@ octree2col = Octree2ColFunction.apply
 col2octree = Col2OctreeFunction.apply
 octree_align = OctreeAlignFunction.apply
 octree_interp_pts = OctreeInterpFunction.apply
+octree_rotary = OctreeRotaryFunction.apply
+octree_attention = OctreeAttentionFunction.apply
+octree_recurrence = OctreeRecurrenceFunction.apply

@@ -1,6 +1,7 @@
 """Module front ends of the hot-path operators, with the class names and constructor
 signatures a user of the reference's `ocnn` package expects (pytorch/ocnn/octree_conv.py:75-158,
-octree_pool.py:69-103, octree_pad.py:47-72, octree2col.py:59-81, modules.py:209-318).
+octree_pool.py:69-103, octree_pad.py:47-72, octree2col.py:59-81, modules.py:209-318), and of the
+operators along the node order of a level, which the reference does not have.
 
 The reference writes one class per (direction, implementation) pair.  Here one module,
 `OctreeConvolution`, carries the whole rule set of the operator:
@@ -227,3 +228,101 @@ class OctreeAlign(_LevelModule):
 
   def forward(self, data, src_octree, des_octree):
     return F.octree_align(data, src_octree, des_octree, self.depth)
+
+
+# ---- mixing along the node order of a level (no counterpart in the reference) ----------------------------
+def _as_rows(data):
+  """[1, C, H, 1] -> [H, C]"""
+  return data[0, :, :, 0].t().contiguous()
+
+
+def _as_channels(rows):
+  """[H, C] -> [1, C, H, 1]"""
+  return rows.t().contiguous()[None, :, :, None]
+
+
+class OctreeRotary(nn.Module):
+  """Rotary positions of the nodes of a level: data [rows, heads, dim], `pairs[i]` pairs of channels turn with
+  axis i (x, y, z).  `positions`: octree_positions(octree, depth), or any that octree_rotary takes."""
+
+  def __init__(self, pairs, base=10000.0, interleaved=False):
+    super().__init__()
+    self.pairs, self.base, self.interleaved = [int(n) for n in pairs], float(base), interleaved
+    self._frequencies = {}      # by device; kept out of the module's tensors: they stay 64 bits under .to(bfloat16)
+
+  def forward(self, data, positions):
+    from . import nn as ops
+    if data.device not in self._frequencies:
+      self._frequencies[data.device] = ops.rotary_frequencies(self.pairs, self.base, device=data.device)
+    return F.octree_rotary(data, positions, self._frequencies[data.device], self.pairs, self.interleaved)
+
+  def extra_repr(self):
+    return 'pairs={}, base={}, interleaved={}'.format(self.pairs, self.base, self.interleaved)
+
+
+class OctreeAttention(_LevelModule):
+  """Attention between the nodes of a level, octree by octree, along the Morton order: every node sees the nodes
+  from `left` before to `right` behind it and the first `sinks` of its octree (-1: no bound).  Query, key and value
+  come from one 1x1x1 convolution, the result goes through another; queries and keys turn with the nodes'
+  coordinates, a third of a head's channels with each axis (rotary=False: not at all).
+  [1, channels, H, 1] -> the same shape; H: the nodes (nempty: the non-empty nodes) of `depth`."""
+
+  def __init__(self, depth, channels, heads, kv_heads=None, left=-1, right=-1, sinks=0, nempty=False, rotary=True):
+    super().__init__(depth)
+    self.heads, self.kv_heads = heads, heads if kv_heads is None else kv_heads
+    if channels % heads or self.heads % self.kv_heads:
+      raise ValueError("%d channels in %d heads over %d key heads" % (channels, heads, self.kv_heads))
+    self.dim, self.nempty = channels // heads, nempty
+    self.left, self.right, self.sinks = left, right, sinks
+    self.qkv = nn.Parameter(torch.empty((heads + 2 * self.kv_heads) * self.dim, channels))
+    self.out = nn.Parameter(torch.empty(channels, channels))
+    nn.init.xavier_uniform_(self.qkv)
+    nn.init.xavier_uniform_(self.out)
+    third = self.dim // 6
+    self.rotary = OctreeRotary([third] * 3) if rotary and third else None
+
+  def forward(self, data, octree):
+    from . import nn as ops
+    project = ((1, 1, 1), 1, self.nempty)
+    joint = F.octree_conv(data, self.qkv, octree, self.depth, self.qkv.shape[0], *project)
+    joint = _as_rows(joint).unflatten(1, (-1, self.dim))
+    q, k, v = joint.split([self.heads, self.kv_heads, self.kv_heads], dim=1)
+    if self.rotary is not None:
+      positions = ops.octree_positions(octree, self.depth, self.nempty)
+      q, k = self.rotary(q, positions), self.rotary(k, positions)
+    offsets = ops.octree_offsets(octree, self.depth, self.nempty)
+    mixed = F.octree_attention(q, k, v, offsets, None, None, self.left, self.right, self.sinks)
+    return F.octree_conv(_as_channels(mixed.flatten(1)), self.out, octree, self.depth, self.out.shape[0], *project)
+
+  def extra_repr(self):
+    return 'depth={}, heads={}, kv_heads={}, dim={}, left={}, right={}, sinks={}, nempty={}'.format(
+        self.depth, self.heads, self.kv_heads, self.dim, self.left, self.right, self.sinks, self.nempty)
+
+
+class OctreeRecurrence(_LevelModule):
+  """Gated linear recurrence along the Morton order of a level, octree by octree; gate and value come from one
+  1x1x1 convolution, the result goes through another.  both=True: half of the channels run from an octree's
+  last node to its first.  [1, channels, H, 1] -> the same shape."""
+
+  def __init__(self, depth, channels, nempty=False, both=True):
+    super().__init__(depth)
+    self.channels, self.nempty, self.both = channels, nempty, both
+    self.gate_value = nn.Parameter(torch.empty(2 * channels, channels))
+    self.out = nn.Parameter(torch.empty(channels, channels))
+    nn.init.xavier_uniform_(self.gate_value)
+    nn.init.xavier_uniform_(self.out)
+
+  def forward(self, data, octree):
+    from . import nn as ops
+    project = ((1, 1, 1), 1, self.nempty)
+    joint = _as_rows(F.octree_conv(data, self.gate_value, octree, self.depth, 2 * self.channels, *project))
+    gate, value = joint.split(self.channels, dim=1)
+    offsets = ops.octree_offsets(octree, self.depth, self.nempty)
+    cut = self.channels // 2 if self.both else 0
+    parts = [F.octree_recurrence(gate[:, cut:], value[:, cut:], offsets)[0]]
+    if cut:
+      parts.insert(0, F.octree_recurrence(gate[:, :cut], value[:, :cut], offsets, None, True)[0])
+    return F.octree_conv(_as_channels(torch.cat(parts, 1)), self.out, octree, self.depth, self.channels, *project)
+
+  def extra_repr(self):
+    return 'depth={}, channels={}, nempty={}, both={}'.format(self.depth, self.channels, self.nempty, self.both)

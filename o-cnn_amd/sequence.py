@@ -18,9 +18,9 @@ import torch
 
 from . import lib as _lib
 from .lib import OcnnError, AttentionParams
-from .nn import _dtype_code, _ptr, _stream, _to_dev, octree_info
+from .nn import _dtype_code, _ptr, _stream, _to_dev, octree_info, octree_property
 
-__all__ = ["octree_offsets", "rotary_frequencies", "octree_rotary", "octree_attention", "octree_attention_grad",
+__all__ = ["octree_offsets", "octree_positions", "rotary_frequencies", "octree_rotary", "octree_attention", "octree_attention_grad",
            "octree_recurrence", "octree_recurrence_grad"]
 
 _POS_INT32, _POS_F32, _POS_XYZ = 0, 1, 2
@@ -135,6 +135,20 @@ def octree_offsets(octree, depth, nempty=False):
   out = torch.empty(info.batch_size + 1, dtype=torch.int32, device=octree.device)
   _call(octree.device, "ocnn_octree_offsets", _ptr(out), _ptr(octree), info.p, int(depth), int(bool(nempty)))
   return out
+
+
+def octree_positions(octree, depth, nempty=False):
+  """Packed coordinates (int64, 16 bits an axis) of the nodes (nempty: the non-empty nodes) of a level, in node
+  order: what octree_rotary takes as positions."""
+  octree = _to_dev(octree)
+  xyz = octree_property(octree, "xyz", depth)
+  if not nempty:
+    return xyz
+  count = octree_info(octree).nnum_nempty(depth)
+  child = octree_property(octree, "child", depth).long()
+  out = torch.empty(count + 1, dtype=xyz.dtype, device=xyz.device)     # (the last entry takes the empty nodes)
+  out[torch.where(child >= 0, child, count)] = xyz
+  return out[:count]
 
 
 # ---- rotary positions -----------------------------------------------------------------------------

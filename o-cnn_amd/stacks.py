@@ -10,6 +10,8 @@ applies bias and ReLU to the accumulator before the store.
   unet_trunk   encoder / decoder with 2x2x2 stride-2 down-convolutions and deconvolutions and
                skip concatenations, the op order of pytorch/ocnn/unet.py:61-92 with one
                convolution per stage
+  node_mixer   attention with rotary positions and a gated recurrence along the nodes of a level,
+               optional between the encoder and the decoder of unet_trunk
 """
 import torch
 
@@ -77,8 +79,40 @@ def lenet_trunk_rows(octree, depth, params, data=None, to_depth=2, constant_weig
   return F.from_rows(x, cin)
 
 
+def node_mixer(data, octree, depth, mix, nempty=False):
+  """Mixing along the Morton order of a level, octree by octree, at inference (layers.OctreeAttention and
+  layers.OctreeRecurrence train): data + out(attention(rotary(q), rotary(k), v)), and where `mix` has a "scan", that
+  plus scan_out(recurrence(gate, value)).  The reference's networks stop at convolutions.
+  mix: "qkv", "out" and optionally "scan", "scan_out": (w, b) of 1x1x1 convolutions; "heads", "kv_heads", "pairs"
+  (pairs of channels that turn with x, y, z), "left", "right", "sinks" as in nn.octree_attention."""
+  offsets = F.octree_offsets(octree, depth, nempty)
+
+  def project(x, weights, to_rows=True):
+    w, b = weights
+    if not to_rows:
+      x = x.t().contiguous()[None, :, :, None]
+    x = conv_bn_relu(x, w, b, octree, depth, w.shape[0], (1, 1, 1), nempty=nempty, relu=False)
+    return x[0, :, :, 0].t().contiguous() if to_rows else x
+
+  heads, kv = mix["heads"], mix["kv_heads"]
+  joint = project(data, mix["qkv"]).unflatten(1, (heads + 2 * kv, -1))
+  if sum(mix["pairs"]):
+    turned = joint[:, :heads + kv]
+    F.octree_rotary(turned, F.octree_positions(octree, depth, nempty),
+                    F.rotary_frequencies(mix["pairs"], device=data.device), mix["pairs"], out=turned)
+  mixed = F.octree_attention(joint[:, :heads], joint[:, heads:heads + kv], joint[:, heads + kv:], offsets,
+                             left=mix["left"], right=mix["right"], sinks=mix["sinks"])
+  data = data + project(mixed.flatten(1), mix["out"], to_rows=False)
+  if "scan" in mix:
+    gate, value = project(data, mix["scan"]).chunk(2, dim=1)
+    h, _ = F.octree_recurrence(gate, value, offsets)
+    data = data + project(h, mix["scan_out"], to_rows=False)
+  return data
+
+
 def unet_trunk(octree, depth, params, data=None, stages=3, nempty=False):
-  """params: dict with keys ('conv', d), ('down', d), ('up', d), ('dec', d) -> (w, b).
+  """params: dict with keys ('conv', d), ('down', d), ('up', d), ('dec', d) -> (w, b), and optionally
+  ('mix', d) for the coarsest level d = depth - stages: what node_mixer takes, run between encoder and decoder.
   Encoder: conv at `depth`, then per stage a 2x2x2 stride-2 conv to depth-1 and a 3x3x3 conv;
   decoder: per stage a 2x2x2 stride-2 deconv to depth+1, concatenation with the encoder
   feature of that depth, and a 3x3x3 conv."""
@@ -110,6 +144,8 @@ def unet_trunk(octree, depth, params, data=None, stages=3, nempty=False):
     d -= 1
     feats[d] = encoder_conv(x, d, i + 1 < stages)
   x = feats[d]
+  if ("mix", d) in params:
+    x = node_mixer(x, octree, d, params[("mix", d)], nempty)
   for _ in range(stages):
     w, b = params[("up", d)]
     cout = w.shape[1] // 8
@@ -163,6 +199,8 @@ def unet_trunk_rows(octree, depth, params, data=None, stages=3, nempty=False, co
     d -= 1
     feats[d] = encoder_conv(x, w.shape[0], d, i + 1 < stages)
   x, cin = feats[d]
+  if ("mix", d) in params:
+    x = F.to_rows(node_mixer(F.from_rows(x, cin), octree, d, params[("mix", d)], nempty))
   for _ in range(stages):
     w, b = params[("up", d)]
     cout = w.shape[1] // 8
