@@ -26,6 +26,14 @@ namespace {
 
 // wavefronts a SIMD that the registers leave room for, by the bytes of a row
 constexpr int forward_waves(int row) { return row <= 128 ? 3 : row <= 256 ? 2 : 1; }
+// The gradients of the scores are not rounded to bf16 once but held as two bf16 (one more product): rounded once they leave dq
+// and dk 1.42 times as far off as the rounding of dq and dk themselves does (16 x 1500 rows, window 512, 8 heads of 64, forward
+// and backward: 203 us rounded once, 224 us so).
+constexpr bool kFine = true;
+// dO . o with the o that was rounded to bf16 leaves dq 2.0 times as far off as its own rounding does where a row sees 2 keys,
+// 1.19 times with 9, 1.06 with 33, 1.01 with 512.  Rows of up to kFewKeys keys get rowsum(P dP) from a pass of its own.
+constexpr int kFewKeys = 32;
+
 constexpr int grad_q_waves(int row) { return row <= 64 ? 3 : row <= 192 ? 2 : 1; }
 constexpr int grad_kv_waves(int row) { return row <= 128 ? 2 : 1; }
 
@@ -145,8 +153,9 @@ __device__ inline uint32_t pack_bf16(float lo, float hi) {
 }
 
 // The fragments of 32 rows of a tile, by channel, for  acc[block][channel][column] += sum over the rows of
-// tile[row][channel] * w[row][column], w as an accumulator of rows_times holds it.  bf16: w is rounded to bf16 (2^-8 of
-// each weight at most, as the tile's own elements are); statistics and sums stay in 32 bits.
+// tile[row][channel] * w[row][column], w as an accumulator of rows_times holds it.  bf16: w is rounded to bf16 (half a
+// step, 2^-9 of each weight, as the tile's own elements are); statistics and sums stay in 32 bits.  FINE: what the rounding
+// left is multiplied too, rounded by itself, so that a weight is 2^-18 off at most.
 template <typename T, int DP> struct ColumnFrags;
 template <int DP> struct ColumnFrags<uint16_t, DP> {
   using S = Shape<uint16_t, DP>;
@@ -164,15 +173,24 @@ template <int DP> struct ColumnFrags<uint16_t, DP> {
         v[s][d] = __builtin_bit_cast(bf16x8, a);
       }
   }
-  __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
+  template <bool FINE = false> __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      uintx4 b;
+      uintx4 b, c;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = pack_bf16(w[8 * s + 2 * i], w[8 * s + 2 * i + 1]);
+      for (int i = 0; i < 4; ++i) {
+        const float x = w[8 * s + 2 * i], y = w[8 * s + 2 * i + 1];
+        b[i] = pack_bf16(x, y);
+        if constexpr (FINE) c[i] = pack_bf16(x - __uint_as_float(b[i] << 16), y - __uint_as_float(b[i] & 0xffff0000u));
+      }
       const bf16x8 bw = __builtin_bit_cast(bf16x8, b);
 #pragma unroll
       for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[s][d], bw, acc[d]);
+      if constexpr (FINE) {
+        const bf16x8 cw = __builtin_bit_cast(bf16x8, c);
+#pragma unroll
+        for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[s][d], cw, acc[d]);
+      }
     }
   }
 };
@@ -187,7 +205,7 @@ template <int DP> struct ColumnFrags<float, DP> {
 #pragma unroll
       for (int d = 0; d < S::kBlocks; ++d) v[r][d] = at[(8 * (r >> 2) + (r & 3)) * S::kPitch + 32 * d];
   }
-  __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
+  template <bool = false> __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
 #pragma unroll
     for (int r = 0; r < 16; ++r)
 #pragma unroll
@@ -885,11 +903,13 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
 #pragma unroll
     for (int e = 0; e < S::kPiece; ++e) delta = fmaf((float)q.v[i][e], (float)go.v[i][e], delta);
   delta += __shfl_xor(delta, 32, 64);
+  const int sees = p.left >= 0 && p.right >= 0 ? min(p.left + p.right + 1 + p.sinks, s.keys) : s.keys;
+  const bool exact = sizeof(T) == 2 && sees <= kFewKeys;
   load_row<T, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   const int64_t at_row = at * p.heads + head;
   const float lse = have ? a.lse[at_row] : -__builtin_inff();
   const float lse2 = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
-  if (have && half == 0) a.delta[at_row] = delta;
+  if (have && half == 0 && !exact) a.delta[at_row] = delta;
 
   floatx16 dq[S::kBlocks];
 #pragma unroll
@@ -930,8 +950,24 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
     }
     cf[1].load(kt + 32 * S::kPitch);
     in_order();
-    cf[0].times(dq, x[0]);
-    cf[1].times(dq, x[1]);
+    cf[0].template times<kFine>(dq, x[0]);
+    cf[1].template times<kFine>(dq, x[1]);
+  };
+  // the share of these keys in rowsum(P dP)
+  auto weigh = [&](const T* kt, const T* vt, int j0, uint64_t live) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      RowFrags<T, DP> kf, vf;
+      kf.load(kt + i * 32 * S::kPitch);
+      vf.load(vt + i * 32 * S::kPitch);
+      floatx16 dp = zero16(), x = zero16();
+      rows_times<T, DP>(kf, q, x, vf, go, dp);
+      const uint32_t seen = seen_bits(j0 + 32 * i, (uint32_t)(live >> (32 * i)));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += where_seen(seen, r, __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -lse2)) * dp[r], 0u);
+    }
+    return sum;
   };
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
   Staged<T, DP, KT, 256, true> sk, sv;
@@ -949,19 +985,29 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
       sv.load(vbase + (int64_t)j0 * p.v_row, tid, s.keys - j0);
     }
   };
-  if (tiles > 0) fetch(0);
   T* kt = lds;
-  for (int v = 0; v < tiles; ++v) {
-    T* vt = kt + kTile;
-    sk.store(kt, tid);
-    sv.store(vt, tid);
-    const uint64_t live = next;
-    __syncthreads();
-    if (v + 1 < tiles) fetch(v + 1);
-    const int j0 = tile_key(v);
-    if (reach(j0)) keys(kt, vt, j0, live);
-    kt = kt == lds ? lds + 2 * kTile : lds;
-  }
+  auto over = [&](auto use) {
+    if (tiles > 0) fetch(0);
+    for (int v = 0; v < tiles; ++v) {
+      T* vt = kt + kTile;
+      sk.store(kt, tid);
+      sv.store(vt, tid);
+      const uint64_t live = next;
+      __syncthreads();
+      if (v + 1 < tiles) fetch(v + 1);
+      const int j0 = tile_key(v);
+      if (reach(j0)) use(vt, j0, live);
+      kt = kt == lds ? lds + 2 * kTile : lds;
+    }
+  };
+  if constexpr (sizeof(T) == 2)
+    if (exact) {
+      delta = 0.0f;
+      over([&](const T* vt, int j0, uint64_t live) { delta += weigh(kt, vt, j0, live); });
+      delta += __shfl_xor(delta, 32, 64);
+      if (have && half == 0) a.delta[at_row] = delta;
+    }
+  over([&](const T* vt, int j0, uint64_t live) { keys(kt, vt, j0, live); });
   float worst = 0.0f;
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d)
@@ -1057,6 +1103,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
     int near_items) {
   using S = Shape<T, DP>;
   constexpr int RT = 64, kTile = RT * S::kPitch;
+  constexpr bool kLate = sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
   __shared__ float row_lse[2][RT], row_delta[2][RT];
   const ocnn_attention_params& p = a.p;
@@ -1143,17 +1190,20 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
     RowFrags<T, DP> qf, gf;
     qf.load(qt);
     gf.load(gt);
-    // the products start from -lse and -dO . o of their rows, in the units of the scores
-    floatx16 x, dp;
+    // The products start from -lse and -dO . o of their rows, in the units of the scores.  fp32: the lse is taken off
+    // behind, since it may be many times a score, and every step of the product would round at its size (dk and dv of
+    // 700 queries: 1.1e-6 off instead of 6e-7).
+    floatx16 x = zero16(), dp, ls;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const floatx4 ls = *(const floatx4*)(lse2 + 8 * i + 4 * half), de = *(const floatx4*)(delta + 8 * i + 4 * half);
+      const floatx4 l4 = *(const floatx4*)(lse2 + 8 * i + 4 * half), d4 = *(const floatx4*)(delta + 8 * i + 4 * half);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[4 * i + e] = ls[e];
-        dp[4 * i + e] = de[e];
+        ls[4 * i + e] = l4[e];
+        dp[4 * i + e] = d4[e];
       }
     }
+    if constexpr (!kLate) x = ls;
     in_order();
     rows_times<T, DP>(qf, k, x, gf, vv, dp);
     ColumnFrags<T, DP> gc, qc;
@@ -1161,7 +1211,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
     in_order();
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      x[r] = __builtin_amdgcn_exp2f(x[r] * a.scale2);
+      x[r] = __builtin_amdgcn_exp2f(kLate ? fmaf(x[r], a.scale2, ls[r]) : x[r] * a.scale2);
       dp[r] *= x[r];
     }
     if (masked) {
@@ -1175,7 +1225,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
     qc.load(qt);
     in_order();
     gc.times(dv, x);
-    qc.times(dk, dp);
+    qc.template times<kFine>(dk, dp);
   };
 
   // a tile holds whole tokens: `step` of them, group rows each, so that a thread's rows keep their offsets
@@ -1188,7 +1238,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
   sg.init(tid, p.dim, [&](int i) { const int t = i / a.group; return t * (int)a.grad_row + (i - t * a.group) * (int)a.grad_head; });
   const int my_token = tid / a.group;
   const int64_t my_stat = (int64_t)(s.q0 + ta + my_token) * p.heads + kv * a.group + tid - my_token * a.group;
-  const float lse_unit = kLog2e / a.scale2;
+  const float lse_unit = kLate ? kLog2e : kLog2e / a.scale2;
   float one_lse = 0.0f, one_delta = 0.0f;
   auto fetch = [&](int v) {
     const int t = v * step, rows = min(tb - ta - t, step) * a.group;

@@ -20,6 +20,15 @@ template <typename T, int N> struct Pack {
   T v[N];
   __device__ inline void load(const T* p) { __builtin_memcpy(v, p, sizeof(v)); }
   __device__ inline void store(T* p) const { __builtin_memcpy(p, v, sizeof(v)); }
+  // past the caches: what is written is not read again soon, and must not displace what is
+  __device__ inline void store_past(T* p) const {
+    if constexpr (sizeof(v) >= 8) {
+      typedef uint32_t words __attribute__((ext_vector_type(sizeof(v) / 4)));
+      __builtin_nontemporal_store(__builtin_bit_cast(words, v), (words*)p);
+    } else {
+      store(p);
+    }
+  }
   __device__ inline void fill(T x) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = x;

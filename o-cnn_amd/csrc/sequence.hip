@@ -217,6 +217,7 @@ struct ScanArgs {
   const int* offsets;
   int n_seq, rows, channels, groups, reverse, fill;
   int64_t threads;                                // ids x groups
+  bool past;                                      // results go past the caches
 };
 
 constexpr int kScanRows = 8;   // rows whose loads are in flight together
@@ -496,7 +497,8 @@ __global__ void __launch_bounds__(kBlock) scan_apply_kernel(ScanArgs a) {
           h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
           x[j].v[v] = from_f32<T>(h[v]);
         }
-        x[j].store(out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row);
+        T* to = out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row;
+        if (a.past) x[j].store_past(to); else x[j].store(to);
       }
   }
   if (a.last && (int64_t)(ch.index + 1) * L >= ch.length)
@@ -643,7 +645,8 @@ __global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
           h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
           x[j].v[v] = from_f32<T>(h[v]);
         }
-        x[j].store(out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row);
+        T* to = out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row;
+        if (a.past) x[j].store_past(to); else x[j].store(to);
       }
   }
   if (a.last)
@@ -850,6 +853,9 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
   OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence needs %zu bytes, got %zu", need,
       workspace_bytes);
   a.carry = carries;
+  // (bf16, 256 channels, past the caches and not: 262147 rows 123.5 / 134 us, 131072 rows 67.6 / 67.4; an operator that reads
+  // the result next then loses 2 to 3 us up to 65536 rows and nothing from 200000 on)
+  a.past = (int64_t)rows * channels * size >= (96ll << 20);
   scan_lists(&a, ids, workspace_dev);
   by_width(v, [&](auto w) {
     by_chunk(shift, [&](auto l) {
