@@ -24,8 +24,6 @@
 namespace ocnn {
 namespace {
 
-// wavefronts a SIMD that the registers leave room for, by the bytes of a row
-constexpr int forward_waves(int row) { return row <= 128 ? 3 : row <= 256 ? 2 : 1; }
 // The gradients of the scores are not rounded to bf16 once but held as two bf16 (one more product): rounded once they leave dq
 // and dk 1.42 times as far off as the rounding of dq and dk themselves does (16 x 1500 rows, window 512, 8 heads of 64, forward
 // and backward: 203 us rounded once, 224 us so).
@@ -34,8 +32,6 @@ constexpr bool kFine = true;
 // 1.19 times with 9, 1.06 with 33, 1.01 with 512.  Rows of up to kFewKeys keys get rowsum(P dP) from a pass of its own.
 constexpr int kFewKeys = 32;
 
-constexpr int grad_q_waves(int row) { return row <= 64 ? 3 : row <= 192 ? 2 : 1; }
-constexpr int grad_kv_waves(int row) { return row <= 128 ? 2 : 1; }
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -62,21 +58,41 @@ struct AttnArgs {
   float scale2;                                               // |scale| * log2(e); a negative scale turns one operand around
 };
 
-template <typename T> struct Frag;
-template <> struct Frag<uint16_t> { using type = bf16x8; };
+// How an element is held: bf16; fp32 (v_mfma_f32_32x32x2_f32); Planes: fp32 in memory and three bf16 in LDS and operands,
+// x = hi + mid + lo with 8 significant bits each.  A product of two is six of the nine bf16 products (mid lo, lo mid and lo lo
+// stay below 2^-26 of it), 192 cycles for 16 channels instead of 512.  What is left out: below 2^-108 an element's lo (then its
+// mid) is a bf16 denormal, and beyond the largest bf16 it is infinite, as the weights of a row that is taken again.
+struct Planes {};
+template <typename E> struct Elem { using Memory = E; using Lds = E; static constexpr int kPlanes = 1; };
+template <> struct Elem<Planes> { using Memory = float; using Lds = uint16_t; static constexpr int kPlanes = 3; };
+template <typename E> struct Frag { using type = bf16x8; };
 template <> struct Frag<float> { using type = floatx4; };
 
-// What a tile of rows looks like in LDS and in operands.  A 16-byte piece is kPiece elements; one step of the
+// What a tile of rows looks like in LDS and in operands.  A 16-byte piece of an operand is kPiece elements; one step of the
 // contraction over channels takes two pieces, one from each half of the wavefront.
-template <typename T, int DP> struct Shape {
-  static constexpr int kPiece = 16 / (int)sizeof(T);
+template <typename E, int DP> struct Shape {
+  using Memory = typename Elem<E>::Memory;
+  using Lds = typename Elem<E>::Lds;
+  static constexpr int kPiece = 16 / (int)sizeof(Lds), kMemoryPiece = 16 / (int)sizeof(Memory);
   static constexpr int kSteps = DP / (2 * kPiece);
-  static constexpr int kPieces = DP / kPiece;           // of a row
+  static constexpr int kPieces = DP / kMemoryPiece;     // of a row in memory
   static constexpr int kPitch = DP + kPiece;            // one piece of padding: rows start 4 banks apart
   static constexpr int kBlocks = DP / 32;               // 32-channel blocks of a transposed accumulator
+  static constexpr int kPlanes = Elem<E>::kPlanes;
+  static constexpr int kPlane = 64 * kPitch;            // (tiles in planes have 64 rows)
 };
+// wavefronts a SIMD that the registers leave room for
+template <typename E> constexpr int forward_waves(int dp) {
+  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 128 ? 3 : dp * (int)sizeof(E) <= 256 ? 2 : 1;
+}
+template <typename E> constexpr int grad_q_waves(int dp) {
+  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 64 ? 3 : dp * (int)sizeof(E) <= 192 ? 2 : 1;
+}
+template <typename E> constexpr int grad_kv_waves(int dp) {
+  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 128 ? 2 : 1;
+}
 // a lane's pieces of one row: a column of a B operand
-template <typename T, int DP> struct Column { typename Frag<T>::type v[Shape<T, DP>::kSteps]; };
+template <typename E, int DP> struct Column { typename Frag<E>::type v[Shape<E, DP>::kPlanes][Shape<E, DP>::kSteps]; };
 
 __device__ inline floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -94,20 +110,73 @@ __device__ inline floatx16 zero16() {
   return z;
 }
 
+__device__ inline uint32_t pack_bf16(float lo, float hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  bf16x2 v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+// two floats as the bf16 next to them; what that leaves stays in x, y (exact: it has fewer bits)
+__device__ inline uint32_t take_bf16(float& x, float& y) {
+  const uint32_t b = pack_bf16(x, y);
+  x -= __uint_as_float(b << 16);
+  y -= __uint_as_float(b & 0xffff0000u);
+  return b;
+}
+
 // The lane's pieces of a row (a column of a B operand), straight from memory; zeros where the row or the
 // channels do not exist.
-template <typename T, int DP>
-__device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim, bool negate = false) {
-  using S = Shape<T, DP>;
+template <typename E, int DP>
+__device__ inline void load_row(Column<E, DP>& f, const typename Elem<E>::Memory* row, bool ok, int dim, bool negate = false) {
+  using S = Shape<E, DP>;
   const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) {
     const int c = (2 * s + half) * S::kPiece;
-    uintx4 v = {0, 0, 0, 0};
-    if (ok && c < dim) v = *(const uintx4*)(row + c);
-    if (negate) v ^= sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
-    f.v[s] = __builtin_bit_cast(typename Frag<T>::type, v);
+    uintx4 v = {0, 0, 0, 0}, w = {0, 0, 0, 0};
+    if (ok && c < dim) {
+      v = *(const uintx4*)(row + c);
+      if constexpr (S::kPlanes == 3) w = *(const uintx4*)(row + c + 4);
+    }
+    if (negate) {
+      v ^= sizeof(typename S::Memory) == 2 ? 0x80008000u : 0x80000000u;
+      if constexpr (S::kPlanes == 3) w ^= 0x80000000u;
+    }
+    if constexpr (S::kPlanes == 3) {
+      floatx4 x = __builtin_bit_cast(floatx4, v), y = __builtin_bit_cast(floatx4, w);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        uintx4 b;
+        float t[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = take_bf16(t[2 * i], t[2 * i + 1]);
+        x = floatx4{t[0], t[1], t[2], t[3]};
+        y = floatx4{t[4], t[5], t[6], t[7]};
+        f.v[n][s] = __builtin_bit_cast(bf16x8, b);
+      }
+    } else {
+      f.v[0][s] = __builtin_bit_cast(typename Frag<E>::type, v);
+    }
   }
+}
+// the row's sum of x y, a share in each half of the wavefront
+template <typename T, int DP> __device__ inline float row_dot(const T* x, const T* y, bool ok, int dim) {
+  using S = Shape<T, DP>;
+  const int half = (threadIdx.x >> 5) & 1;
+  float sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    const int c = (2 * s + half) * S::kPiece;
+    Pack<T, S::kPiece> a, b;
+    a.fill(0);
+    b.fill(0);
+    if (ok && c < dim) {
+      a.load(x + c);
+      b.load(y + c);
+    }
+#pragma unroll
+    for (int e = 0; e < S::kPiece; ++e) sum = fmaf(to_f32(a.v[e]), to_f32(b.v[e]), sum);
+  }
+  return sum + __shfl_xor(sum, 32, 64);
 }
 
 // Keeps the compiler from moving instructions across.  It otherwise reads each fragment right in front of the
@@ -116,80 +185,93 @@ __device__ inline void load_row(Column<T, DP>& f, const T* row, bool ok, int dim
 __device__ inline void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // The fragments of 32 rows of a tile as the left operand of tile rows . column
-template <typename T, int DP> struct RowFrags {
-  using S = Shape<T, DP>;
-  typename Frag<T>::type v[S::kSteps];
-  __device__ inline void load(const T* tile) {
+template <typename E, int DP> struct RowFrags {
+  using S = Shape<E, DP>;
+  typename Frag<E>::type v[S::kPlanes][S::kSteps];
+  __device__ inline void load(const typename S::Lds* tile) {
     const int lane = threadIdx.x & 63;
-    const T* at = tile + (lane & 31) * S::kPitch + (lane >> 5) * S::kPiece;
+    const typename S::Lds* at = tile + (lane & 31) * S::kPitch + (lane >> 5) * S::kPiece;
 #pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) v[s] = *(const typename Frag<T>::type*)(at + 2 * s * S::kPiece);
+    for (int n = 0; n < S::kPlanes; ++n)
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) v[n][s] = *(const typename Frag<E>::type*)(at + n * S::kPlane + 2 * s * S::kPiece);
   }
 };
+// the planes whose products count, small ones first
+constexpr int kPairs = 6, kPairA[kPairs] = {0, 1, 2, 0, 1, 0}, kPairB[kPairs] = {2, 1, 0, 1, 0, 0};
 // two products whose steps alternate, so that none waits for the one before it
-template <typename T, int DP>
-__device__ inline void rows_times(const RowFrags<T, DP>& a, const Column<T, DP>& x, floatx16& ax, const RowFrags<T, DP>& b,
-    const Column<T, DP>& y, floatx16& by) {
+template <typename E, int DP>
+__device__ inline void rows_times(const RowFrags<E, DP>& a, const Column<E, DP>& x, floatx16& ax, const RowFrags<E, DP>& b,
+    const Column<E, DP>& y, floatx16& by) {
+  constexpr int first = Elem<E>::kPlanes == 3 ? 0 : kPairs - 1;
 #pragma unroll
-  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) {
-    ax = mma(a.v[s], x.v[s], ax);
-    by = mma(b.v[s], y.v[s], by);
-  }
+  for (int n = first; n < kPairs; ++n)
+#pragma unroll
+    for (int s = 0; s < Shape<E, DP>::kSteps; ++s) {
+      ax = mma(a.v[kPairA[n]][s], x.v[kPairB[n]][s], ax);
+      by = mma(b.v[kPairA[n]][s], y.v[kPairB[n]][s], by);
+    }
 }
-template <typename T, int DP>
-__device__ inline void rows_times(const RowFrags<T, DP>& a, const Column<T, DP>& x, floatx16& ax) {
+template <typename E, int DP>
+__device__ inline void rows_times(const RowFrags<E, DP>& a, const Column<E, DP>& x, floatx16& ax) {
+  constexpr int first = Elem<E>::kPlanes == 3 ? 0 : kPairs - 1;
 #pragma unroll
-  for (int s = 0; s < Shape<T, DP>::kSteps; ++s) ax = mma(a.v[s], x.v[s], ax);
+  for (int n = first; n < kPairs; ++n)
+#pragma unroll
+    for (int s = 0; s < Shape<E, DP>::kSteps; ++s) ax = mma(a.v[kPairA[n]][s], x.v[kPairB[n]][s], ax);
 }
 
 __device__ inline shortx4 read_transposed(const uint16_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)(p));
 }
 
-__device__ inline uint32_t pack_bf16(float lo, float hi) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  bf16x2 v = {(__bf16)lo, (__bf16)hi};
-  return __builtin_bit_cast(uint32_t, v);
-}
-
 // The fragments of 32 rows of a tile, by channel, for  acc[block][channel][column] += sum over the rows of
 // tile[row][channel] * w[row][column], w as an accumulator of rows_times holds it.  bf16: w is rounded to bf16 (half a
 // step, 2^-9 of each weight, as the tile's own elements are); statistics and sums stay in 32 bits.  FINE: what the rounding
 // left is multiplied too, rounded by itself, so that a weight is 2^-18 off at most.
-template <typename T, int DP> struct ColumnFrags;
-template <int DP> struct ColumnFrags<uint16_t, DP> {
-  using S = Shape<uint16_t, DP>;
-  bf16x8 v[2][S::kBlocks];
+template <typename E, int DP> struct ColumnFrags {            // (bf16 and planes)
+  using S = Shape<E, DP>;
+  bf16x8 v[S::kPlanes][2][S::kBlocks];
   __device__ inline void load(const uint16_t* tile) {
     const int lane = threadIdx.x & 63;
     // 16 lanes read 4 rows of 16 channels and get them back by channel
     const uint16_t* at = tile + ((lane >> 5) * 4 + ((lane >> 2) & 3)) * S::kPitch + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int n = 0; n < S::kPlanes; ++n)
 #pragma unroll
-      for (int d = 0; d < S::kBlocks; ++d) {
-        struct { shortx4 lo, hi; } a = {read_transposed(at + 16 * s * S::kPitch + 32 * d),
-                                        read_transposed(at + (16 * s + 8) * S::kPitch + 32 * d)};
-        v[s][d] = __builtin_bit_cast(bf16x8, a);
-      }
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int d = 0; d < S::kBlocks; ++d) {
+          struct { shortx4 lo, hi; } a = {read_transposed(at + n * S::kPlane + 16 * s * S::kPitch + 32 * d),
+                                          read_transposed(at + n * S::kPlane + (16 * s + 8) * S::kPitch + 32 * d)};
+          v[n][s][d] = __builtin_bit_cast(bf16x8, a);
+        }
   }
   template <bool FINE = false> __device__ inline void times(floatx16 (&acc)[S::kBlocks], const floatx16& w) const {
+    constexpr int kParts = S::kPlanes == 3 ? 3 : FINE ? 2 : 1;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      uintx4 b, c;
+      bf16x8 part[kParts];
+      float t[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = w[8 * s + 2 * i], y = w[8 * s + 2 * i + 1];
-        b[i] = pack_bf16(x, y);
-        if constexpr (FINE) c[i] = pack_bf16(x - __uint_as_float(b[i] << 16), y - __uint_as_float(b[i] & 0xffff0000u));
+      for (int i = 0; i < 8; ++i) t[i] = w[8 * s + i];
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) {
+        uintx4 b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = take_bf16(t[2 * i], t[2 * i + 1]);
+        part[n] = __builtin_bit_cast(bf16x8, b);
       }
-      const bf16x8 bw = __builtin_bit_cast(bf16x8, b);
+      if constexpr (S::kPlanes == 3) {
 #pragma unroll
-      for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[s][d], bw, acc[d]);
-      if constexpr (FINE) {
-        const bf16x8 cw = __builtin_bit_cast(bf16x8, c);
+        for (int n = 0; n < kPairs; ++n)
 #pragma unroll
-        for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[s][d], cw, acc[d]);
+          for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[kPairA[n]][s][d], part[kPairB[n]], acc[d]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kParts; ++n)
+#pragma unroll
+          for (int d = 0; d < S::kBlocks; ++d) acc[d] = mma(v[0][s][d], part[n], acc[d]);
       }
     }
   }
@@ -249,8 +331,9 @@ __device__ inline __amdgpu_buffer_rsrc_t buffer_at(const void* base) {
 
 // EVEN: rows a constant stride apart; the pieces of a thread are then too, and all but the first offset
 // are scalars (where the threads of a row divide the workgroup).
-template <typename T, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
-  using S = Shape<T, DP>;
+template <typename E, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
+  using S = Shape<E, DP>;
+  using T = typename S::Memory;
   static constexpr int kEach = ROWS * S::kPieces / THREADS;
   static_assert(kEach * THREADS == ROWS * S::kPieces, "whole pieces a thread");
   static constexpr bool kScalar = EVEN && THREADS % S::kPieces == 0;
@@ -264,7 +347,7 @@ template <typename T, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
   template <typename Offset> __device__ inline void init(int tid, int dim, Offset offset) {
 #pragma unroll
     for (int i = 0; i < (kScalar ? 1 : kEach); ++i) {
-      const int n = tid + i * THREADS, r = n / S::kPieces, c = (n % S::kPieces) * S::kPiece;
+      const int n = tid + i * THREADS, r = n / S::kPieces, c = (n % S::kPieces) * S::kMemoryPiece;
       at[i] = c < dim ? (uint32_t)(offset(r) + c) * (uint32_t)sizeof(T) : kNowhere;
     }
     apart = __builtin_amdgcn_readfirstlane(kScalar ? offset(THREADS / S::kPieces) * (int)sizeof(T) : 0);
@@ -284,11 +367,24 @@ template <typename T, int DP, int ROWS, int THREADS, bool EVEN> struct Staged {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) v[i] = piece(buf, i, live >> row_of(tid, i) & 1);
   }
-  __device__ inline void store(T* tile, int tid) const {
+  __device__ inline void store(typename S::Lds* tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int c = (kScalar ? tid : tid + i * THREADS) % S::kPieces * S::kPiece;
-      *(uintx4*)(tile + row_of(tid, i) * S::kPitch + c) = v[i];
+      const int c = (kScalar ? tid : tid + i * THREADS) % S::kPieces * S::kMemoryPiece;
+      typename S::Lds* at = tile + row_of(tid, i) * S::kPitch + c;
+      if constexpr (S::kPlanes == 3) {
+        static_assert(ROWS * S::kPitch == S::kPlane, "64 rows");
+        floatx4 x = __builtin_bit_cast(floatx4, v[i]);
+        float t[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+          typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+          const uint32_t b0 = take_bf16(t[0], t[1]), b1 = take_bf16(t[2], t[3]);
+          *(uintx2*)(at + n * S::kPlane) = uintx2{b0, b1};
+        }
+      } else {
+        *(uintx4*)at = v[i];
+      }
     }
   }
 };
@@ -351,12 +447,12 @@ __device__ inline int window_hi(const ocnn_attention_params& p, int pos, int key
 // four.  QW = 1 (few rows a sequence): 32 packed rows, and the wavefronts take every fourth tile of 32
 // keys each on their own, joined at the end.  Where rows x key heads leave compute units empty, the
 // tiles are dealt out over `splits` workgroups, joined by attention_join_kernel.
-template <typename T, int DP, int QW> struct ForwardShape {
+template <typename E, int DP, int QW> struct ForwardShape {
   static constexpr int kKeys = QW == 4 ? 64 : 32;
-  static constexpr int kTile = kKeys * Shape<T, DP>::kPitch;
+  static constexpr int kTile = kKeys * Shape<E, DP>::kPitch * Shape<E, DP>::kPlanes;
   static constexpr int kBuffers = QW == 4 ? 2 : 4;            // double buffer, or one a wavefront
   static constexpr size_t kJoin = QW == 4 ? 0 : 3 * (size_t)(DP / 32) * 16 * 64 * 4;
-  static constexpr size_t kTiles = (size_t)kBuffers * 2 * kTile * sizeof(T);
+  static constexpr size_t kTiles = (size_t)kBuffers * 2 * kTile * sizeof(typename Shape<E, DP>::Lds);
   static constexpr size_t kLds = kTiles > kJoin ? kTiles : kJoin;
 };
 
@@ -415,10 +511,12 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
   st->l = l;
 }
 
-template <typename T, int DP, int QW, bool SPLIT>
-__global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) attention_kernel(AttnArgs a) {
-  using S = Shape<T, DP>;
-  using F = ForwardShape<T, DP, QW>;
+template <typename E, int DP, int QW, bool SPLIT>
+__global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(AttnArgs a) {
+  using S = Shape<E, DP>;
+  using T = typename S::Memory;
+  using L = typename S::Lds;
+  using F = ForwardShape<E, DP, QW>;
   constexpr int kRows = 32 * QW, kShift = Log2<kRows>::value;
   __shared__ __attribute__((aligned(16))) char lds[F::kLds];
   __shared__ Softmax stats[4][32];
@@ -455,7 +553,7 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
     }
     if (a.fill && have && (QW == 4 || wave == 0)) {
       T* o = (T*)a.out + out_at * a.out_row + head * a.out_head;
-      for (int c = half * S::kPiece; c < p.dim; c += 2 * S::kPiece) *(uintx4*)(o + c) = uintx4{0, 0, 0, 0};
+      for (int c = half * S::kMemoryPiece; c < p.dim; c += 2 * S::kMemoryPiece) *(uintx4*)(o + c) = uintx4{0, 0, 0, 0};
       if (a.lse && half == 0) a.lse[out_at * p.heads + head] = -__builtin_inff();
     }
     return;
@@ -484,8 +582,8 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
   const int tiles = sink_tiles + t1 - t0;
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
 
-  Column<T, DP> q;
-  load_row<T, DP>(q, (const T*)p.q + out_at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
+  Column<E, DP> q;
+  load_row<E, DP>(q, (const T*)p.q + out_at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   floatx16 o[S::kBlocks];
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d) o[d] = zero16();
@@ -515,25 +613,25 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
   // not wait for a vote.  Only a weight beyond 2^100 of the base is too much: the tile says so, and the
   // workgroup takes all its tiles again, with the maximum of each (careful).
   bool careful = QW == 1, over = false;       // (QW = 1 waits for memory: careful from the start)
-  auto keys = [&](const T* kt, const T* vt, int j0, uint64_t live) {
+  auto keys = [&](const L* kt, const L* vt, int j0, uint64_t live) {
     constexpr int N = KT / 32;
     const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
     const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | ((live & all) != all));
     const bool measure = careful || decided(__any(m == -__builtin_inff()));
     floatx16 x[N];
     if constexpr (N == 2) {
-      RowFrags<T, DP> ka, kb;
+      RowFrags<E, DP> ka, kb;
       ka.load(kt);
       kb.load(kt + 32 * S::kPitch);
       in_order();
       x[0] = x[1] = zero16();
-      rows_times<T, DP>(ka, q, x[0], kb, q, x[1]);
+      rows_times<E, DP>(ka, q, x[0], kb, q, x[1]);
     } else {
-      RowFrags<T, DP> ka;
+      RowFrags<E, DP> ka;
       ka.load(kt);
       in_order();
       x[0] = zero16();
-      rows_times<T, DP>(ka, q, x[0]);
+      rows_times<E, DP>(ka, q, x[0]);
     }
     if (masked) {
       settle();
@@ -556,7 +654,7 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
     }
     const float base = m == -__builtin_inff() ? 0.0f : m;
     float sums[2 * N];
-    ColumnFrags<T, DP> vf[N];
+    ColumnFrags<E, DP> vf[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {             // the values of one half arrive while the other half's weights are formed
       vf[i].load(vt + i * 32 * S::kPitch);
@@ -585,7 +683,7 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
 
   constexpr int kThreads = QW == 4 ? 256 : 64;
   const int mine = QW == 4 ? tid : lane;
-  Staged<T, DP, KT, kThreads, true> sk, sv;
+  Staged<E, DP, KT, kThreads, true> sk, sv;
   sk.init(mine, p.dim, [&](int r) { return r * (int)p.k_row; });
   sv.init(mine, p.dim, [&](int r) { return r * (int)p.v_row; });
   uint64_t next = ~0ull;
@@ -605,10 +703,10 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
 #pragma unroll 1
     for (;;) {
       if (split < tiles) fetch(split);
-      T* kt = (T*)lds;
+      L* kt = (L*)lds;
 #pragma unroll 1
       for (int v = split; v < tiles; v += step) {
-        T* vt = kt + F::kTile;
+        L* vt = kt + F::kTile;
         sk.store(kt, tid);
         sv.store(vt, tid);
         const uint64_t live = next;
@@ -616,7 +714,7 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
         if (v + step < tiles) fetch(v + step);
         const int j0 = tile_key(v);
         if (reach(j0)) keys(kt, vt, j0, live);
-        kt = kt == (T*)lds ? (T*)lds + 2 * F::kTile : (T*)lds;
+        kt = kt == (L*)lds ? (L*)lds + 2 * F::kTile : (L*)lds;
       }
       if (careful || !__syncthreads_or(over)) break;
       careful = true;
@@ -626,8 +724,8 @@ __global__ void __launch_bounds__(256, forward_waves(DP * (int)sizeof(T))) atten
       for (int d = 0; d < S::kBlocks; ++d) o[d] = zero16();
     }
   } else {
-    T* kt = (T*)lds + wave * 2 * F::kTile;
-    T* vt = kt + F::kTile;
+    L* kt = (L*)lds + wave * 2 * F::kTile;
+    L* vt = kt + F::kTile;
     // (the splits take turns: at any time the workgroups together read one stretch of the keys, which spreads
     // over all memory channels; shares of their own, a power of two apart, met on a few of them)
     const int first = split * 4 + wave, step = 4 * (SPLIT ? a.splits : 1);
@@ -844,11 +942,13 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
   }
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attention_grad_q_kernel(AttnArgs a) {
-  using S = Shape<T, DP>;
-  constexpr int KT = 64, kTile = KT * S::kPitch, kRows = 128, kShift = 7;
-  __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
+template <typename E, int DP>
+__global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_kernel(AttnArgs a) {
+  using S = Shape<E, DP>;
+  using T = typename S::Memory;
+  using L = typename S::Lds;
+  constexpr int KT = 64, kTile = KT * S::kPitch * S::kPlanes, kRows = 128, kShift = 7;
+  __shared__ __attribute__((aligned(16))) L lds[2 * 2 * kTile];
   const ocnn_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y;
@@ -873,7 +973,7 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
   T* dq_row = (T*)a.dq + at * a.dq_row + head * a.dq_head;
   if (b >= p.n_seq) {
     if (have)
-      for (int c = half * S::kPiece; c < p.dim; c += 2 * S::kPiece) *(uintx4*)(dq_row + c) = uintx4{0, 0, 0, 0};
+      for (int c = half * S::kMemoryPiece; c < p.dim; c += 2 * S::kMemoryPiece) *(uintx4*)(dq_row + c) = uintx4{0, 0, 0, 0};
     return;
   }
   const int pos = token + s.shift();
@@ -894,18 +994,13 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
   const int sink_tiles = min((min(p.sinks, b_hi) + KT - 1) / KT, t0);
   const int tiles = sink_tiles + t1 - t0;
 
-  Column<T, DP> q, go;
-  load_row<T, DP>(go, (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
-  float delta = 0.0f;
-  load_row<T, DP>(q, (const T*)a.fwd + at * a.fwd_row + head * a.fwd_head, have, p.dim);
-#pragma unroll
-  for (int i = 0; i < S::kSteps; ++i)
-#pragma unroll
-    for (int e = 0; e < S::kPiece; ++e) delta = fmaf((float)q.v[i][e], (float)go.v[i][e], delta);
-  delta += __shfl_xor(delta, 32, 64);
+  Column<E, DP> q, go;
+  load_row<E, DP>(go, (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
+  float delta = row_dot<T, DP>((const T*)a.fwd + at * a.fwd_row + head * a.fwd_head,
+      (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
   const int sees = p.left >= 0 && p.right >= 0 ? min(p.left + p.right + 1 + p.sinks, s.keys) : s.keys;
   const bool exact = sizeof(T) == 2 && sees <= kFewKeys;
-  load_row<T, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
+  load_row<E, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   const int64_t at_row = at * p.heads + head;
   const float lse = have ? a.lse[at_row] : -__builtin_inff();
   const float lse2 = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
@@ -923,22 +1018,22 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
     return (live & first_bits(hi - j0) & (~first_bits(lo - j0) | first_bits(sinks - j0))) >> (4 * half);
   };
   auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + KT > w_lo) | (j0 < p.sinks)); };
-  auto keys = [&](const T* kt, const T* vt, int j0, uint64_t live) {
+  auto keys = [&](const L* kt, const L* vt, int j0, uint64_t live) {
     const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | (live != ~0ull));
     floatx16 x[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      RowFrags<T, DP> kf, vf;
+      RowFrags<E, DP> kf, vf;
       kf.load(kt + i * 32 * S::kPitch);
       vf.load(vt + i * 32 * S::kPitch);
       in_order();
       floatx16 dp = zero16();
       x[i] = zero16();
-      rows_times<T, DP>(kf, q, x[i], vf, go, dp);
+      rows_times<E, DP>(kf, q, x[i], vf, go, dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], a.scale2, -lse2)) * (dp[r] - delta);
     }
-    ColumnFrags<T, DP> cf[2];
+    ColumnFrags<E, DP> cf[2];
     cf[0].load(kt);
     if (masked) {
 #pragma unroll
@@ -954,15 +1049,15 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
     cf[1].template times<kFine>(dq, x[1]);
   };
   // the share of these keys in rowsum(P dP)
-  auto weigh = [&](const T* kt, const T* vt, int j0, uint64_t live) {
+  auto weigh = [&](const L* kt, const L* vt, int j0, uint64_t live) {
     float sum = 0.0f;
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
-      RowFrags<T, DP> kf, vf;
+      RowFrags<E, DP> kf, vf;
       kf.load(kt + i * 32 * S::kPitch);
       vf.load(vt + i * 32 * S::kPitch);
       floatx16 dp = zero16(), x = zero16();
-      rows_times<T, DP>(kf, q, x, vf, go, dp);
+      rows_times<E, DP>(kf, q, x, vf, go, dp);
       const uint32_t seen = seen_bits(j0 + 32 * i, (uint32_t)(live >> (32 * i)));
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += where_seen(seen, r, __builtin_amdgcn_exp2f(fmaf(x[r], a.scale2, -lse2)) * dp[r], 0u);
@@ -970,7 +1065,7 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
     return sum;
   };
   auto tile_key = [&](int v) { return (v < sink_tiles ? v : t0 + v - sink_tiles) * KT; };
-  Staged<T, DP, KT, 256, true> sk, sv;
+  Staged<E, DP, KT, 256, true> sk, sv;
   sk.init(tid, p.dim, [&](int r) { return r * (int)p.k_row; });
   sv.init(tid, p.dim, [&](int r) { return r * (int)p.v_row; });
   uint64_t next = ~0ull;
@@ -985,11 +1080,11 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
       sv.load(vbase + (int64_t)j0 * p.v_row, tid, s.keys - j0);
     }
   };
-  T* kt = lds;
+  L* kt = lds;
   auto over = [&](auto use) {
     if (tiles > 0) fetch(0);
     for (int v = 0; v < tiles; ++v) {
-      T* vt = kt + kTile;
+      L* vt = kt + kTile;
       sk.store(kt, tid);
       sv.store(vt, tid);
       const uint64_t live = next;
@@ -1003,11 +1098,11 @@ __global__ void __launch_bounds__(256, grad_q_waves(DP * (int)sizeof(T))) attent
   if constexpr (sizeof(T) == 2)
     if (exact) {
       delta = 0.0f;
-      over([&](const T* vt, int j0, uint64_t live) { delta += weigh(kt, vt, j0, live); });
+      over([&](const L* vt, int j0, uint64_t live) { delta += weigh(kt, vt, j0, live); });
       delta += __shfl_xor(delta, 32, 64);
       if (have && half == 0) a.delta[at_row] = delta;
     }
-  over([&](const T* vt, int j0, uint64_t live) { keys(kt, vt, j0, live); });
+  over([&](const L* vt, int j0, uint64_t live) { keys(kt, vt, j0, live); });
   float worst = 0.0f;
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d)
@@ -1098,13 +1193,15 @@ __device__ __forceinline__ void grad_k_row_again(const AttnArgs& a, const Seq& s
   }
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) attention_grad_kv_kernel(AttnArgs a,
+template <typename E, int DP>
+__global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_kernel(AttnArgs a,
     int near_items) {
-  using S = Shape<T, DP>;
-  constexpr int RT = 64, kTile = RT * S::kPitch;
+  using S = Shape<E, DP>;
+  using T = typename S::Memory;
+  using L = typename S::Lds;
+  constexpr int RT = 64, kTile = RT * S::kPitch * S::kPlanes;
   constexpr bool kLate = sizeof(T) == 4;
-  __shared__ __attribute__((aligned(16))) T lds[2 * 2 * kTile];
+  __shared__ __attribute__((aligned(16))) L lds[2 * 2 * kTile];
   __shared__ float row_lse[2][RT], row_delta[2][RT];
   const ocnn_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -1130,7 +1227,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
     const int k_begin = clamped(p.k_offsets, b, p.rows_k);
     const int64_t r = k_begin + item * 128 + wave * 32 + col;
     if (r < p.rows_k)
-      for (int c = half * S::kPiece; c < p.dim; c += 2 * S::kPiece) {
+      for (int c = half * S::kMemoryPiece; c < p.dim; c += 2 * S::kMemoryPiece) {
         *(uintx4*)((T*)a.dk + r * a.dk_row + kv * a.dk_head + c) = uintx4{0, 0, 0, 0};
         *(uintx4*)((T*)a.dv + r * a.dv_row + kv * a.dv_head + c) = uintx4{0, 0, 0, 0};
       }
@@ -1176,18 +1273,18 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
       all_hi = min(end_token(jw), tb) * a.group;
     }
   }
-  Column<T, DP> k, vv;
-  load_row<T, DP>(k, (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head, key, p.dim, p.scale < 0.0f);
-  load_row<T, DP>(vv, (const T*)p.v + (int64_t)(s.k0 + j) * p.v_row + kv * p.v_head, key, p.dim);
+  Column<E, DP> k, vv;
+  load_row<E, DP>(k, (const T*)p.k + (int64_t)(s.k0 + j) * p.k_row + kv * p.k_head, key, p.dim, p.scale < 0.0f);
+  load_row<E, DP>(vv, (const T*)p.v + (int64_t)(s.k0 + j) * p.v_row + kv * p.v_head, key, p.dim);
   floatx16 dk[S::kBlocks], dv[S::kBlocks];
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d) dk[d] = dv[d] = zero16();
 
   // 32 packed rows from r0 on, those before `end`
-  auto subtile = [&](const T* qt, const T* gt, const float* lse2, const float* delta, int r0, int end) {
+  auto subtile = [&](const L* qt, const L* gt, const float* lse2, const float* delta, int r0, int end) {
     if (r0 + 32 <= w_lo || r0 >= min(w_hi, end)) return;
     const bool masked = decided((r0 < all_lo) | (r0 + 32 > min(all_hi, end)));
-    RowFrags<T, DP> qf, gf;
+    RowFrags<E, DP> qf, gf;
     qf.load(qt);
     gf.load(gt);
     // The products start from -lse and -dO . o of their rows, in the units of the scores.  fp32: the lse is taken off
@@ -1205,8 +1302,8 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
     }
     if constexpr (!kLate) x = ls;
     in_order();
-    rows_times<T, DP>(qf, k, x, gf, vv, dp);
-    ColumnFrags<T, DP> gc, qc;
+    rows_times<E, DP>(qf, k, x, gf, vv, dp);
+    ColumnFrags<E, DP> gc, qc;
     gc.load(gt);
     in_order();
 #pragma unroll
@@ -1233,7 +1330,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves(DP * (int)sizeof(T))) atten
   const int tiles = s.keys > 0 && tb > ta ? (tb - ta + step - 1) / step : 0;
   const T* qbase = (const T*)p.q + (int64_t)(s.q0 + ta) * p.q_row + (int64_t)kv * a.group * p.q_head;
   const T* gbase = (const T*)a.grad + (int64_t)(s.q0 + ta) * a.grad_row + (int64_t)kv * a.group * a.grad_head;
-  Staged<T, DP, RT, 256, false> sq, sg;
+  Staged<E, DP, RT, 256, false> sq, sg;
   sq.init(tid, p.dim, [&](int i) { const int t = i / a.group; return t * (int)p.q_row + (i - t * a.group) * (int)p.q_head; });
   sg.init(tid, p.dim, [&](int i) { const int t = i / a.group; return t * (int)a.grad_row + (i - t * a.group) * (int)a.grad_head; });
   const int my_token = tid / a.group;
@@ -1477,28 +1574,37 @@ template <typename F> void by_dim(int dim, F f) {
   else f(std::integral_constant<int, 128>());
 }
 
+// fp32 in planes, where the registers hold three of everything: 8 x 700 rows, all visible, 6 heads, in planes and not: of 32
+// channels 40 and 60 us forward, 114 and 179 backward; of 64 channels 88 and 102, 255 and 369.  96 channels and more would want
+// over 512 registers a lane.  (Few rows, QW = 1, wait for memory and stay in fp32.)
+template <typename T, int DP> struct Held { using type = T; };
+template <> struct Held<float, 32> { using type = Planes; };
+template <> struct Held<float, 64> { using type = Planes; };
+
 template <typename T, int DP> void forward_launch(const AttnArgs& a, const Plan& n, hipStream_t s) {
   const dim3 grid = n.splits > 1 ? dim3(n.splits, a.p.kv_heads, (unsigned)n.tiles) : dim3((unsigned)whole_sets(n.tiles), a.p.kv_heads);
   if (n.few) {
     if (n.splits > 1) attention_kernel<T, DP, 1, true><<<grid, 256, 0, s>>>(a);
     else attention_kernel<T, DP, 1, false><<<grid, 256, 0, s>>>(a);
   } else {
-    if (n.splits > 1) attention_kernel<T, DP, 4, true><<<grid, 256, 0, s>>>(a);
-    else attention_kernel<T, DP, 4, false><<<grid, 256, 0, s>>>(a);
+    using E = typename Held<T, DP>::type;
+    if (n.splits > 1) attention_kernel<E, DP, 4, true><<<grid, 256, 0, s>>>(a);
+    else attention_kernel<E, DP, 4, false><<<grid, 256, 0, s>>>(a);
   }
   if (n.splits > 1) attention_join_kernel<T><<<(unsigned)((int64_t)a.p.rows_q * a.p.heads), 256, 0, s>>>(a);
 }
 
 template <typename T, int DP> void backward_launch(const AttnArgs& a, hipStream_t s) {
   const ocnn_attention_params& p = a.p;
+  using E = typename Held<T, DP>::type;
   if (p.rows_q > 0) {
     const int64_t tiles = ((int64_t)p.rows_q * a.group >> 7) + p.n_seq + 1;
-    attention_grad_q_kernel<T, DP><<<dim3((unsigned)whole_sets(tiles), p.kv_heads), 256, 0, s>>>(a);
+    attention_grad_q_kernel<E, DP><<<dim3((unsigned)whole_sets(tiles), p.kv_heads), 256, 0, s>>>(a);
   }
   if (p.rows_k > 0) {
     const int64_t near_items = whole_sets((p.rows_k >> 7) + p.n_seq + 1);
     const int64_t all = near_items + (has_far(p) ? far_items(p) * (p.sinks > 32 ? 2 : 1) : 0);
-    attention_grad_kv_kernel<T, DP><<<dim3((unsigned)all, p.kv_heads), 256, 0, s>>>(a, (int)near_items);
+    attention_grad_kv_kernel<E, DP><<<dim3((unsigned)all, p.kv_heads), 256, 0, s>>>(a, (int)near_items);
     if (has_far(p)) attention_sink_kernel<T><<<dim3(p.sinks, p.kv_heads, p.n_seq), 1024, 0, s>>>(a);
   }
 }
