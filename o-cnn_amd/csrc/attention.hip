@@ -55,6 +55,7 @@ struct AttnArgs {
   float* part_o; float* part_ml;                              // split keys: [split][row][dim], [split][row][2]
   float* sink_part;                                           // [work item][kv head][2][sinks][dim]
   int splits, fill, group;
+  int near_keys;                                              // of a workgroup of the keys' gradient: 128 or 64
   float scale2;                                               // |scale| * log2(e); a negative scale turns one operand around
 };
 
@@ -444,14 +445,14 @@ __device__ inline int window_hi(const ocnn_attention_params& p, int pos, int key
 
 // ---- forward -------------------------------------------------------------------------------------------
 // QW = 4: a workgroup takes 128 packed rows, 32 a wavefront; tiles of 64 keys go through LDS once for all
-// four.  QW = 1 (few rows a sequence): 32 packed rows, and the wavefronts take every fourth tile of 32
+// four.  QW = 2: 64 packed rows, and each half of a tile has a wavefront of its own for them; joined at the end.  QW = 1 (few rows a sequence): 32 packed rows, and the wavefronts take every fourth tile of 32
 // keys each on their own, joined at the end.  Where rows x key heads leave compute units empty, the
 // tiles are dealt out over `splits` workgroups, joined by attention_join_kernel.
 template <typename E, int DP, int QW> struct ForwardShape {
-  static constexpr int kKeys = QW == 4 ? 64 : 32;
+  static constexpr int kKeys = QW == 1 ? 32 : 64;
   static constexpr int kTile = kKeys * Shape<E, DP>::kPitch * Shape<E, DP>::kPlanes;
-  static constexpr int kBuffers = QW == 4 ? 2 : 4;            // double buffer, or one a wavefront
-  static constexpr size_t kJoin = QW == 4 ? 0 : 3 * (size_t)(DP / 32) * 16 * 64 * 4;
+  static constexpr int kBuffers = QW == 1 ? 4 : 2;            // double buffer, or one a wavefront
+  static constexpr size_t kJoin = (4 - QW) * (size_t)(DP / 32) * 16 * 64 * 4;
   static constexpr size_t kTiles = (size_t)kBuffers * 2 * kTile * sizeof(typename Shape<E, DP>::Lds);
   static constexpr size_t kLds = kTiles > kJoin ? kTiles : kJoin;
 };
@@ -464,7 +465,7 @@ struct Softmax { float m, l; };
 template <typename T, int DP, int QW>
 __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& s, int kv, int row, int split, int tiles, int sink_tiles,
     int t0, Softmax* st, float (&o)[(DP + 63) / 64]) {
-  constexpr int key_tile = QW == 4 ? 64 : 32, kWays = QW == 4 ? 1 : 4;
+  constexpr int key_tile = QW == 1 ? 32 : 64, kWays = QW == 1 ? 4 : 1;
   const ocnn_attention_params& p = a.p;
   const int lane = threadIdx.x & 63;
   const int token = row / a.group, head = kv * a.group + row % a.group;
@@ -536,7 +537,8 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
   const int64_t row0 = tile * kRows;
   const int rows = s.queries * a.group;
   if (tile < 0 || row0 >= rows) return;
-  const int row = (int)row0 + (QW == 4 ? wave * 32 : 0) + col;
+  const int share = wave / QW, first_row = (int)row0 + wave % QW * 32;     // of the wavefronts of the same 32 rows
+  const int row = first_row + col;
   const bool have = row < rows;
   const int token = have ? row / a.group : 0, in_group = have ? row - token * a.group : 0;
   const int head = kv * a.group + in_group;
@@ -544,14 +546,14 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
 
   if (b >= p.n_seq) {                       // rows behind the last sequence
     if (SPLIT) {
-      if (have && half == 0 && (QW == 4 || wave == 0)) {
+      if (have && half == 0 && share == 0) {
         float* ml = a.part_ml + (((int64_t)split * p.rows_q + out_at) * p.heads + head) * 2;
         ml[0] = -__builtin_inff();
         ml[1] = -1.0f;                      // (what the joining kernel knows them by)
       }
       return;
     }
-    if (a.fill && have && (QW == 4 || wave == 0)) {
+    if (a.fill && have && share == 0) {
       T* o = (T*)a.out + out_at * a.out_row + head * a.out_head;
       for (int c = half * S::kMemoryPiece; c < p.dim; c += 2 * S::kMemoryPiece) *(uintx4*)(o + c) = uintx4{0, 0, 0, 0};
       if (a.lse && half == 0) a.lse[out_at * p.heads + head] = -__builtin_inff();
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
   const int pos = token + s.shift();
   const int lo = have ? window_lo(p, pos) : 0, hi = have ? window_hi(p, pos, s.keys) : 0;
   const int sinks = have ? p.sinks : 0;
-  const int first_row = (int)row0 + (QW == 4 ? wave * 32 : 0), last_row = min(first_row + 31, rows - 1);
+  const int last_row = min(first_row + 31, rows - 1);
   int w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;            // some row sees / every row sees
   if (first_row < rows) {
     const int pa = first_row / a.group + s.shift(), pb = last_row / a.group + s.shift();
@@ -612,11 +614,11 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
   // powers without loss, so most tiles need neither a maximum nor a rescaling, and the second product does
   // not wait for a vote.  Only a weight beyond 2^100 of the base is too much: the tile says so, and the
   // workgroup takes all its tiles again, with the maximum of each (careful).
+  constexpr int N = QW == 4 ? 2 : 1;          // times 32 keys
   bool careful = QW == 1, over = false;       // (QW = 1 waits for memory: careful from the start)
   auto keys = [&](const L* kt, const L* vt, int j0, uint64_t live) {
-    constexpr int N = KT / 32;
     const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
-    const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | ((live & all) != all));
+    const bool masked = decided((j0 < all_lo) | (j0 + 32 * N > all_hi) | ((live & all) != all));
     const bool measure = careful || decided(__any(m == -__builtin_inff()));
     floatx16 x[N];
     if constexpr (N == 2) {
@@ -671,18 +673,18 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
     float sum = sums[0] + sums[1];
     if (N == 2) sum += sums[2] + sums[3];
     l += sum;
-    if (QW == 4 && __any(!(sum <= 1024.0f))) {
+    if (QW != 1 && __any(!(sum <= 1024.0f))) {
       settle();
       over = over || !(sum <= 1.2676506e30f);
       const float most = fmaxf(sum, __shfl_xor(sum, 32, 64));
       rebase(most > 1024.0f && most <= 1.2676506e30f ? m + rintf(__builtin_amdgcn_logf(most)) : m);
     }
   };
-  auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + KT > w_lo) | (j0 < p.sinks)); };
+  auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + 32 * N > w_lo) | (j0 < p.sinks)); };
   if (!have) m = 0.0f;                        // (does not ask for a maximum)
 
-  constexpr int kThreads = QW == 4 ? 256 : 64;
-  const int mine = QW == 4 ? tid : lane;
+  constexpr int kThreads = QW == 1 ? 64 : 256;
+  const int mine = QW == 1 ? lane : tid;
   Staged<E, DP, KT, kThreads, true> sk, sv;
   sk.init(mine, p.dim, [&](int r) { return r * (int)p.k_row; });
   sv.init(mine, p.dim, [&](int r) { return r * (int)p.v_row; });
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
       sv.load(vbase + (int64_t)j0 * p.v_row, mine, s.keys - j0);
     }
   };
-  if constexpr (QW == 4) {
+  if constexpr (QW != 1) {
     const int step = SPLIT ? a.splits : 1;
 #pragma unroll 1
     for (;;) {
@@ -712,8 +714,8 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
         const uint64_t live = next;
         __syncthreads();                      // (the other buffer's readers are done: they passed the last barrier)
         if (v + step < tiles) fetch(v + step);
-        const int j0 = tile_key(v);
-        if (reach(j0)) keys(kt, vt, j0, live);
+        const int part = QW == 2 ? share * 32 : 0, j0 = tile_key(v) + part;
+        if (reach(j0)) keys(kt + part * S::kPitch, vt + part * S::kPitch, j0, live >> part);
         kt = kt == (L*)lds ? (L*)lds + 2 * F::kTile : (L*)lds;
       }
       if (careful || !__syncthreads_or(over)) break;
@@ -744,33 +746,35 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
   if (!have) m = -__builtin_inff();
   l += __shfl_xor(l, 32, 64);
 
-  if constexpr (QW == 1) {                    // the wavefronts' shares, joined in the first one
+  if constexpr (QW != 4) {                    // the wavefronts' shares, joined in the first one
+    constexpr int kWays = 4 / QW;
+    const int w0 = wave % QW;
     if (half == 0) stats[wave][col] = Softmax{m, l};
     __syncthreads();
     float top = -__builtin_inff();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, stats[w][col].m);
+    for (int w = 0; w < kWays; ++w) top = fmaxf(top, stats[w0 + QW * w][col].m);
     const float base = top == -__builtin_inff() ? 0.0f : top;
     const float mine = __builtin_amdgcn_exp2f(m - base);
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) sum += stats[w][col].l * __builtin_amdgcn_exp2f(stats[w][col].m - base);
+    for (int w = 0; w < kWays; ++w) sum += stats[w0 + QW * w][col].l * __builtin_amdgcn_exp2f(stats[w0 + QW * w][col].m - base);
     float* join = (float*)lds;
 #pragma unroll
     for (int d = 0; d < S::kBlocks; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         o[d][r] *= mine;
-        if (wave) join[(((wave - 1) * S::kBlocks + d) * 16 + r) * 64 + lane] = o[d][r];
+        if (share) join[(((wave - QW) * S::kBlocks + d) * 16 + r) * 64 + lane] = o[d][r];
       }
     __syncthreads();
-    if (wave) return;
+    if (share) return;
 #pragma unroll
-    for (int w = 0; w < 3; ++w)
+    for (int w = 0; w + 1 < kWays; ++w)
 #pragma unroll
       for (int d = 0; d < S::kBlocks; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] += join[((w * S::kBlocks + d) * 16 + r) * 64 + lane];
+        for (int r = 0; r < 16; ++r) o[d][r] += join[(((w0 + QW * w) * S::kBlocks + d) * 16 + r) * 64 + lane];
     m = top;
     l = sum;
   }
@@ -942,13 +946,15 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
   }
 }
 
-template <typename E, int DP>
+template <typename E, int DP, int QW>
 __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_kernel(AttnArgs a) {
   using S = Shape<E, DP>;
   using T = typename S::Memory;
   using L = typename S::Lds;
-  constexpr int KT = 64, kTile = KT * S::kPitch * S::kPlanes, kRows = 128, kShift = 7;
+  constexpr int KT = 64, kTile = KT * S::kPitch * S::kPlanes, kRows = 32 * QW, kShift = Log2<kRows>::value;
+  constexpr int N = QW == 4 ? 2 : 1;              // times 32 keys
   __shared__ __attribute__((aligned(16))) L lds[2 * 2 * kTile];
+  __shared__ float sums[4][32];
   const ocnn_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int kv = blockIdx.y;
@@ -965,20 +971,21 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
   const int64_t row0 = tile * kRows;
   const int rows = s.queries * a.group;
   if (tile < 0 || row0 >= rows) return;
-  const int row = (int)row0 + wave * 32 + col;
+  const int share = wave / QW, first_row = (int)row0 + wave % QW * 32;     // of the wavefronts of the same 32 rows
+  const int row = first_row + col;
   const bool have = row < rows;
   const int token = have ? row / a.group : 0, in_group = have ? row - token * a.group : 0;
   const int head = kv * a.group + in_group;
   const int64_t at = (int64_t)(s.q0 + token);
   T* dq_row = (T*)a.dq + at * a.dq_row + head * a.dq_head;
   if (b >= p.n_seq) {
-    if (have)
+    if (have && share == 0)
       for (int c = half * S::kMemoryPiece; c < p.dim; c += 2 * S::kMemoryPiece) *(uintx4*)(dq_row + c) = uintx4{0, 0, 0, 0};
     return;
   }
   const int pos = token + s.shift();
   const int lo = have ? window_lo(p, pos) : 0, hi = have ? window_hi(p, pos, s.keys) : 0, sinks = have ? p.sinks : 0;
-  const int first_row = (int)row0 + wave * 32, last_row = min(first_row + 31, rows - 1);
+  const int last_row = min(first_row + 31, rows - 1);
   int w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
   if (first_row < rows) {
     const int pa = first_row / a.group + s.shift(), pb = last_row / a.group + s.shift();
@@ -1004,7 +1011,7 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
   const int64_t at_row = at * p.heads + head;
   const float lse = have ? a.lse[at_row] : -__builtin_inff();
   const float lse2 = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
-  if (have && half == 0 && !exact) a.delta[at_row] = delta;
+  if (have && half == 0 && share == 0 && !exact) a.delta[at_row] = delta;
 
   floatx16 dq[S::kBlocks];
 #pragma unroll
@@ -1017,12 +1024,13 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
   auto seen_bits = [&](int j0, uint32_t live) {
     return (live & first_bits(hi - j0) & (~first_bits(lo - j0) | first_bits(sinks - j0))) >> (4 * half);
   };
-  auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + KT > w_lo) | (j0 < p.sinks)); };
+  auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + 32 * N > w_lo) | (j0 < p.sinks)); };
   auto keys = [&](const L* kt, const L* vt, int j0, uint64_t live) {
-    const bool masked = decided((j0 < all_lo) | (j0 + KT > all_hi) | (live != ~0ull));
-    floatx16 x[2];
+    const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
+    const bool masked = decided((j0 < all_lo) | (j0 + 32 * N > all_hi) | ((live & all) != all));
+    floatx16 x[N];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < N; ++i) {
       RowFrags<E, DP> kf, vf;
       kf.load(kt + i * 32 * S::kPitch);
       vf.load(vt + i * 32 * S::kPitch);
@@ -1033,26 +1041,26 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], a.scale2, -lse2)) * (dp[r] - delta);
     }
-    ColumnFrags<E, DP> cf[2];
+    ColumnFrags<E, DP> cf[N];
     cf[0].load(kt);
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < N; ++i) {
         const uint32_t seen = seen_bits(j0 + 32 * i, (uint32_t)(live >> (32 * i)));
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[i][r] = where_seen(seen, r, x[i][r], 0u);
       }
     }
-    cf[1].load(kt + 32 * S::kPitch);
+    if constexpr (N == 2) cf[1].load(kt + 32 * S::kPitch);
     in_order();
     cf[0].template times<kFine>(dq, x[0]);
-    cf[1].template times<kFine>(dq, x[1]);
+    if constexpr (N == 2) cf[1].template times<kFine>(dq, x[1]);
   };
   // the share of these keys in rowsum(P dP)
   auto weigh = [&](const L* kt, const L* vt, int j0, uint64_t live) {
     float sum = 0.0f;
 #pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < N; ++i) {
       RowFrags<E, DP> kf, vf;
       kf.load(kt + i * 32 * S::kPitch);
       vf.load(vt + i * 32 * S::kPitch);
@@ -1090,19 +1098,40 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
       const uint64_t live = next;
       __syncthreads();
       if (v + 1 < tiles) fetch(v + 1);
-      const int j0 = tile_key(v);
-      if (reach(j0)) use(vt, j0, live);
+      const int part = QW == 2 ? share * 32 : 0, j0 = tile_key(v) + part;
+      if (reach(j0)) use(kt + part * S::kPitch, vt + part * S::kPitch, j0, live >> part);
       kt = kt == lds ? lds + 2 * kTile : lds;
     }
   };
   if constexpr (sizeof(T) == 2)
     if (exact) {
       delta = 0.0f;
-      over([&](const L* vt, int j0, uint64_t live) { delta += weigh(kt, vt, j0, live); });
+      over([&](const L* kt, const L* vt, int j0, uint64_t live) { delta += weigh(kt, vt, j0, live); });
       delta += __shfl_xor(delta, 32, 64);
-      if (have && half == 0) a.delta[at_row] = delta;
+      if constexpr (QW == 2) {
+        if (half == 0) sums[wave][col] = delta;
+        __syncthreads();
+        delta = sums[wave % QW][col] + sums[wave % QW + QW][col];
+      }
+      if (have && half == 0 && share == 0) a.delta[at_row] = delta;
     }
-  over([&](const L* vt, int j0, uint64_t live) { keys(kt, vt, j0, live); });
+  over([&](const L* kt, const L* vt, int j0, uint64_t live) { keys(kt, vt, j0, live); });
+  if constexpr (QW == 2) {                    // the second wavefront's share
+    float* join = (float*)lds;
+    __syncthreads();
+    settle();
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (share) join[((wave % QW * S::kBlocks + d) * 16 + r) * 64 + lane] = dq[d][r];
+    __syncthreads();
+    if (share) return;
+#pragma unroll
+    for (int d = 0; d < S::kBlocks; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[d][r] += join[((wave * S::kBlocks + d) * 16 + r) * 64 + lane];
+  }
   float worst = 0.0f;
 #pragma unroll
   for (int d = 0; d < S::kBlocks; ++d)
@@ -1139,14 +1168,15 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
 // ---- gradients of the keys and values --------------------------------------------------------------------
 // A workgroup owns 128 keys of a key head, 32 a wavefront, in registers; the packed rows that see them go
 // through LDS 64 at a time, so the query heads that share the key head are summed where they are
-// accumulated.  The first keys (sinks) are seen by every later row: the rows beyond the window of
+// accumulated.  Where that makes few workgroups, one owns 64 keys, and two wavefronts share the rows of 32.  The first keys (sinks) are seen by every later row: the rows beyond the window of
 // their tile ("far") are dealt out in items of kFarRows tokens to workgroups of their own, in which all four
 // wavefronts hold the same 32 sinks and share the rows (with a wavefront for every 32 keys, three of them had
 // nothing to do).  Their sums go to memory in 32 bits and are added in order by attention_sink_kernel.
 struct FarRange { int first; bool any; };        // tokens [first, queries) see the sinks only
-__device__ inline FarRange far_tokens(const ocnn_attention_params& p, const Seq& s) {
+__device__ inline FarRange far_tokens(const AttnArgs& a, const Seq& s) {
+  const ocnn_attention_params& p = a.p;
   FarRange f;
-  f.first = min(max(127 + p.left - s.shift() + 1, 0), s.queries);
+  f.first = min(max(a.near_keys - 1 + p.left - s.shift() + 1, 0), s.queries);
   f.any = p.sinks > 0 && p.left >= 0 && s.keys > 0 && f.first < s.queries;
   return f;
 }
@@ -1208,12 +1238,15 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
   const int kv = blockIdx.y;
   const bool far = (int)blockIdx.x >= near_items;
   const int sink_blocks = p.sinks > 32 ? 2 : 1;    // of 32
+  // `ways` wavefronts share the rows of 32 keys; this one's share, and its 32 keys
+  const int key_shift = a.near_keys == 64 ? 6 : 7, ways = far ? 4 : 128 >> key_shift;
+  const int share = ways == 4 ? wave : ways == 2 ? wave >> 1 : 0, key_wave = ways == 4 ? 0 : ways == 2 ? wave & 1 : wave;
   int b, j0 = 0, far_id = 0;
   int64_t item;
   if (!far) {
     const int id = item_of(blockIdx.x, near_items);
-    b = locate_packed(p.k_offsets, p.n_seq, p.rows_k, id, 7, 1);
-    item = (int64_t)id - ((clamped(p.k_offsets, b, p.rows_k) >> 7) + b);
+    b = locate_packed(p.k_offsets, p.n_seq, p.rows_k, id, key_shift, 1);
+    item = (int64_t)id - ((clamped(p.k_offsets, b, p.rows_k) >> key_shift) + b);
   } else {
     far_id = ((int)blockIdx.x - near_items) / sink_blocks;
     j0 = (((int)blockIdx.x - near_items) % sink_blocks) * 32;
@@ -1225,8 +1258,8 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
   if (item < 0) return;
   if (b >= p.n_seq) {                              // key rows behind the last sequence
     const int k_begin = clamped(p.k_offsets, b, p.rows_k);
-    const int64_t r = k_begin + item * 128 + wave * 32 + col;
-    if (r < p.rows_k)
+    const int64_t r = k_begin + item * a.near_keys + key_wave * 32 + col;
+    if (r < p.rows_k && share == 0)
       for (int c = half * S::kMemoryPiece; c < p.dim; c += 2 * S::kMemoryPiece) {
         *(uintx4*)((T*)a.dk + r * a.dk_row + kv * a.dk_head + c) = uintx4{0, 0, 0, 0};
         *(uintx4*)((T*)a.dv + r * a.dv_row + kv * a.dv_head + c) = uintx4{0, 0, 0, 0};
@@ -1234,17 +1267,17 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
     return;
   }
   const Seq s = sequence(p, b);
-  const FarRange fr = far_tokens(p, s);
+  const FarRange fr = far_tokens(a, s);
   const int shift = s.shift();
   // the tokens that see the window keys [x, y]
   auto first_token = [&](int x) { return p.right < 0 ? 0 : min(max(x - p.right - shift, 0), s.queries); };
   auto end_token = [&](int y) { return p.left < 0 ? s.queries : min(max(y + p.left + 1 - shift, 0), s.queries); };
   int ta, tb;                                      // tokens of this workgroup
   if (!far) {
-    if (item * 128 >= s.room) return;
-    j0 = (int)item * 128;
+    if (item * a.near_keys >= s.room) return;
+    j0 = (int)item * a.near_keys;
     ta = first_token(j0);
-    tb = end_token(j0 + 127);
+    tb = end_token(j0 + a.near_keys - 1);
   } else {
     if (!fr.any) return;
     ta = max((int)item * kFarRows, fr.first);
@@ -1252,7 +1285,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
     if (ta >= tb) return;
   }
   const bool sink_tile = (far || j0 == 0) && fr.any;   // its first keys' sums go to memory
-  const int jw = far ? j0 : j0 + wave * 32, j = jw + col;
+  const int jw = j0 + key_wave * 32, j = jw + col;
   bool key = j < s.keys && (!far || j < p.sinks);
   if (key && p.key_mask) key = p.key_mask[s.k0 + j] != 0;
   // this key's packed rows: [lo, hi), and what some / every key of the wavefront has
@@ -1369,7 +1402,8 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
       __syncthreads();
       if (v + 1 < tiles) fetch(v + 1);
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) half_tile(v & 1, h, v);
+      for (int h = 0; h < 2; ++h)
+        if (ways == 1 || h == share) half_tile(v & 1, h, v);
     }
   } else {
 #pragma unroll 1
@@ -1384,19 +1418,21 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
       __syncthreads();
       if (v + (wave >> 1) < tiles) half_tile(wave >> 1, wave & 1, v + (wave >> 1));
     }
-    // the four shares, added in order by the first wavefront
+  }
+  if (ways > 1) {
+    // the shares, added in order by the wavefronts of the first
     float* join = (float*)lds;
+    const int per = 4 / ways;
     auto add_up = [&](floatx16 (&x)[S::kBlocks]) {
       __syncthreads();
-      if (wave)
+      if (share)
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) join[(((wave - 1) * S::kBlocks + d) * 16 + r) * 64 + lane] = x[d][r];
+          for (int r = 0; r < 16; ++r) join[(((wave - per) * S::kBlocks + d) * 16 + r) * 64 + lane] = x[d][r];
       __syncthreads();
-      if (!wave)
-#pragma unroll
-        for (int w = 0; w < 3; ++w)
+      if (!share)
+        for (int w = wave; w < 4 - per; w += per)
 #pragma unroll
           for (int d = 0; d < S::kBlocks; ++d)
 #pragma unroll
@@ -1405,7 +1441,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
     settle();
     add_up(dk);
     add_up(dv);
-    if (wave) return;
+    if (share) return;
   }
 
   float worst = 0.0f;
@@ -1474,7 +1510,7 @@ __global__ void __launch_bounds__(1024) attention_sink_kernel(AttnArgs a) {
   const ocnn_attention_params& p = a.p;
   const int j = blockIdx.x, kv = blockIdx.y, b = blockIdx.z;
   const Seq s = sequence(p, b);
-  const FarRange fr = far_tokens(p, s);
+  const FarRange fr = far_tokens(a, s);
   if (!fr.any || j >= s.keys) return;
   const int t = threadIdx.x & 255, share = threadIdx.x >> 8, c = t & 127, which = t >> 7;
   const int64_t one = (int64_t)p.kv_heads * 2 * p.sinks * p.dim;
@@ -1581,6 +1617,15 @@ template <typename T, int DP> struct Held { using type = T; };
 template <> struct Held<float, 32> { using type = Planes; };
 template <> struct Held<float, 64> { using type = Planes; };
 
+// 64 packed rows a workgroup instead of 128, two wavefronts on the same 32, where 128 leave a quarter of the compute units and
+// more without one (us with 64 and with 128; heads of 64 channels; forward in bf16, in fp32, queries' and keys' gradient in bf16):
+//   1 x 1000 rows, 4 heads over 2, window 200: 9.5 11.5, 18.0 23.8, 27.8 30.6      (about 32 workgroups of 128)
+//   3 x 1800 rows, 4 heads, causal: 34.6 41.5, 111 109, 86 97                      (180)
+//   9 x 800 rows, 8 heads over 4, all visible: 34.9 27.7, 137 104, 94.9 89.9       (484)
+bool half_tiles(const ocnn_attention_params& p) {
+  return ((int64_t)p.rows_q * (p.heads / p.kv_heads) / 128 + p.n_seq) * p.kv_heads <= 192;
+}
+
 template <typename T, int DP> void forward_launch(const AttnArgs& a, const Plan& n, hipStream_t s) {
   const dim3 grid = n.splits > 1 ? dim3(n.splits, a.p.kv_heads, (unsigned)n.tiles) : dim3((unsigned)whole_sets(n.tiles), a.p.kv_heads);
   if (n.few) {
@@ -1589,20 +1634,30 @@ template <typename T, int DP> void forward_launch(const AttnArgs& a, const Plan&
   } else {
     using E = typename Held<T, DP>::type;
     if (n.splits > 1) attention_kernel<E, DP, 4, true><<<grid, 256, 0, s>>>(a);
+    else if (half_tiles(a.p))
+      attention_kernel<E, DP, 2, false><<<dim3((unsigned)whole_sets(((int64_t)a.p.rows_q * a.group >> 6) + a.p.n_seq + 1), a.p.kv_heads), 256, 0, s>>>(a);
     else attention_kernel<E, DP, 4, false><<<grid, 256, 0, s>>>(a);
   }
   if (n.splits > 1) attention_join_kernel<T><<<(unsigned)((int64_t)a.p.rows_q * a.p.heads), 256, 0, s>>>(a);
 }
 
-template <typename T, int DP> void backward_launch(const AttnArgs& a, hipStream_t s) {
+template <typename T, int DP> void backward_launch(AttnArgs a, hipStream_t s) {
   const ocnn_attention_params& p = a.p;
   using E = typename Held<T, DP>::type;
   if (p.rows_q > 0) {
-    const int64_t tiles = ((int64_t)p.rows_q * a.group >> 7) + p.n_seq + 1;
-    attention_grad_q_kernel<E, DP><<<dim3((unsigned)whole_sets(tiles), p.kv_heads), 256, 0, s>>>(a);
+    const bool half = half_tiles(p);
+    const dim3 grid((unsigned)whole_sets(((int64_t)p.rows_q * a.group >> (half ? 6 : 7)) + p.n_seq + 1), p.kv_heads);
+    if (half) attention_grad_q_kernel<E, DP, 2><<<grid, 256, 0, s>>>(a);
+    else attention_grad_q_kernel<E, DP, 4><<<grid, 256, 0, s>>>(a);
   }
   if (p.rows_k > 0) {
-    const int64_t near_items = whole_sets((p.rows_k >> 7) + p.n_seq + 1);
+    // 64 keys a workgroup where 128 leave much of the chip idle: half the work each, but every row staged twice as often.
+    // 1 x 1000 rows, 4 heads over 2 of 64, window 200: 99 and 73 us (fp32); 4 x 1500 rows, 8 over 4, window 512: 81 and 71 us
+    // (bf16); 16 x 1500 rows (760 workgroups of 128 keys): 197 and 201 us; 2 x 20000 rows, 16 heads: 620 and 693 us.  Of 128
+    // channels, one workgroup a compute unit: 64 and 53, 144 and 165, 462 and 502 us.
+    const int64_t blocks = (p.rows_k / 128 + p.n_seq) * (int64_t)p.kv_heads;
+    a.near_keys = blocks <= 160 * grad_kv_waves<E>(DP) ? 64 : 128;
+    const int64_t near_items = whole_sets((p.rows_k / a.near_keys) + p.n_seq + 1);
     const int64_t all = near_items + (has_far(p) ? far_items(p) * (p.sinks > 32 ? 2 : 1) : 0);
     attention_grad_kv_kernel<E, DP><<<dim3((unsigned)all, p.kv_heads), 256, 0, s>>>(a, (int)near_items);
     if (has_far(p)) attention_sink_kernel<T><<<dim3(p.sinks, p.kv_heads, p.n_seq), 1024, 0, s>>>(a);

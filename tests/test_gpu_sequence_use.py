@@ -7,7 +7,7 @@ import torch
 
 import sequence_reference as ref
 from oracle.checker import make_points_blob
-from test_gpu_sequence import TYPES, attention_inputs, ids, offs, recurrence_inputs, within
+from test_gpu_sequence import TYPES, attention_inputs, check_attention, ids, offs, recurrence_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -201,6 +201,19 @@ def test_unet_trunk_with_a_mixer(oc, tree, nempty):
   rows_mixed = S.unet_trunk_rows(tree, 6, narrow | {("mix", 4): mix}, stages=2, nempty=nempty)
   err = float((rows_mixed.float() - mixed).abs().max() / mixed.abs().max())
   assert err < 0.1, err          # (bf16 between some twenty operators, none of them checked here: that it is the same network)
+
+
+# ---- many sequences at once: the shapes that a filled chip takes --------------------------------------------
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_attention_of_many_sequences(oc, dtype, dim):
+  """as many workgroups as fill the chip, most of them of short sequences, one sequence with rows that see its sinks only"""
+  lengths = [(7 * i) % 23 for i in range(200)]
+  lengths[50], lengths[120] = 300, 150
+  q, k, v, go = attention_inputs(lengths, lengths, 4, 2, dim, dtype, 17)
+  o = offs(lengths)
+  for kw in (dict(left=40, right=0, sinks=2), dict(left=9, right=5), {}):
+    check_attention(oc, dtype, q, k, v, go, o, o, **kw)
 
 
 # ---- streams, graphs, repeats ------------------------------------------------------------------------------
