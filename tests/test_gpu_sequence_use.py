@@ -376,6 +376,36 @@ def test_cache_beyond_32_bit_offsets(oc):
   torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("reverse", [False, True])
+def test_long_chunks_of_the_recurrence(oc, dtype, reverse):
+  """2^25 elements and more go in chunks of 64 rows and past the caches; each sequence by itself goes in chunks of 16"""
+  lengths, channels = [60001, 1, 0, 63, 74000], 264
+  gate, data, state, dy, dl = (t.cuda() for t in recurrence_inputs(lengths, channels, dtype, 12))
+  o = offs(lengths).cuda()
+  h, last, carries = oc.nn.octree_recurrence(gate, data, o, state, reverse, return_carries=True)
+  grads = oc.nn.octree_recurrence_grad(dy, gate, data, o, carries, state, dl, reverse)
+  at = offs(lengths).tolist()
+  # the same sums cut elsewhere: a few hundred rows weigh in a state, 2^-24 each of a partial sum: 2^-18 of the largest at most.
+  # bf16: and a step more where that tips a rounding
+  step = 0.0 if dtype == torch.float32 else 2.0 ** -7
+
+  def near(a, b):
+    b = b.double().cpu()
+    within(a, b, 2.0 ** -18 * max(float(b.abs().max()), 1.0) + step * b.abs())
+  for i, n in enumerate(lengths):
+    if n == 0:
+      continue
+    r, own = slice(at[i], at[i + 1]), offs([n]).cuda()
+    one = oc.nn.octree_recurrence(gate[r], data[r], own, state[i:i + 1], reverse, return_carries=True)
+    near(h[r], one[0])
+    near(last[i:i + 1], one[1])
+    g = oc.nn.octree_recurrence_grad(dy[r], gate[r], data[r], own, one[2], state[i:i + 1], dl[i:i + 1], reverse)
+    near(grads[0][r], g[0])
+    near(grads[1][r], g[1])
+    near(grads[2][i:i + 1], g[2])
+
+
 def test_rotary_and_recurrence_beyond_32_bit_offsets(oc):
   rows, channels = 4400000, 512                      # 2.25e9 elements
   x = torch.zeros(rows, 8, 64, dtype=torch.bfloat16, device="cuda")
