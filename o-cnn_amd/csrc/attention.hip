@@ -1005,7 +1005,7 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
   load_row<E, DP>(go, (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
   float delta = row_dot<T, DP>((const T*)a.fwd + at * a.fwd_row + head * a.fwd_head,
       (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
-  const int sees = p.left >= 0 && p.right >= 0 ? min(p.left + p.right + 1 + p.sinks, s.keys) : s.keys;
+  const int sees = p.left >= 0 && p.right >= 0 ? (int)min((int64_t)p.left + p.right + 1 + p.sinks, (int64_t)s.keys) : s.keys;
   const bool exact = sizeof(T) == 2 && sees <= kFewKeys;
   load_row<E, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   const int64_t at_row = at * p.heads + head;
@@ -1545,8 +1545,9 @@ int check_params(const ocnn_attention_params* p) {
       "%d channels a head: multiples of 8 up to 128", p->dim);
   OCNN_REQUIRE(p->left >= -1 && p->right >= -1, OCNN_E_BADARG, "window %d, %d: -1 for no bound", p->left, p->right);
   OCNN_REQUIRE(p->sinks >= 0 && p->sinks <= kMaxSinks, OCNN_E_UNSUPPORTED, "%d sinks: at most %d", p->sinks, kMaxSinks);
-  OCNN_REQUIRE((int64_t)p->rows_q * p->heads < (1ll << 30) && p->rows_k < (1 << 30), OCNN_E_UNSUPPORTED,
-      "%d x %d query rows, %d key rows: at most 2^30", p->rows_q, p->heads, p->rows_k);
+  // (positions and rows of a tile more, plus a bound of 2^30 in front or behind, stay below 2^31)
+  OCNN_REQUIRE((int64_t)p->rows_q * p->heads <= (1ll << 30) - 1024 && p->rows_k <= (1 << 30) - 1024, OCNN_E_UNSUPPORTED,
+      "%d x %d query rows, %d key rows: at most 2^30 - 1024", p->rows_q, p->heads, p->rows_k);
   OCNN_REQUIRE(p->q_offsets && p->k_offsets && (p->rows_q == 0 || p->q) && (p->rows_k == 0 || (p->k && p->v)), OCNN_E_BADARG,
       "null pointer");
   return OCNN_OK;

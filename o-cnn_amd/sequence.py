@@ -47,6 +47,8 @@ def _rows(t, name, ndim, like=None):
 def _aligned(t):
   """rows and heads at multiples of 16 bytes and not too far apart for the kernels' offsets, copied where they are not"""
   e = 16 // t.element_size()
+  if t.size(0) == 1 or t.size(1) == 1:       # (the stride of an axis of one is anything)
+    t = t.as_strided(t.shape, [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())][:2] + [1])
   if t.stride(0) >= 1 << 22 or t.stride(1) >= 1 << 22 or t.data_ptr() % 16 or t.stride(0) % e or t.stride(1) % e or (t.size(-1) > 1 and t.stride(-1) != 1):
     t = t.contiguous()
     if t.data_ptr() % 16:
@@ -291,10 +293,15 @@ def octree_attention(q, k, v, q_offsets, k_offsets=None, k_lengths=None, left=-1
              "out must be a %s %s tensor on %s" % (tuple(q.shape), q.dtype, q.device))
     _own_rows(out, "out")
     _apart(out, (q,) + keep, "out")
-  lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+  lse = None
+  if return_lse:             # (rows of no sequence: -inf, also where those of `out` are left alone)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    if not fill:
+      lse.fill_(-math.inf)
   ws = _scratch(need, q.device)
-  _call(q.device, "ocnn_octree_attention", _ptr(out), _i64(out.stride(0)), _i64(out.stride(1)), _ptr(lse), C.byref(p),
-        int(fill), _ptr(ws), C.c_size_t(need))
+  rows, heads = (s if n > 1 else 0 for n, s in zip(out.shape[:2], out.stride()))
+  _call(q.device, "ocnn_octree_attention", _ptr(out), _i64(rows), _i64(heads), _ptr(lse), C.byref(p), int(fill), _ptr(ws),
+        C.c_size_t(need))
   return (out, lse) if return_lse else out
 
 

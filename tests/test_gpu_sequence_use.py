@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import sequence_reference as ref
+import test_gpu_sequence as S
 from oracle.checker import make_points_blob
 from test_gpu_sequence import TYPES, attention_inputs, check_attention, ids, offs, recurrence_inputs, within
 
@@ -111,7 +112,7 @@ def test_modules_on_an_octree_level(oc, tree, nempty):
     q, k = (ref.rotary(t, pos, f, [2, 2, 2], False, False)[0] for t in (q, k))
     mixed = ref.attention(q, k, v, o, o, **window)["out"].flatten(1) @ m.out.detach().double().cpu().t()
     # (the convolutions are fp32 within 1e-4 of their largest value, as everywhere; the operators are finer)
-    within(y[0, :, :, 0].t(), mixed, 3e-4 * float(mixed.abs().max()))
+    within(y.detach()[0, :, :, 0].t(), mixed, 3e-4 * float(mixed.abs().max()))
     y.square().sum().backward()
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) and float(p.grad.abs().max()) > 0 for p in m.parameters())
   for both in (False, True):
@@ -122,7 +123,7 @@ def test_modules_on_an_octree_level(oc, tree, nempty):
     cut = c // 2 if both else 0
     h = torch.cat([ref.recurrence(gate[:, :cut], value[:, :cut], o, None, True)["out"],
                    ref.recurrence(gate[:, cut:], value[:, cut:], o)["out"]], 1) @ m.out.detach().double().cpu().t()
-    within(y[0, :, :, 0].t(), h, 3e-4 * float(h.abs().max()))
+    within(y.detach()[0, :, :, 0].t(), h, 3e-4 * float(h.abs().max()))
     y.square().sum().backward()
     assert all(p.grad is not None and float(p.grad.abs().max()) > 0 for p in m.parameters())
   assert bool(torch.isfinite(x.grad).all())
@@ -188,17 +189,17 @@ def test_unet_trunk_with_a_mixer(oc, tree, nempty):
   for d in (4, 5):
     mk(("up", d), (ch[d], ch[d + 1] * 8), ch[d])
     mk(("dec", d + 1), (ch[d + 1], 2 * ch[d + 1] * 27), 2 * ch[d + 1] * 27)
-  S = oc.stacks
-  plain = S.unet_trunk(tree, 6, params, stages=2, nempty=nempty)
+  stacks = oc.stacks
+  plain = stacks.unet_trunk(tree, 6, params, stages=2, nempty=nempty)
   mix = mixer_params(64, 4, 2, torch.float32)
-  mixed = S.unet_trunk(tree, 6, params | {("mix", 4): mix}, stages=2, nempty=nempty)
+  mixed = stacks.unet_trunk(tree, 6, params | {("mix", 4): mix}, stages=2, nempty=nempty)
   assert mixed.shape == plain.shape and bool(torch.isfinite(mixed).all()) and not torch.equal(mixed, plain)
   nothing = mix | {n: tuple(torch.zeros_like(t) for t in mix[n]) for n in ("out", "scan_out")}
-  assert torch.equal(S.unet_trunk(tree, 6, params | {("mix", 4): nothing}, stages=2, nempty=nempty), plain)
+  assert torch.equal(stacks.unet_trunk(tree, 6, params | {("mix", 4): nothing}, stages=2, nempty=nempty), plain)
   narrow = {key: (w.bfloat16(), b) for key, (w, b) in params.items()}
-  rows = S.unet_trunk_rows(tree, 6, narrow, stages=2, nempty=nempty)
-  assert torch.equal(S.unet_trunk_rows(tree, 6, narrow | {("mix", 4): nothing}, stages=2, nempty=nempty), rows)
-  rows_mixed = S.unet_trunk_rows(tree, 6, narrow | {("mix", 4): mix}, stages=2, nempty=nempty)
+  rows = stacks.unet_trunk_rows(tree, 6, narrow, stages=2, nempty=nempty)
+  assert torch.equal(stacks.unet_trunk_rows(tree, 6, narrow | {("mix", 4): nothing}, stages=2, nempty=nempty), rows)
+  rows_mixed = stacks.unet_trunk_rows(tree, 6, narrow | {("mix", 4): mix}, stages=2, nempty=nempty)
   err = float((rows_mixed.float() - mixed).abs().max() / mixed.abs().max())
   assert err < 0.1, err          # (bf16 between some twenty operators, none of them checked here: that it is the same network)
 
@@ -214,6 +215,79 @@ def test_attention_of_many_sequences(oc, dtype, dim):
   o = offs(lengths)
   for kw in (dict(left=40, right=0, sinks=2), dict(left=9, right=5), {}):
     check_attention(oc, dtype, q, k, v, go, o, o, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_attention_among_many_empty_sequences(oc, dtype, monkeypatch):
+  """the cases of the few-workgroup shapes again with 330 empty sequences behind, which the rules count as work"""
+  plain = S.offs
+  monkeypatch.setattr(S, "offs", lambda lengths: plain(list(lengths) + [0] * 330))
+  for case in S.SELF:
+    S.test_attention_and_its_gradient(oc, dtype, case)
+  for bad in (float("nan"), float("inf")):
+    S.test_attention_bad_values_stay_with_the_rows_that_see_them(oc, dtype, bad)
+  S.test_attention_key_mask(oc, dtype)
+  S.test_attention_large_scores(oc, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_attention_split_keys_with_large_scores(oc, dtype):
+  """many rows whose keys are dealt out over workgroups: weights beyond the base's reach, and a bad value"""
+  lengths = [4096]
+  q, k, v, go = attention_inputs(lengths, lengths, 2, 2, 32, dtype, 23)
+  check_attention(oc, dtype, q * 40, k * 40, v, go, offs(lengths), offs(lengths), backward=False)
+  v[3000] = float("nan")
+  out = oc.nn.octree_attention(q.cuda(), k.cuda(), v.cuda(), offs(lengths).cuda(), right=0)
+  v[3000] = 0.0
+  want = ref.attention(q, k, v, offs(lengths), offs(lengths), right=0, dtype=dtype)
+  within(out[:3000], want["out"][:3000], want["out_tol"][:3000])
+  assert bool(torch.isnan(out[3000:]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("lengths", [[50, 70, 1, 0, 90], [3000, 900, 5000, 0, 1, 4000]], ids=["short", "long"])
+def test_recurrence_bad_values_stay_in_their_sequence(oc, dtype, reverse, lengths):
+  gate, data, state, dy, dl = recurrence_inputs(lengths, 20, dtype, 24)
+  o = offs(lengths)
+  a, b = int(o[1]), int(o[2])
+  bad = [x.clone() for x in (gate, data, state, dy, dl)]
+  bad[0][a + 3], bad[1][a + 5], bad[1][b - 2], bad[2][1], bad[3][a], bad[4][1] = (
+      float("nan"), float("inf"), float("nan"), float("inf"), float("nan"), float("inf"))
+
+  def run(gate, data, state, dy, dl):
+    gate, data, state, dy, dl = (x.cuda() for x in (gate, data, state, dy, dl))
+    h, last, carries = oc.nn.octree_recurrence(gate, data, o.cuda(), state, reverse, return_carries=True)
+    grads = oc.nn.octree_recurrence_grad(dy, gate, data, o.cuda(), carries, state, dl, reverse)
+    return (h, *grads[:2]), (last, grads[2])
+  rows, states = run(gate, data, state, dy, dl)
+  bad_rows, bad_states = run(*bad)
+  keep = torch.ones(rows[0].size(0), dtype=torch.bool, device="cuda")
+  keep[a:b] = False
+  assert all(torch.equal(x[keep], y[keep]) for x, y in zip(rows, bad_rows))
+  keep = torch.arange(len(lengths), device="cuda") != 1
+  assert all(torch.equal(x[keep], y[keep]) for x, y in zip(states, bad_states))
+  assert not bool(torch.isfinite(bad_rows[0][a:b]).all())
+
+
+def test_attention_axes_of_one_and_the_lse_beside_an_output(oc):
+  """axes of one with strides of their own; the lse of rows of no sequence where `out` is given"""
+  o = offs([60, 20]).cuda()
+  q, k, v, go = (t.cuda() for t in attention_inputs([60, 20], [60, 20], 1, 1, 16, torch.float32, 25))
+  want, lse = oc.nn.octree_attention(q, k, v, o, return_lse=True)
+  far = [t.as_strided(t.shape, (t.stride(0), (1 << 23) + 3, 1)) for t in (q, k, v)]
+  assert torch.equal(oc.nn.octree_attention(*far, o), want)
+  out = torch.empty_like(q).as_strided(q.shape, (q.stride(0), 7, 1))
+  assert torch.equal(oc.nn.octree_attention(*far, o, out=out), want)
+  grads = oc.nn.octree_attention_grad(go, q, k, v, want, lse, o)
+  assert all(torch.equal(a, b) for a, b in zip(oc.nn.octree_attention_grad(go, *far, want, lse, o), grads))
+  one = [t[:1].as_strided((1, 1, 16), (7, 5, 1)) for t in (q, k, v)]
+  assert torch.equal(oc.nn.octree_attention(*one, offs([1]).cuda()), v[:1])
+  rest = torch.full((90, 1, 16), 3.0, device="cuda")
+  more = [torch.cat([t, torch.full_like(t[:10], float("nan"))]) for t in (q, k, v)]
+  got, lse90 = oc.nn.octree_attention(*more, o, out=rest, return_lse=True)
+  assert torch.equal(got[:80], want) and bool((got[80:] == 3.0).all())
+  assert torch.equal(lse90[:80], lse) and bool((lse90[80:] == -float("inf")).all())
 
 
 # ---- streams, graphs, repeats ------------------------------------------------------------------------------

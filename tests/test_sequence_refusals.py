@@ -100,6 +100,7 @@ def attention_case(**change):
     (dict(sinks=65), "at most 64"),
     (dict(sinks=-1), "sinks"),
     (dict(scale=float("nan")), "scale"),
+    (dict(q=torch.zeros(6, 65, 16), k=torch.zeros(8, 1, 16), v=torch.zeros(8, 1, 16)), "65 query heads a key head"),
 ])
 def test_attention_refuses(pkg, change, message):
   with pytest.raises(pkg.nn.OcnnError, match=message):
