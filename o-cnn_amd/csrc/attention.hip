@@ -182,8 +182,12 @@ template <typename T, int DP> __device__ inline float row_dot(const T* x, const 
 
 // Keeps the compiler from moving instructions across.  It otherwise reads each fragment right in front of the
 // matrix instruction that uses it (fewer registers) and waits for LDS every time: eight times 130 cycles in
-// front of 256 cycles of products.
+// front of 256 cycles of products.  Where the fragments of a product are 64 registers and more (rows of 256 bytes), reading
+// them ahead costs spills instead, and the products are long enough: 16 x 1500 rows, window 512, 8 heads over 4 of 128, ahead
+// and not: bf16 forward 117 and 93 us, backward 461 and 451; fp32 backward 2700 and 2037; 64 channels: 56 and 55, 198 and 198.
 __device__ inline void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+template <typename E, int DP> struct Ahead { static constexpr bool value = DP * (int)sizeof(typename Elem<E>::Lds) < 256; };
 
 // The fragments of 32 rows of a tile as the left operand of tile rows . column
 template <typename E, int DP> struct RowFrags {
@@ -625,13 +629,13 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
       RowFrags<E, DP> ka, kb;
       ka.load(kt);
       kb.load(kt + 32 * S::kPitch);
-      in_order();
+      if constexpr (Ahead<E, DP>::value) in_order();
       x[0] = x[1] = zero16();
       rows_times<E, DP>(ka, q, x[0], kb, q, x[1]);
     } else {
       RowFrags<E, DP> ka;
       ka.load(kt);
-      in_order();
+      if constexpr (Ahead<E, DP>::value) in_order();
       x[0] = zero16();
       rows_times<E, DP>(ka, q, x[0]);
     }
@@ -660,7 +664,7 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
 #pragma unroll
     for (int i = 0; i < N; ++i) {             // the values of one half arrive while the other half's weights are formed
       vf[i].load(vt + i * 32 * S::kPitch);
-      in_order();
+      if constexpr (Ahead<E, DP>::value) in_order();
       if (i) vf[0].times(o, x[0]);
       sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
@@ -1034,7 +1038,7 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
       RowFrags<E, DP> kf, vf;
       kf.load(kt + i * 32 * S::kPitch);
       vf.load(vt + i * 32 * S::kPitch);
-      in_order();
+      if constexpr (Ahead<E, DP>::value) in_order();
       floatx16 dp = zero16();
       x[i] = zero16();
       rows_times<E, DP>(kf, q, x[i], vf, go, dp);
@@ -1052,7 +1056,7 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
       }
     }
     if constexpr (N == 2) cf[1].load(kt + 32 * S::kPitch);
-    in_order();
+    if constexpr (Ahead<E, DP>::value) in_order();
     cf[0].template times<kFine>(dq, x[0]);
     if constexpr (N == 2) cf[1].template times<kFine>(dq, x[1]);
   };
@@ -1334,11 +1338,11 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
       }
     }
     if constexpr (!kLate) x = ls;
-    in_order();
+    if constexpr (Ahead<E, DP>::value) in_order();
     rows_times<E, DP>(qf, k, x, gf, vv, dp);
     ColumnFrags<E, DP> gc, qc;
     gc.load(gt);
-    in_order();
+    if constexpr (Ahead<E, DP>::value) in_order();
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = __builtin_amdgcn_exp2f(kLate ? fmaf(x[r], a.scale2, ls[r]) : x[r] * a.scale2);
@@ -1353,7 +1357,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
       }
     }
     qc.load(qt);
-    in_order();
+    if constexpr (Ahead<E, DP>::value) in_order();
     gc.times(dv, x);
     qc.template times<kFine>(dk, dp);
   };
