@@ -855,7 +855,8 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
 }
 
 // o = sum_s exp(m_s - m) o_s / sum_s exp(m_s - m) l_s.  A workgroup joins one row: its 256 threads weigh the (at
-// most 256) shares, then 8 groups of 32 lanes, 4 channels each, add theirs up and are added in order.
+// most 256) shares, then 8 groups of 32 lanes, 4 channels each, add theirs up and are added in order.  Measured: 248 rows of 7
+// shares 3.9 us, 16 rows of 128 shares of 128 channels 6.2 us: latency of two dependent reads and a launch.
 constexpr int kMaxSplits = 256;
 template <typename T>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs a) {

@@ -197,7 +197,7 @@ def test_recurrence(oc, dtype, case, reverse):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_recurrence_with_long_chunks(oc, dtype):
-  """sizes that take 64 rows a chunk and several channels a thread"""
+  """sizes that take several channels a thread, and lists of chunks in two launches"""
   check_recurrence(oc, dtype, [9000, 0, 1, 7777, 300], 256, False, True)
   check_recurrence(oc, dtype, [17003], 250, True, True)
 
