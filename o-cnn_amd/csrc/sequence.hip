@@ -182,7 +182,7 @@ uint32_t reciprocal(uint32_t d) { return d <= 1 ? 0u : (uint32_t)((1ull << 32) /
 // whatever prefix its predecessors have published would not give that).
 // Threads enumerate (chunk, channels) with the channels innermost.  The state is 32 bits throughout.
 // Sequences of a few rows (a step of a running sequence) take one launch, a thread per (sequence,
-// channels) that walks the rows.
+// channels) that walks the rows; batches of sequences that are not long take one launch too (scan_block_kernel).
 //
 // The gradient, with L_t = dh_t + a_{t+1} L_{t+1} (L_end += the gradient of the last state):
 //   dx = b L,  dg = a b L (h_{t-1} - x),  d state = a_1 L_1
@@ -711,6 +711,157 @@ __global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
     for (int v = 0; v < V; ++v) a.last[(int64_t)seq * a.channels + c0 + v] = h[v];
 }
 
+// One launch for batches of short sequences: a workgroup takes CH channels of one sequence, SEGS chunks of 16 rows at a
+// time, and carries the state along.  The rows stay in registers between the run and the application, so gate and data are read
+// once.  The runs of a wavefront's chunks are scanned by shuffles, the wavefronts' through LDS.  Bound by one compute unit's
+// exponentials and narrow loads: 5.6 us for 1024 rows of 16 channels.
+constexpr int kBlockRows = 16;
+
+// (A, H) of this thread's chunk, the state S in front of the workgroup's chunks -> the state in front of this chunk; S moves on
+template <int CH, int SEGS>
+__device__ inline float scan_block_state(float A, float H, float& S, float2 (*total)[CH]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % CH;
+#pragma unroll
+  for (int d = CH; d < 64; d <<= 1) {
+    const float fa = __shfl_up(A, d, 64), fh = __shfl_up(H, d, 64);
+    if (lane >= d) { H = fmaf(A, fh, H); A *= fa; }
+  }
+  const float ea = __shfl_up(A, CH, 64), eh = __shfl_up(H, CH, 64);
+  if (lane >= 64 - CH) total[wave][c] = make_float2(A, H);
+  __syncthreads();
+  float h = S, mine = S;
+#pragma unroll
+  for (int w = 0; w < SEGS * CH / 64; ++w) {
+    const float2 t = total[w][c];
+    mine = w == wave ? h : mine;
+    h = fmaf(t.x, h, t.y);
+  }
+  S = h;
+  return lane >= CH ? fmaf(ea, mine, eh) : mine;
+}
+
+template <typename T, int CH, int SEGS>
+__global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
+  __shared__ float2 total[2][SEGS * CH / 64][CH];
+  const int seq = blockIdx.x, c = blockIdx.y * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
+  const int begin = clamped(a.offsets, seq, a.rows);
+  const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows, length = max(end - begin, 0);
+  const bool mine = c < a.channels;
+  const int cc = min(c, a.channels - 1);
+  T* out = (T*)a.out + cc;
+  if (seq >= a.n_seq) {
+    if (a.fill && mine)
+      for (int r = begin + seg; r < end; r += SEGS) out[(int64_t)r * a.out_row] = 0;
+    return;
+  }
+  const T* gate = (const T*)a.gate + cc;
+  const T* data = (const T*)a.data + cc;
+  const int64_t id0 = (int64_t)(begin / kBlockRows) + seq;
+  float S = a.state ? a.state[(int64_t)seq * a.channels + cc] : 0.0f;
+  int parity = 0;
+  for (int base = 0; base < length; base += SEGS * kBlockRows, parity ^= 1) {
+    const int first = base + seg * kBlockRows, n = min(length - first, kBlockRows);
+    auto row = [&](int j) {
+      const int t = min(first + j, length - 1);
+      return (int64_t)(a.reverse ? end - 1 - t : begin + t);
+    };
+    T g[kBlockRows], x[kBlockRows];
+#pragma unroll
+    for (int j = 0; j < kBlockRows; ++j) {
+      g[j] = gate[row(j) * a.gate_row];
+      x[j] = data[row(j) * a.data_row];
+    }
+    float p[kBlockRows], qx[kBlockRows], A = 1.0f, H = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kBlockRows; ++j) {
+      float q;
+      gates<T>(to_f32(g[j]), &p[j], &q);
+      qx[j] = q * to_f32(x[j]);
+      if (j < n) {
+        H = fmaf(p[j], H, qx[j]);
+        A *= p[j];
+      }
+    }
+    float h = scan_block_state<CH, SEGS>(A, H, S, total[parity]);
+    if (!mine || n <= 0) continue;
+    if (a.carry && first) a.carry[(id0 + first / kBlockRows) * a.channels + c] = h;
+#pragma unroll
+    for (int j = 0; j < kBlockRows; ++j)
+      if (j < n) {
+        h = fmaf(p[j], h, qx[j]);
+        out[row(j) * a.out_row] = from_f32<T>(h);
+      }
+  }
+  if (a.last && mine && seg == 0) a.last[(int64_t)seq * a.channels + c] = S;
+}
+
+// its gradient, from the last chunk to the first
+template <typename T, int CH, int SEGS>
+__global__ void __launch_bounds__(SEGS * CH) scan_block_back_kernel(ScanArgs a) {
+  __shared__ float2 total[2][SEGS * CH / 64][CH];
+  const int seq = blockIdx.x, c = blockIdx.y * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
+  const int begin = clamped(a.offsets, seq, a.rows);
+  const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows, length = max(end - begin, 0);
+  const bool mine = c < a.channels;
+  const int cc = min(c, a.channels - 1);
+  T* dgate = (T*)a.grad_gate + cc;
+  T* ddata = (T*)a.grad_data + cc;
+  if (seq >= a.n_seq) {
+    if (mine)
+      for (int r = begin + seg; r < end; r += SEGS) {
+        dgate[(int64_t)r * a.grad_gate_row] = 0;
+        ddata[(int64_t)r * a.grad_data_row] = 0;
+      }
+    return;
+  }
+  const T* gate = (const T*)a.gate + cc;
+  const T* data = (const T*)a.data + cc;
+  const T* grad = (const T*)a.grad + cc;
+  const int64_t id0 = (int64_t)(begin / kBlockRows) + seq, at_seq = (int64_t)seq * a.channels + cc;
+  float S = a.grad_last ? a.grad_last[at_seq] : 0.0f;
+  const int chunks = (length + kBlockRows - 1) / kBlockRows;
+  int parity = 0;
+  for (int base = 0; base < chunks; base += SEGS, parity ^= 1) {
+    const int index = chunks - 1 - base - seg, first = max(index, 0) * kBlockRows, n = index < 0 ? 0 : min(length - first, kBlockRows);
+    auto row = [&](int j) {
+      const int t = min(first + j, length - 1);
+      return (int64_t)(a.reverse ? end - 1 - t : begin + t);
+    };
+    T g[kBlockRows], x[kBlockRows], d[kBlockRows];
+#pragma unroll
+    for (int j = 0; j < kBlockRows; ++j) {
+      g[j] = gate[row(j) * a.gate_row];
+      x[j] = data[row(j) * a.data_row];
+      d[j] = grad[row(j) * a.grad_row];
+    }
+    float h = index > 0 ? a.carry[(id0 + index) * a.channels + cc] : a.state ? a.state[at_seq] : 0.0f;
+    float p[kBlockRows], q[kBlockRows], before[kBlockRows], A = 1.0f, M = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kBlockRows; ++j) {
+      gates<T>(to_f32(g[j]), &p[j], &q[j]);
+      before[j] = h;
+      h = fmaf(p[j], h, q[j] * to_f32(x[j]));
+    }
+#pragma unroll
+    for (int j = kBlockRows - 1; j >= 0; --j)
+      if (j < n) {
+        M = p[j] * (to_f32(d[j]) + M);
+        A *= p[j];
+      }
+    float m = scan_block_state<CH, SEGS>(A, M, S, total[parity]);
+    if (!mine) continue;
+#pragma unroll
+    for (int j = kBlockRows - 1; j >= 0; --j)
+      if (j < n) {
+        const float lam = to_f32(d[j]) + m;
+        dgate[row(j) * a.grad_gate_row] = from_f32<T>(p[j] * q[j] * lam * (before[j] - to_f32(x[j])));
+        ddata[row(j) * a.grad_data_row] = from_f32<T>(q[j] * lam);
+        m = p[j] * lam;
+      }
+  }
+  if (a.grad_state && mine && seg == 0) a.grad_state[(int64_t)seq * a.channels + c] = S;
+}
+
 // Rows of a chunk: many where that leaves enough threads for the chip (the runs and states cost 24 bytes a
 // channel and chunk, and the carry step is short), few where it does not.  The rule sees sizes that the
 // forward and the backward call share, so their chunks are the same.  Forward and backward of bf16 in us with chunks of 16, 32
@@ -722,6 +873,17 @@ int scan_shift(int64_t rows, int64_t channels) {
 
 // sequences of 16 rows and fewer on average: one launch that walks them
 bool scan_walks(int64_t rows, int64_t n_seq, bool carries) { return !carries && rows <= 16 * n_seq; }
+
+// A workgroup a sequence and 16 channels (4 where that makes few), for batches whose sequences are not long on average.  Forward
+// and backward of bf16 in us, in one launch and in chunks: 6000 x 128 in 8 sequences 7.5 10.8, 13.7 15.9; 16384 x 97 in 16: 10.9
+// 17.8, 20.2 23.4; 32768 x 64 in 32: 9.9 15.9, 20.9 25.5; 16384 x 192 in 8: 15.9 24.8, 22.4 27.4; but 32768 x 64 in 8: 26 39, 19 24,
+// and 16384 x 512 in 64 (2048 workgroups): 48 56, 35 43.  With 4 channels: 2000 x 64 in 4: 4.7 5.9 (16 channels 7.0 6.4), 12.1 14.0.
+// A batch whose rows nearly all lie in one sequence pays for it: 32768 rows of 64 channels take 182 us instead of 19, hence
+// the bound on the rows.
+bool scan_blocks(int64_t rows, int64_t channels, int64_t n_seq) {
+  return rows <= 32768 && rows <= 2048 * n_seq && n_seq * ((channels + 15) / 16) <= 512 && scan_shift(rows, channels) == 4;
+}
+bool scan_narrow(int64_t channels, int64_t n_seq) { return n_seq * channels <= 512; }
 
 int64_t scan_ids(int64_t rows, int n_seq, int shift) { return (rows >> shift) + n_seq + 1; }
 
@@ -880,8 +1042,9 @@ int ocnn_recurrence_shape(int rows, int channels, int n_seq, int carries, int64_
   const size_t lists = 2 * (size_t)(ids + ((ids + kGroup - 1) >> kGroupShift)) * channels * sizeof(float);
   OCNN_REQUIRE(ids < (1ll << 31) && (channels + 63) / 64 <= 65535, OCNN_E_UNSUPPORTED, "%d rows of %d channels", rows, channels);
   if (carry_rows) *carry_rows = ids;
-  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) ? 0 : lists;
-  if (grad_workspace_bytes) *grad_workspace_bytes = lists;
+  const bool blocks = scan_blocks(rows, channels, n_seq);
+  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) || blocks ? 0 : lists;
+  if (grad_workspace_bytes) *grad_workspace_bytes = blocks ? 0 : lists;
   return OCNN_OK;
 }
 
@@ -913,9 +1076,19 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
     OCNN_LAUNCH_OK("octree_recurrence");
     return OCNN_OK;
   }
+  a.carry = carries;
+  if (scan_blocks(rows, channels, n_seq)) {
+    auto launch = [&](auto type) {
+      using T = decltype(type);
+      if (scan_narrow(channels, n_seq)) scan_block_kernel<T, 4, 64><<<dim3(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
+      else scan_block_kernel<T, 16, 64><<<dim3(n_seq + 1, (channels + 15) / 16), 1024, 0, s>>>(a);
+    };
+    if (dtype == OCNN_F32) launch(float()); else launch(uint16_t());
+    OCNN_LAUNCH_OK("octree_recurrence");
+    return OCNN_OK;
+  }
   OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence needs %zu bytes, got %zu", need,
       workspace_bytes);
-  a.carry = carries;
   // (bf16, 256 channels, past the caches and not: 262147 rows 123.5 / 134 us, 131072 rows 67.6 / 67.4; an operator that reads
   // the result next then loses 2 to 3 us up to 65536 rows and nothing from 200000 on)
   a.past = (int64_t)rows * channels * size >= (96ll << 20);
@@ -941,8 +1114,6 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
   OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
   OCNN_REQUIRE(offsets && carries && (rows == 0 || (grad_gate && grad_data && grad_out && gate && data)), OCNN_E_BADARG,
       "null pointer");
-  OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence_grad needs %zu bytes, got %zu",
-      need, workspace_bytes);
   ScanArgs a = {};
   a.gate = gate; a.data = data; a.grad = grad_out; a.grad_gate = grad_gate; a.grad_data = grad_data;
   a.gate_row = gate_row; a.data_row = data_row; a.grad_row = grad_out_row; a.grad_gate_row = grad_gate_row;
@@ -951,6 +1122,18 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
   a.n_seq = n_seq; a.rows = rows; a.channels = channels; a.reverse = reverse != 0;
   a.carry = const_cast<float*>(carries);
   hipStream_t s = as_stream(stream);
+  if (scan_blocks(rows, channels, n_seq)) {
+    auto launch = [&](auto type) {
+      using T = decltype(type);
+      if (scan_narrow(channels, n_seq)) scan_block_back_kernel<T, 4, 64><<<dim3(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
+      else scan_block_back_kernel<T, 16, 32><<<dim3(n_seq + 1, (channels + 15) / 16), 512, 0, s>>>(a);
+    };
+    if (dtype == OCNN_F32) launch(float()); else launch(uint16_t());
+    OCNN_LAUNCH_OK("octree_recurrence_grad");
+    return OCNN_OK;
+  }
+  OCNN_REQUIRE(workspace_dev && workspace_bytes >= need, OCNN_E_WORKSPACE, "octree_recurrence_grad needs %zu bytes, got %zu",
+      need, workspace_bytes);
   const int size = dtype == OCNN_F32 ? 4 : 2, shift = scan_shift(rows, channels);
   const int64_t ids = scan_ids(rows, n_seq, shift);
   int v = scan_width(a, size, {{grad_gate, grad_gate_row}, {grad_data, grad_data_row}, {grad_out, grad_out_row},

@@ -244,9 +244,23 @@ def test_attention_split_keys_with_large_scores(oc, dtype):
   assert bool(torch.isnan(out[3000:]).all())
 
 
+@pytest.mark.parametrize("lengths, channels", [
+    ([5000], 12), ([3000, 2500], 33),                          # chunks, their list in one launch
+    ([20000], 24),                                             # chunks, their list in two launches
+    ([2000, 1, 1900, 0, 15, 17], 7),                           # a workgroup a sequence, 4 channels
+    ([1500, 0, 1, 2100, 1024, 1025] * 5, 20), ([700] * 9, 64),  # 16 channels, one and more loads of rows
+], ids=lambda x: "+".join(map(str, x[:6])) if isinstance(x, list) else str(x))
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_recurrence_in_each_of_its_shapes(oc, dtype, reverse, lengths, channels):
+  S.check_recurrence(oc, dtype, lengths, channels, reverse, True, seed=41, extra=37)
+  S.check_recurrence(oc, dtype, lengths, channels, reverse, False, seed=42)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("reverse", [False, True])
-@pytest.mark.parametrize("lengths", [[50, 70, 1, 0, 90], [3000, 900, 5000, 0, 1, 4000]], ids=["short", "long"])
+@pytest.mark.parametrize("lengths", [[50, 70, 1, 0, 90], [3000, 900, 2000, 0, 1, 2500] * 2, [3000, 900, 5000, 0, 1, 4000]],
+                         ids=["short", "many", "long"])
 def test_recurrence_bad_values_stay_in_their_sequence(oc, dtype, reverse, lengths):
   gate, data, state, dy, dl = recurrence_inputs(lengths, 20, dtype, 24)
   o = offs(lengths)

@@ -192,7 +192,7 @@ def test_c_entry_points_return_codes(pkg):
   assert L.ocnn_recurrence_shape(8, 8, 0, 0, *map(C.byref, shape)) == -1
   assert L.ocnn_recurrence_shape(1000, 8, 1, 1, *map(C.byref, shape)) == 0 and shape[0].value >= 1000 // 64
 
-  def recurrence(rows=1000, channels=8, dtype=0, data=one, offsets=one, ws=null, ws_bytes=0):
+  def recurrence(rows=5000, channels=8, dtype=0, data=one, offsets=one, ws=null, ws_bytes=0):
     return L.ocnn_octree_recurrence(one, i64(8), null, null, one, i64(8), data, i64(8), null, offsets, 1, rows, channels, 0, 0,
                                     dtype, ws, C.c_size_t(ws_bytes), null)
   assert recurrence() == -4 and recurrence(ws=one, ws_bytes=64) == -4
