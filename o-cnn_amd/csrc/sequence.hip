@@ -717,6 +717,21 @@ __global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
 // exponentials and narrow loads: 5.6 us for 1024 rows of 16 channels.
 constexpr int kBlockRows = 16;
 
+// Workgroups go round the 8 XCDs in turn: the channels of a sequence on one of them, since its lines hold those of several
+// workgroups (from 8 sequences on; fewer would leave XCDs without work).
+__device__ inline void block_item(int n, int groups, int* seq, int* group) {
+  const int id = blockIdx.x;
+  if (n < 8) {
+    *seq = id % n;
+    *group = id / n;
+  } else {
+    const int k = id >> 3;
+    *group = k % groups;
+    *seq = k / groups * 8 + (id & 7);
+  }
+}
+inline unsigned block_items(int64_t n, int64_t groups) { return (unsigned)((n < 8 ? n : (n + 7) / 8 * 8) * groups); }
+
 // (A, H) of this thread's chunk, the state S in front of the workgroup's chunks -> the state in front of this chunk; S moves on
 template <int CH, int SEGS>
 __device__ inline float scan_block_state(float A, float H, float& S, float2 (*total)[CH]) {
@@ -743,7 +758,10 @@ __device__ inline float scan_block_state(float A, float H, float& S, float2 (*to
 template <typename T, int CH, int SEGS>
 __global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
   __shared__ float2 total[2][SEGS * CH / 64][CH];
-  const int seq = blockIdx.x, c = blockIdx.y * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
+  int seq, group;
+  block_item(a.n_seq + 1, (a.channels + CH - 1) / CH, &seq, &group);
+  if (seq > a.n_seq) return;
+  const int c = group * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
   const int begin = clamped(a.offsets, seq, a.rows);
   const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows, length = max(end - begin, 0);
   const bool mine = c < a.channels;
@@ -799,7 +817,10 @@ __global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
 template <typename T, int CH, int SEGS>
 __global__ void __launch_bounds__(SEGS * CH) scan_block_back_kernel(ScanArgs a) {
   __shared__ float2 total[2][SEGS * CH / 64][CH];
-  const int seq = blockIdx.x, c = blockIdx.y * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
+  int seq, group;
+  block_item(a.n_seq + 1, (a.channels + CH - 1) / CH, &seq, &group);
+  if (seq > a.n_seq) return;
+  const int c = group * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
   const int begin = clamped(a.offsets, seq, a.rows);
   const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows, length = max(end - begin, 0);
   const bool mine = c < a.channels;
@@ -874,14 +895,16 @@ int scan_shift(int64_t rows, int64_t channels) {
 // sequences of 16 rows and fewer on average: one launch that walks them
 bool scan_walks(int64_t rows, int64_t n_seq, bool carries) { return !carries && rows <= 16 * n_seq; }
 
-// A workgroup a sequence and 16 channels (4 where that makes few), for batches whose sequences are not long on average.  Forward
-// and backward of bf16 in us, in one launch and in chunks: 6000 x 128 in 8 sequences 7.5 10.8, 13.7 15.9; 16384 x 97 in 16: 10.9
-// 17.8, 20.2 23.4; 32768 x 64 in 32: 9.9 15.9, 20.9 25.5; 16384 x 192 in 8: 15.9 24.8, 22.4 27.4; but 32768 x 64 in 8: 26 39, 19 24,
-// and 16384 x 512 in 64 (2048 workgroups): 48 56, 35 43.  With 4 channels: 2000 x 64 in 4: 4.7 5.9 (16 channels 7.0 6.4), 12.1 14.0.
+// A workgroup a sequence and 16 channels (4 where that makes few), for batches whose sequences are not long on average.  us in
+// one launch and in chunks, forward and backward of bf16, lengths between a half and three halves of what is named: 4 x 500 of
+// 64 channels 5.3 12.0, 6.1 14.0; 8 x 750 of 128: 7.6 13.6, 10.9 15.7; 16 x 1250 of 97: 12.9 20.9, 19.4 24.2; 32 x 1000 of 64: 12.7
+// 20.2, 15.9 23.6; but 8 x 4096 of 64: 26 19, 39 24, 64 x 256 of 512 (2048 workgroups): 48 35, 56 43.  Inputs not in the caches: 16 x
+// 1250 of 97: 20.6 27.2, 33.1 32.0 (the gradient waits for more loads at a time, hence its lower bound).  4 channels: 2000 x 64 in
+// 4: 4.7, 16 channels 7.0.
 // A batch whose rows nearly all lie in one sequence pays for it: 32768 rows of 64 channels take 182 us instead of 19, hence
 // the bound on the rows.
-bool scan_blocks(int64_t rows, int64_t channels, int64_t n_seq) {
-  return rows <= 32768 && rows <= 2048 * n_seq && n_seq * ((channels + 15) / 16) <= 512 && scan_shift(rows, channels) == 4;
+bool scan_blocks(int64_t rows, int64_t channels, int64_t n_seq, bool back) {
+  return rows <= 32768 && rows <= (back ? 1024 : 2048) * n_seq && n_seq * ((channels + 15) / 16) <= 512 && scan_shift(rows, channels) == 4;
 }
 bool scan_narrow(int64_t channels, int64_t n_seq) { return n_seq * channels <= 512; }
 
@@ -1042,9 +1065,8 @@ int ocnn_recurrence_shape(int rows, int channels, int n_seq, int carries, int64_
   const size_t lists = 2 * (size_t)(ids + ((ids + kGroup - 1) >> kGroupShift)) * channels * sizeof(float);
   OCNN_REQUIRE(ids < (1ll << 31) && (channels + 63) / 64 <= 65535, OCNN_E_UNSUPPORTED, "%d rows of %d channels", rows, channels);
   if (carry_rows) *carry_rows = ids;
-  const bool blocks = scan_blocks(rows, channels, n_seq);
-  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) || blocks ? 0 : lists;
-  if (grad_workspace_bytes) *grad_workspace_bytes = blocks ? 0 : lists;
+  if (workspace_bytes) *workspace_bytes = scan_walks(rows, n_seq, carries) || scan_blocks(rows, channels, n_seq, false) ? 0 : lists;
+  if (grad_workspace_bytes) *grad_workspace_bytes = scan_blocks(rows, channels, n_seq, true) ? 0 : lists;
   return OCNN_OK;
 }
 
@@ -1077,11 +1099,11 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
     return OCNN_OK;
   }
   a.carry = carries;
-  if (scan_blocks(rows, channels, n_seq)) {
+  if (scan_blocks(rows, channels, n_seq, false)) {
     auto launch = [&](auto type) {
       using T = decltype(type);
-      if (scan_narrow(channels, n_seq)) scan_block_kernel<T, 4, 64><<<dim3(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
-      else scan_block_kernel<T, 16, 64><<<dim3(n_seq + 1, (channels + 15) / 16), 1024, 0, s>>>(a);
+      if (scan_narrow(channels, n_seq)) scan_block_kernel<T, 4, 64><<<block_items(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
+      else scan_block_kernel<T, 16, 64><<<block_items(n_seq + 1, (channels + 15) / 16), 1024, 0, s>>>(a);
     };
     if (dtype == OCNN_F32) launch(float()); else launch(uint16_t());
     OCNN_LAUNCH_OK("octree_recurrence");
@@ -1122,11 +1144,11 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
   a.n_seq = n_seq; a.rows = rows; a.channels = channels; a.reverse = reverse != 0;
   a.carry = const_cast<float*>(carries);
   hipStream_t s = as_stream(stream);
-  if (scan_blocks(rows, channels, n_seq)) {
+  if (scan_blocks(rows, channels, n_seq, true)) {
     auto launch = [&](auto type) {
       using T = decltype(type);
-      if (scan_narrow(channels, n_seq)) scan_block_back_kernel<T, 4, 64><<<dim3(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
-      else scan_block_back_kernel<T, 16, 32><<<dim3(n_seq + 1, (channels + 15) / 16), 512, 0, s>>>(a);
+      if (scan_narrow(channels, n_seq)) scan_block_back_kernel<T, 4, 64><<<block_items(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
+      else scan_block_back_kernel<T, 16, 32><<<block_items(n_seq + 1, (channels + 15) / 16), 512, 0, s>>>(a);
     };
     if (dtype == OCNN_F32) launch(float()); else launch(uint16_t());
     OCNN_LAUNCH_OK("octree_recurrence_grad");
