@@ -83,8 +83,9 @@ template <typename E, int DP> struct Shape {
   static constexpr int kPlane = 64 * kPitch;            // (tiles in planes have 64 rows)
 };
 // wavefronts a SIMD that the registers leave room for
+constexpr int plain_waves(int row_bytes) { return row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1; }
 template <typename E> constexpr int forward_waves(int dp) {
-  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 128 ? 3 : dp * (int)sizeof(E) <= 256 ? 2 : 1;
+  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : plain_waves(dp * (int)sizeof(E));
 }
 template <typename E> constexpr int grad_q_waves(int dp) {
   return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 64 ? 3 : dp * (int)sizeof(E) <= 192 ? 2 : 1;
@@ -1578,6 +1579,31 @@ int check_rows(int dtype, const char* name, const void* at, int64_t row, int64_t
 struct Plan { bool few; int splits; int64_t tiles; };
 // few: 32 packed rows a workgroup, where a sequence has that many or fewer on average.  splits: the keys are
 // dealt out where the row tiles leave compute units empty, as long as a workgroup keeps some tiles.
+// Shares of the keys for few rows, from an estimate in us.  `blocks` workgroups a share take 128 keys at a time; such a step
+// takes what its products and waits take (rows of B bytes: bf16 B / 140, fp32 B / 80; measured at 128 to 512 bytes) or what
+// memory gives all workgroups that run (5 TB/s).  A load of the chip costs its steps and 2 to begin, the joining launch 3.5.  The
+// shares that fill one to four loads are tried.  In us, so and with a share for every 1024 keys: 4 x 772 keys, 2 heads of 48,
+// fp32 11.8 27.7; 1 x 4000 keys, 8 heads over 2 of 64, bf16 10.4 20.2, fp32 12.4 43.7; 8 x 15000 keys, 16 heads over 4 of 128,
+// fp32 122 147 (32 shares: 157); 32 x 600 keys, 8 heads over 2 of 64, bf16: one share 10.8, two 12.1.
+int few_splits(int64_t blocks, int64_t keys, int64_t slots, int row_bytes, bool f32) {
+  const int64_t steps = std::max<int64_t>((keys + 127) / 128, 1), most = std::min<int64_t>(steps, kMaxSplits);
+  const double floor_us = row_bytes / (f32 ? 80.0 : 140.0);
+  auto estimate = [&](int64_t n) {
+    const int64_t all = blocks * n;
+    const double step = std::max(floor_us, std::min(all, slots) * 256.0 * row_bytes / 5e6);
+    return (double)((all + slots - 1) / slots) * ((double)((steps + n - 1) / n) * step + 2.0) + (n > 1 ? 3.5 : 0.0);
+  };
+  int64_t best = 1;
+  for (int64_t k = 1; k <= 4; ++k) {
+    int64_t n = std::min(k * slots / std::max<int64_t>(blocks, 1), most);
+    if (n <= 1) continue;
+    const int64_t each = (steps + n - 1) / n;
+    if (each <= 4) n = (steps + each - 1) / each;            // (no more shares than these steps need)
+    if (n > 1 && estimate(n) < estimate(best)) best = n;
+  }
+  return (int)best;
+}
+
 Plan plan_of(const ocnn_attention_params& p) {
   Plan n;
   const int64_t group = p.heads / p.kv_heads, packed = (int64_t)p.rows_q * group;
@@ -1586,8 +1612,14 @@ Plan plan_of(const ocnn_attention_params& p) {
   int64_t keys = p.rows_k / p.n_seq;
   if (p.left >= 0 && p.right >= 0) keys = std::min<int64_t>(keys, (int64_t)p.left + p.right + p.rows_q / p.n_seq + p.sinks);
   const int64_t blocks = std::max<int64_t>((packed + (n.few ? 31 : 127)) / (n.few ? 32 : 128), n.few ? p.n_seq : 1) * p.kv_heads;
-  const int64_t most = n.few ? keys / 256 : keys / 1024;
-  n.splits = n.tiles > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(n.few ? 1024 : 512) / std::max<int64_t>(blocks, 1), most, kMaxSplits}));
+  if (n.tiles > 65535) {
+    n.splits = 1;
+  } else if (n.few) {
+    const int row_bytes = (p.dim + 31) / 32 * 32 * (p.dtype == OCNN_F32 ? 4 : 2);
+    n.splits = few_splits(blocks, keys, 256 * plain_waves(row_bytes), row_bytes, p.dtype == OCNN_F32);
+  } else {
+    n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(blocks, 1), keys / 1024, kMaxSplits}));
+  }
   return n;
 }
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
