@@ -668,7 +668,6 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
 #pragma unroll
     for (int i = 0; i < N; ++i) {             // the values of one half arrive while the other half's weights are formed
       vf[i].load(vt + i * 32 * S::kPitch);
-      if constexpr (Ahead<E, DP>::value) in_order();
       if (i) vf[0].times(o, x[0]);
       sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
