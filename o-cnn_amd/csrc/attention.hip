@@ -87,8 +87,9 @@ constexpr int plain_waves(int row_bytes) { return row_bytes <= 128 ? 3 : row_byt
 template <typename E> constexpr int forward_waves(int dp) {
   return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : plain_waves(dp * (int)sizeof(E));
 }
+// (128 channels of bf16 spill 42 registers at two a SIMD and are faster all the same: 16 x 1500 rows, backward 435 and 451 us)
 template <typename E> constexpr int grad_q_waves(int dp) {
-  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 64 ? 3 : dp * (int)sizeof(E) <= 192 ? 2 : 1;
+  return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 64 ? 3 : dp * (int)sizeof(E) <= 256 ? 2 : 1;
 }
 template <typename E> constexpr int grad_kv_waves(int dp) {
   return Elem<E>::kPlanes == 3 ? (dp <= 32 ? 2 : 1) : dp * (int)sizeof(E) <= 128 ? 2 : 1;
@@ -453,7 +454,7 @@ __device__ inline int window_hi(const ocnn_attention_params& p, int pos, int key
 // four.  QW = 2: 64 packed rows, and each half of a tile has a wavefront of its own for them; joined at the end.  QW = 1 (few rows a sequence): 32 packed rows, and the wavefronts take every fourth tile of 32
 // keys each on their own, joined at the end.  Where rows x key heads leave compute units empty, the
 // tiles are dealt out over `splits` workgroups, joined by attention_join_kernel.
-// Measured: 4 sequences of about 16384 rows, window 2047, 8 heads of 64, bf16: 171-177 us (690 TFLOP/s), bound by VALU work
+// Measured: 4 sequences of about 16384 rows, window 2047, 8 heads of 64, bf16: 168-177 us (700 TFLOP/s), bound by VALU work
 // (60 % of the SIMD cycles: a 32 x 32 tile is 16 exponentials, shifts and sums a lane against 256 cycles of products); one query
 // of 262147 keys, 16 heads over 2 of 128, bf16: 51 us, 5.2 TB/s of keys and values, and 6 us for the join.
 template <typename E, int DP, int QW> struct ForwardShape {
@@ -1043,7 +1044,6 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
       RowFrags<E, DP> kf, vf;
       kf.load(kt + i * 32 * S::kPitch);
       vf.load(vt + i * 32 * S::kPitch);
-      if constexpr (Ahead<E, DP>::value) in_order();
       floatx16 dp = zero16();
       x[i] = zero16();
       rows_times<E, DP>(kf, q, x[i], vf, go, dp);
@@ -1061,7 +1061,6 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
       }
     }
     if constexpr (N == 2) cf[1].load(kt + 32 * S::kPitch);
-    if constexpr (Ahead<E, DP>::value) in_order();
     cf[0].template times<kFine>(dq, x[0]);
     if constexpr (N == 2) cf[1].template times<kFine>(dq, x[1]);
   };
