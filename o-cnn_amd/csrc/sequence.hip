@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
 // One launch for batches of short sequences: a workgroup takes CH channels of one sequence, SEGS chunks of 16 rows at a
 // time, and carries the state along.  The rows stay in registers between the run and the application, so gate and data are read
 // once.  The runs of a wavefront's chunks are scanned by shuffles, the wavefronts' through LDS.  Bound by one compute unit's
-// exponentials and narrow loads: 5.6 us for 1024 rows of 16 channels.
+// exponentials and narrow loads: 3.5 us for 1024 rows of 8 channels.
 constexpr int kBlockRows = 16;
 
 // Workgroups go round the 8 XCDs in turn: the channels of a sequence on one of them, since its lines hold those of several
@@ -895,16 +895,16 @@ int scan_shift(int64_t rows, int64_t channels) {
 // sequences of 16 rows and fewer on average: one launch that walks them
 bool scan_walks(int64_t rows, int64_t n_seq, bool carries) { return !carries && rows <= 16 * n_seq; }
 
-// A workgroup a sequence and 16 channels (4 where that makes few), for batches whose sequences are not long on average.  us in
+// A workgroup a sequence and 8 channels (4 where that makes few), for batches whose sequences are not long on average.  us in
 // one launch and in chunks, forward and backward of bf16, lengths between a half and three halves of what is named: 4 x 500 of
-// 64 channels 5.3 12.0, 6.1 14.0; 8 x 750 of 128: 7.6 13.6, 10.9 15.7; 16 x 1250 of 97: 12.9 20.9, 19.4 24.2; 32 x 1000 of 64: 12.7
-// 20.2, 15.9 23.6; but 8 x 4096 of 64: 26 19, 39 24, 64 x 256 of 512 (2048 workgroups): 48 35, 56 43.  Inputs not in the caches: 16 x
-// 1250 of 97: 20.6 27.2, 33.1 32.0 (the gradient waits for more loads at a time, hence its lower bound).  4 channels: 2000 x 64 in
-// 4: 4.7, 16 channels 7.0.
-// A batch whose rows nearly all lie in one sequence pays for it: 32768 rows of 64 channels take 182 us instead of 19, hence
+// 64 channels 4.9 12.0, 6.1 14.0; 8 x 750 of 128: 5.7 13.6, 7.7 15.7; 16 x 1250 of 97: 10.0 21.0, 15.1 24.0; 8 x 2000 of 192: 12.9
+// 22.4, 22.6 27.5; but 8 x 4096 of 64: 22 19, 32 24, 64 x 256 of 512: 60 35, 108 43.  Inputs not in the caches: 16 x 1250 of 97:
+// 17.8 27.6, 26.1 32.1; 8 x 2000 of 192: 25.3 27.7, 38.4 33.7 (the gradient waits for more loads at a time, hence its lower bound).
+// 16 channels: 16 x 1250 of 97: 12.9 and 19.4.
+// A batch whose rows nearly all lie in one sequence pays for it: 32768 rows of 64 channels take 129 us instead of 19, hence
 // the bound on the rows.
 bool scan_blocks(int64_t rows, int64_t channels, int64_t n_seq, bool back) {
-  return rows <= 32768 && rows <= (back ? 1024 : 2048) * n_seq && n_seq * ((channels + 15) / 16) <= 512 && scan_shift(rows, channels) == 4;
+  return rows <= 32768 && rows <= (back ? 1536 : 2048) * n_seq && n_seq * ((channels + 7) / 8) <= 1024 && scan_shift(rows, channels) == 4;
 }
 bool scan_narrow(int64_t channels, int64_t n_seq) { return n_seq * channels <= 512; }
 
@@ -1103,7 +1103,7 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
     auto launch = [&](auto type) {
       using T = decltype(type);
       if (scan_narrow(channels, n_seq)) scan_block_kernel<T, 4, 64><<<block_items(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
-      else scan_block_kernel<T, 16, 64><<<block_items(n_seq + 1, (channels + 15) / 16), 1024, 0, s>>>(a);
+      else scan_block_kernel<T, 8, 64><<<block_items(n_seq + 1, (channels + 7) / 8), 512, 0, s>>>(a);
     };
     if (dtype == OCNN_F32) launch(float()); else launch(uint16_t());
     OCNN_LAUNCH_OK("octree_recurrence");
@@ -1148,7 +1148,7 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
     auto launch = [&](auto type) {
       using T = decltype(type);
       if (scan_narrow(channels, n_seq)) scan_block_back_kernel<T, 4, 64><<<block_items(n_seq + 1, (channels + 3) / 4), 256, 0, s>>>(a);
-      else scan_block_back_kernel<T, 16, 32><<<block_items(n_seq + 1, (channels + 15) / 16), 512, 0, s>>>(a);
+      else scan_block_back_kernel<T, 8, 64><<<block_items(n_seq + 1, (channels + 7) / 8), 512, 0, s>>>(a);
     };
     if (dtype == OCNN_F32) launch(float()); else launch(uint16_t());
     OCNN_LAUNCH_OK("octree_recurrence_grad");

@@ -248,7 +248,7 @@ def test_attention_split_keys_with_large_scores(oc, dtype):
     ([5000], 12), ([3000, 2500], 33),                          # chunks, their list in one launch
     ([20000], 24),                                             # chunks, their list in two launches
     ([2000, 1, 1900, 0, 15, 17], 7),                           # a workgroup a sequence, 4 channels
-    ([1500, 0, 1, 2100, 1024, 1025] * 5, 20), ([700] * 9, 64),  # 16 channels, one and more loads of rows
+    ([1500, 0, 1, 2100, 1024, 1025] * 5, 20), ([700] * 9, 64),  # 8 channels, one and more loads of rows
 ], ids=lambda x: "+".join(map(str, x[:6])) if isinstance(x, list) else str(x))
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
