@@ -313,7 +313,9 @@ def every_call(oc, dtype, seed=21):
   q1, k1, v1, _ = (t.cuda() for t in attention_inputs(few, long, 8, 2, 64, dtype, seed + 1))
   gate, data, state, dy, dl = (t.cuda() for t in recurrence_inputs([700, 3, 900], 40, dtype, seed + 2))
   step = [t.cuda() for t in recurrence_inputs([1] * 9, 40, dtype, seed + 3)]
+  gate2, data2, state2, dy2, dl2 = (t.cuda() for t in recurrence_inputs([20000], 12, dtype, seed + 4))
   o, fo, lo, ro, so = (offs(x).cuda() for x in (lengths, few, long, [700, 3, 900], [1] * 9))
+  full, short, whole = (offs(x).cuda() for x in (lengths + [0] * 330, [5000], [20000]))
   pos = torch.randint(0, 500, (q.size(0), 3), generator=torch.Generator().manual_seed(seed), dtype=torch.int32).cuda()
   f = nn.rotary_frequencies([8, 8, 8])
   w = dict(left=40, right=20, sinks=3)
@@ -321,11 +323,16 @@ def every_call(oc, dtype, seed=21):
   def run():
     out, lse = nn.octree_attention(q, k, v, o, return_lse=True, **w)
     h, last, carries = nn.octree_recurrence(gate, data, ro, state, return_carries=True)
-    return [nn.octree_rotary(q, pos, f, [8, 8, 8]), nn.octree_rotary(q, pos, f, [8, 8, 8], True, True), out, lse,
+    out2, lse2 = nn.octree_attention(q, k, v, full, return_lse=True, **w)
+    more = [out2, lse2, *nn.octree_attention_grad(go, q, k, v, out2, lse2, full, **w)]
+    for offsets, n in ((short, 5000), (whole, 20000)):
+      h2, last2, carries2 = nn.octree_recurrence(gate2[:n], data2[:n], offsets, state2, return_carries=True)
+      more += [h2, last2, *nn.octree_recurrence_grad(dy2[:n], gate2[:n], data2[:n], offsets, carries2, state2, dl2)]
+    return more + [nn.octree_rotary(q, pos, f, [8, 8, 8]), nn.octree_rotary(q, pos, f, [8, 8, 8], True, True), out, lse,
             *nn.octree_attention_grad(go, q, k, v, out, lse, o, **w), nn.octree_attention(q1, k1, v1, fo, lo, right=0),
             h, last, *nn.octree_recurrence_grad(dy, gate, data, ro, carries, state, dl),
             *nn.octree_recurrence(step[0], step[1], so, step[2])]
-  return run, [q, k, v, go, q1, k1, v1, gate, data, state, dy, dl] + step[:3]
+  return run, [q, k, v, go, q1, k1, v1, gate, data, state, dy, dl, gate2, data2, state2, dy2, dl2] + step[:3]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
