@@ -505,6 +505,13 @@ __device__ __forceinline__ void forward_row_again(const AttnArgs& a, const Seq& 
     const float shrink = exp2f(m - base), e = see ? exp2f(x - base) : 0.0f;
     l = l * shrink + wave_sum(e);
     m = top;
+    if (l != l) {                             // a NaN stays, in every channel.  (m: the joining kernel must not weigh it by zero)
+#pragma unroll
+      for (int i = 0; i < (DP + 63) / 64; ++i) o[i] = l;
+      st->m = __builtin_inff();
+      st->l = l;
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < (DP + 63) / 64; ++i) o[i] *= shrink;
     while (left) {
@@ -944,6 +951,11 @@ __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s
       ds = exp2f(fmaf(dot, p.scale < 0.0f ? -a.scale2 : a.scale2, -lse2)) * (dp - delta);
     }
     uint64_t left = __ballot(see);
+    if (__any(ds != ds)) {                    // (stays in every channel)
+#pragma unroll
+      for (int i = 0; i < (DP + 63) / 64; ++i) dq[i] = __builtin_nanf("");
+      return;
+    }
     while (left) {
       const int jj = __ffsll((unsigned long long)left) - 1;
       left &= left - 1;
@@ -1216,6 +1228,11 @@ __device__ __forceinline__ void grad_k_row_again(const AttnArgs& a, const Seq& s
       const float lse = a.lse[at * p.heads + head];
       w = exp2f(fmaf(dot, p.scale < 0.0f ? -a.scale2 : a.scale2, lse == -__builtin_inff() ? 0.0f : -lse * kLog2e));
       ds = w * (dp - a.delta[at * p.heads + head]);
+    }
+    if (__any(w != w) && __any(ds != ds)) {    // (both stay in every channel)
+#pragma unroll
+      for (int n = 0; n < (DP + 63) / 64; ++n) dk[n] = dv[n] = __builtin_nanf("");
+      return;
     }
     for (int i = 0; i < min(64, to - r0); ++i) {
       const float wi = __shfl(w, i, 64), di = __shfl(ds, i, 64);

@@ -258,6 +258,27 @@ def test_recurrence_in_each_of_its_shapes(oc, dtype, reverse, lengths, channels)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_attention_share_of_nan_keys(oc, dtype):
+  """one query whose keys are dealt out: shares in which no visible score is a number must not be lost in the join"""
+  for keys in (512, 2048, 4096):
+    q, k, v, go = (t.cuda() for t in attention_inputs([1], [keys], 1, 1, 64, dtype, 43))
+    for first in range(0, keys, 128):
+      bad = k.clone()
+      bad[first:first + 128] = float("nan")
+      out, lse = oc.nn.octree_attention(q, bad, v, offs([1]).cuda(), offs([keys]).cuda(), return_lse=True)
+      assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all()), (keys, first)
+
+
+def test_attention_of_nothing_but_nan_ends_soon(oc):
+  """a diverged model: every row is taken again, and ends at its first NaN (30000 rows; a full second pass takes seconds)"""
+  q, k, v, go = (torch.full((30000, 2, 64), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(4))
+  o = offs([30000]).cuda()
+  out, lse = oc.nn.octree_attention(q, k, v, o, return_lse=True)
+  grads = oc.nn.octree_attention_grad(go, q, k, v, out, lse, o)
+  assert all(bool(torch.isnan(t).all()) for t in (out, lse, *grads))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("lengths", [[50, 70, 1, 0, 90], [3000, 900, 2000, 0, 1, 2500] * 2, [3000, 900, 5000, 0, 1, 4000]],
                          ids=["short", "many", "long"])
