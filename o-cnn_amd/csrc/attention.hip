@@ -456,7 +456,7 @@ __device__ inline int window_hi(const ocnn_attention_params& p, int pos, int key
 // tiles are dealt out over `splits` workgroups, joined by attention_join_kernel.
 // Measured: 4 sequences of about 16384 rows, window 2047, 8 heads of 64, bf16: 168-177 us (700 TFLOP/s), bound by VALU work
 // (60 % of the SIMD cycles: a 32 x 32 tile is 16 exponentials, shifts and sums a lane against 256 cycles of products); one query
-// of 262147 keys, 16 heads over 2 of 128, bf16: 51 us, 5.2 TB/s of keys and values, and 6 us for the join.
+// of 262147 keys, 16 heads over 2 of 128, bf16: 48 us, 5.6 TB/s of keys and values, and 6 us for the join.
 template <typename E, int DP, int QW> struct ForwardShape {
   static constexpr int kKeys = QW == 1 ? 32 : 64;
   static constexpr int kTile = kKeys * Shape<E, DP>::kPitch * Shape<E, DP>::kPlanes;
