@@ -29,9 +29,9 @@ namespace {
 // and backward: 203 us rounded once, 224 us so).
 constexpr bool kFine = true;
 // dO . o with the o that was rounded to bf16 leaves dq 2.0 times as far off as its own rounding does where a row sees 2 keys,
-// 1.19 times with 9, 1.06 with 33, 1.01 with 512.  Rows of up to kFewKeys keys get rowsum(P dP) from a pass of its own.
+// 1.19 times with 9, 1.06 with 33, 1.01 with 512.  Rows that see up to kFewKeys keys -- the first of a causal sequence, those
+// between masked keys -- get rowsum(P dP) from a pass of its own over the tiles of their workgroup.
 constexpr int kFewKeys = 32;
-
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -1027,13 +1027,10 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
   load_row<E, DP>(go, (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
   float delta = row_dot<T, DP>((const T*)a.fwd + at * a.fwd_row + head * a.fwd_head,
       (const T*)a.grad + at * a.grad_row + head * a.grad_head, have, p.dim);
-  const int sees = p.left >= 0 && p.right >= 0 ? (int)min((int64_t)p.left + p.right + 1 + p.sinks, (int64_t)s.keys) : s.keys;
-  const bool exact = sizeof(T) == 2 && sees <= kFewKeys;
   load_row<E, DP>(q, (const T*)p.q + at * p.q_row + head * p.q_head, have, p.dim, p.scale < 0.0f);
   const int64_t at_row = at * p.heads + head;
   const float lse = have ? a.lse[at_row] : -__builtin_inff();
   const float lse2 = lse == -__builtin_inff() ? 0.0f : lse * kLog2e;
-  if (have && half == 0 && share == 0 && !exact) a.delta[at_row] = delta;
 
   floatx16 dq[S::kBlocks];
 #pragma unroll
@@ -1042,10 +1039,9 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
   const T* vbase = (const T*)p.v + (int64_t)s.k0 * p.v_row + kv * p.v_head;
   const unsigned char* mask = p.key_mask ? p.key_mask + s.k0 : nullptr;
 
-  // the keys j0 .. j0 + 31 that this lane's row sees, as bits for where_seen
-  auto seen_bits = [&](int j0, uint32_t live) {
-    return (live & first_bits(hi - j0) & (~first_bits(lo - j0) | first_bits(sinks - j0))) >> (4 * half);
-  };
+  // the keys j0 .. j0 + 31 that this lane's row sees, and as bits for where_seen
+  auto visible_bits = [&](int j0, uint32_t live) { return live & first_bits(hi - j0) & (~first_bits(lo - j0) | first_bits(sinks - j0)); };
+  auto seen_bits = [&](int j0, uint32_t live) { return visible_bits(j0, live) >> (4 * half); };
   auto reach = [&](int j0) { return (j0 < w_hi) & ((j0 + 32 * N > w_lo) | (j0 < p.sinks)); };
   auto keys = [&](const L* kt, const L* vt, int j0, uint64_t live) {
     const uint64_t all = N == 2 ? ~0ull : 0xffffffffull;
@@ -1123,18 +1119,30 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
       kt = kt == lds ? lds + 2 * kTile : lds;
     }
   };
-  if constexpr (sizeof(T) == 2)
-    if (exact) {
-      delta = 0.0f;
-      over([&](const L* kt, const L* vt, int j0, uint64_t live) { delta += weigh(kt, vt, j0, live); });
-      delta += __shfl_xor(delta, 32, 64);
-      if constexpr (QW == 2) {
-        if (half == 0) sums[wave][col] = delta;
-        __syncthreads();
-        delta = sums[wave % QW][col] + sums[wave % QW + QW][col];
+  if constexpr (sizeof(T) == 2) {
+    int sees = max(hi - lo, 0) + min(sinks, min(lo, hi));
+    if (mask) {                               // (counted no further than it takes to know that there are more)
+      sees = 0;
+      for (int v = 0; v < tiles && __any(have && sees <= kFewKeys); ++v) {
+        const int j0 = tile_key(v);
+        const uint64_t live = live_keys<KT>(mask, j0, s.keys);
+        sees += __popc(visible_bits(j0, (uint32_t)live)) + __popc(visible_bits(j0 + 32, (uint32_t)(live >> 32)));
       }
-      if (have && half == 0 && share == 0) a.delta[at_row] = delta;
     }
+    const bool few = have && sees <= kFewKeys;
+    if (__syncthreads_or(few)) {
+      float sum = 0.0f;
+      over([&](const L* kt, const L* vt, int j0, uint64_t live) { sum += weigh(kt, vt, j0, live); });
+      sum += __shfl_xor(sum, 32, 64);
+      if constexpr (QW == 2) {
+        if (half == 0) sums[wave][col] = sum;
+        __syncthreads();
+        sum = sums[wave % QW][col] + sums[wave % QW + QW][col];
+      }
+      if (few) delta = sum;
+    }
+  }
+  if (have && half == 0 && share == 0) a.delta[at_row] = delta;
   over([&](const L* kt, const L* vt, int j0, uint64_t live) { keys(kt, vt, j0, live); });
   if constexpr (QW == 2) {                    // the second wavefront's share
     float* join = (float*)lds;
