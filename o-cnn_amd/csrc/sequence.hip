@@ -7,6 +7,8 @@
 // Tensors are row-major (a row is a node), so consecutive lanes hold consecutive channels.
 #include "sequence.h"
 
+#include <algorithm>
+
 namespace ocnn {
 namespace {
 
@@ -660,57 +662,6 @@ __global__ void __launch_bounds__(kBlock) scan_apply_back_kernel(ScanArgs a) {
     for (int v = 0; v < V; ++v) a.grad_state[at_seq + v] = m[v];
 }
 
-// One launch for sequences of a few rows: a thread walks the rows of one sequence (and, behind the last
-// sequence, zeroes the rows that belong to none).
-template <typename T, int V>
-__global__ void __launch_bounds__(64) scan_walk_kernel(ScanArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (i >= a.threads) return;
-  const int seq = (int)(i / a.groups);
-  const int c0 = (int)(i - (int64_t)seq * a.groups) * V;
-  const int begin = clamped(a.offsets, seq, a.rows);
-  const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows;
-  T* out = (T*)a.out + c0;
-  Chunk ch;
-  ch.count = max(end - begin, 0);
-  ch.first = seq < a.n_seq && a.reverse ? end - 1 : begin;
-  ch.step = seq < a.n_seq && a.reverse ? -1 : 1;
-  if (seq >= a.n_seq) {
-    if (a.fill) zero_rows<T, V>(out, a.out_row, ch);
-    return;
-  }
-  const T* gate = (const T*)a.gate + c0;
-  const T* data = (const T*)a.data + c0;
-  float h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = a.state ? a.state[(int64_t)seq * a.channels + c0 + v] : 0.0f;
-  for (int t = 0; t < ch.count; t += kScanRows) {
-    Pack<T, V> g[kScanRows], x[kScanRows];
-#pragma unroll
-    for (int j = 0; j < kScanRows; ++j) {
-      const int64_t row = ch.first + (int64_t)min(t + j, ch.count - 1) * ch.step;
-      g[j].load(gate + row * a.gate_row);
-      x[j].load(data + row * a.data_row);
-    }
-#pragma unroll
-    for (int j = 0; j < kScanRows; ++j)
-      if (t + j < ch.count) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float p, q;
-          gates<T>(to_f32(g[j].v[v]), &p, &q);
-          h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
-          x[j].v[v] = from_f32<T>(h[v]);
-        }
-        T* to = out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row;
-        if (a.past) x[j].store_past(to); else x[j].store(to);
-      }
-  }
-  if (a.last)
-#pragma unroll
-    for (int v = 0; v < V; ++v) a.last[(int64_t)seq * a.channels + c0 + v] = h[v];
-}
-
 // One launch for batches of short sequences: a workgroup takes CH channels of one sequence, SEGS chunks of 16 rows at a
 // time, and carries the state along.  The rows stay in registers between the run and the application, so gate and data are read
 // once.  The runs of a wavefront's chunks are scanned by shuffles, the wavefronts' through LDS.  Bound by one compute unit's
@@ -755,12 +706,8 @@ __device__ inline float scan_block_state(float A, float H, float& S, float2 (*to
   return lane >= CH ? fmaf(ea, mine, eh) : mine;
 }
 
-template <typename T, int CH, int SEGS>
-__global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
-  __shared__ float2 total[2][SEGS * CH / 64][CH];
-  int seq, group;
-  block_item(a.n_seq + 1, (a.channels + CH - 1) / CH, &seq, &group);
-  if (seq > a.n_seq) return;
+template <typename T, int CH, int SEGS, int ROWS>
+__device__ inline void scan_block(const ScanArgs& a, int seq, int group, float2 (*total)[SEGS * CH / 64][CH]) {
   const int c = group * CH + threadIdx.x % CH, seg = threadIdx.x / CH;
   const int begin = clamped(a.offsets, seq, a.rows);
   const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows, length = max(end - begin, 0);
@@ -774,24 +721,24 @@ __global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
   }
   const T* gate = (const T*)a.gate + cc;
   const T* data = (const T*)a.data + cc;
-  const int64_t id0 = (int64_t)(begin / kBlockRows) + seq;
+  const int64_t id0 = (int64_t)(begin / ROWS) + seq;
   float S = a.state ? a.state[(int64_t)seq * a.channels + cc] : 0.0f;
   int parity = 0;
-  for (int base = 0; base < length; base += SEGS * kBlockRows, parity ^= 1) {
-    const int first = base + seg * kBlockRows, n = min(length - first, kBlockRows);
+  for (int base = 0; base < length; base += SEGS * ROWS, parity ^= 1) {
+    const int first = base + seg * ROWS, n = min(length - first, ROWS);
     auto row = [&](int j) {
       const int t = min(first + j, length - 1);
       return (int64_t)(a.reverse ? end - 1 - t : begin + t);
     };
-    T g[kBlockRows], x[kBlockRows];
+    T g[ROWS], x[ROWS];
 #pragma unroll
-    for (int j = 0; j < kBlockRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       g[j] = gate[row(j) * a.gate_row];
       x[j] = data[row(j) * a.data_row];
     }
-    float p[kBlockRows], qx[kBlockRows], A = 1.0f, H = 0.0f;
+    float p[ROWS], qx[ROWS], A = 1.0f, H = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kBlockRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       float q;
       gates<T>(to_f32(g[j]), &p[j], &q);
       qx[j] = q * to_f32(x[j]);
@@ -802,9 +749,9 @@ __global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
     }
     float h = scan_block_state<CH, SEGS>(A, H, S, total[parity]);
     if (!mine || n <= 0) continue;
-    if (a.carry && first) a.carry[(id0 + first / kBlockRows) * a.channels + c] = h;
+    if (a.carry && first) a.carry[(id0 + first / ROWS) * a.channels + c] = h;
 #pragma unroll
-    for (int j = 0; j < kBlockRows; ++j)
+    for (int j = 0; j < ROWS; ++j)
       if (j < n) {
         h = fmaf(p[j], h, qx[j]);
         out[row(j) * a.out_row] = from_f32<T>(h);
@@ -813,7 +760,108 @@ __global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
   if (a.last && mine && seg == 0) a.last[(int64_t)seq * a.channels + c] = S;
 }
 
-// its gradient, from the last chunk to the first
+template <typename T, int CH, int SEGS>
+__global__ void __launch_bounds__(SEGS * CH) scan_block_kernel(ScanArgs a) {
+  __shared__ float2 total[2][SEGS * CH / 64][CH];
+  int seq, group;
+  block_item(a.n_seq + 1, (a.channels + CH - 1) / CH, &seq, &group);
+  if (seq > a.n_seq) return;
+  scan_block<T, CH, SEGS, kBlockRows>(a, seq, group, total);
+}
+
+// One launch for sequences of a few rows on average: a thread walks the rows of one sequence (and, behind the last
+// sequence, zeroes the rows that belong to none).  A sequence of more than kWalkRows rows among them is left to workgroups
+// of their own in the same launch, which take 4 channels of it as the kernel above does: the length of a sequence is known to
+// the device only.  Such a sequence holds a row that is a multiple of kWalkRows; a workgroup (of 4 channels) looks up who owns
+// kWalkSlots of those, and takes the long sequences whose first such row is among them.  us, bf16, 64 channels, so and with every
+// sequence walked: 3800 rows among 255 single ones 15 378; 61000 among 4095 243 16100; 4096 single rows of 256 channels 9.5 8.2.
+constexpr int kWalkRows = 64, kWalkSlots = 8, kWalkChannels = 4, kWalkSegs = kBlock / kWalkChannels;
+
+// The last entry of a rising table that is at most `row` (0 where none is).  8 neighbouring lanes have a row of their own and
+// probe 8 entries at a time.
+__device__ inline int owner_of(const int* offsets, int entries, int rows, int row) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = entries;
+  while (__any(n > 1)) {
+    const int step = (n + 7) / 8, at = (lane & 7) * step;
+    const uint64_t below = __ballot(at < n && clamped(offsets, lo + min(at, n - 1), rows) <= row);
+    const int skip = max(__popc((uint32_t)(below >> (lane & ~7)) & 0xffu) - 1, 0) * step;
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  return lo;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kBlock) scan_walk_kernel(ScanArgs a, unsigned seekers) {
+  __shared__ float2 total[2][kBlock / 64][kWalkChannels];
+  if (blockIdx.x < seekers) {                 // (first: what they find takes longest)
+    const int groups = (a.channels + kWalkChannels - 1) / kWalkChannels;
+    const int64_t items = (int64_t)((a.rows + kWalkRows * kWalkSlots - 1) / (kWalkRows * kWalkSlots)) * groups;
+    for (int64_t n = blockIdx.x; n < items; n += seekers) {
+      const int group = (int)(n % groups);
+      const int64_t row = (n / groups * kWalkSlots + ((threadIdx.x & 63) >> 3)) * kWalkRows;
+      const int owner = owner_of(a.offsets, a.n_seq + 1, a.rows, (int)min(row, (int64_t)a.rows));
+      const int begin = clamped(a.offsets, owner, a.rows), end = owner < a.n_seq ? clamped(a.offsets, owner + 1, a.rows) : a.rows;
+      uint64_t take = __ballot((threadIdx.x & 7) == 0 && row < a.rows && row >= begin && row - begin < kWalkRows && end - begin > kWalkRows);
+      while (take) {                          // (the same in every wavefront)
+        const int at = __ffsll((unsigned long long)take) - 1;
+        take &= take - 1;
+        scan_block<T, kWalkChannels, kWalkSegs, kScanRows>(a, __builtin_amdgcn_readlane(owner, at), group, total);
+        __syncthreads();
+      }
+    }
+    return;
+  }
+  const int64_t i = (int64_t)(blockIdx.x - seekers) * kBlock + threadIdx.x;
+  if (i >= a.threads) return;
+  const int seq = (int)(i / a.groups);
+  const int c0 = (int)(i - (int64_t)seq * a.groups) * V;
+  const int begin = clamped(a.offsets, seq, a.rows);
+  const int end = seq < a.n_seq ? clamped(a.offsets, seq + 1, a.rows) : a.rows;
+  T* out = (T*)a.out + c0;
+  Chunk ch;
+  ch.count = max(end - begin, 0);
+  if (ch.count > kWalkRows) return;
+  ch.first = seq < a.n_seq && a.reverse ? end - 1 : begin;
+  ch.step = seq < a.n_seq && a.reverse ? -1 : 1;
+  if (seq >= a.n_seq) {
+    if (a.fill) zero_rows<T, V>(out, a.out_row, ch);
+    return;
+  }
+  const T* gate = (const T*)a.gate + c0;
+  const T* data = (const T*)a.data + c0;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = a.state ? a.state[(int64_t)seq * a.channels + c0 + v] : 0.0f;
+  for (int t = 0; t < ch.count; t += kScanRows) {
+    Pack<T, V> g[kScanRows], x[kScanRows];
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j) {
+      const int64_t row = ch.first + (int64_t)min(t + j, ch.count - 1) * ch.step;
+      g[j].load(gate + row * a.gate_row);
+      x[j].load(data + row * a.data_row);
+    }
+#pragma unroll
+    for (int j = 0; j < kScanRows; ++j)
+      if (t + j < ch.count) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float p, q;
+          gates<T>(to_f32(g[j].v[v]), &p, &q);
+          h[v] = fmaf(p, h[v], q * to_f32(x[j].v[v]));
+          x[j].v[v] = from_f32<T>(h[v]);
+        }
+        T* to = out + (ch.first + (int64_t)(t + j) * ch.step) * a.out_row;
+        if (a.past) x[j].store_past(to); else x[j].store(to);
+      }
+  }
+  if (a.last)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.last[(int64_t)seq * a.channels + c0 + v] = h[v];
+}
+
+// The gradient of scan_block_kernel, from the last chunk to the first
 template <typename T, int CH, int SEGS>
 __global__ void __launch_bounds__(SEGS * CH) scan_block_back_kernel(ScanArgs a) {
   __shared__ float2 total[2][SEGS * CH / 64][CH];
@@ -892,7 +940,7 @@ int scan_shift(int64_t rows, int64_t channels) {
   return rows * channels >= (int64_t)1 << 25 ? 6 : 4;
 }
 
-// sequences of 16 rows and fewer on average: one launch that walks them
+// sequences of 16 rows and fewer on average: one launch that walks them, but for long ones among them
 bool scan_walks(int64_t rows, int64_t n_seq, bool carries) { return !carries && rows <= 16 * n_seq; }
 
 // A workgroup a sequence and 8 channels (4 where that makes few), for batches whose sequences are not long on average.  us in
@@ -1091,9 +1139,12 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
   a.groups = (channels + v - 1) / v;
   a.threads = ids * a.groups;
   if (walk) {
+    // (a grid has fewer than 2^24 workgroups; where there are more items, these take several)
+    const int64_t items = rows > kWalkRows ? (int64_t)blocks_for(rows, kWalkRows * kWalkSlots) * blocks_for(channels, kWalkChannels) : 0;
+    const unsigned seekers = (unsigned)std::min<int64_t>(items, 16384), blocks = seekers + blocks_for(a.threads);
     by_width(v, [&](auto w) {
-      if (dtype == OCNN_F32) scan_walk_kernel<float, w.value><<<blocks_for(a.threads, 64), 64, 0, s>>>(a);
-      else scan_walk_kernel<uint16_t, w.value><<<blocks_for(a.threads, 64), 64, 0, s>>>(a);
+      if (dtype == OCNN_F32) scan_walk_kernel<float, w.value><<<blocks, kBlock, 0, s>>>(a, seekers);
+      else scan_walk_kernel<uint16_t, w.value><<<blocks, kBlock, 0, s>>>(a, seekers);
     });
     OCNN_LAUNCH_OK("octree_recurrence");
     return OCNN_OK;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import sequence_reference as ref
-from test_gpu_sequence import BF16, attention_inputs, offs, within
+from test_gpu_sequence import BF16, attention_inputs, offs, recurrence_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,109 @@ def test_gradient_of_rows_that_see_few_keys(oc, case, empty):
   dq, dk, _ = oc.nn.octree_attention_grad(go, q, k, v, out, lse, o, **kw)
   within(dq[few.cuda()], want["dq"][few], want["dq_tol"][few], "dq")
   within(dk, want["dk"], want["dk_tol"], "dk")
+
+
+# ---- the recurrence, row by row ---------------------------------------------------------------------------
+def recurrence_bounds(gate, data, offsets, state=None, reverse=False, grad=None, grad_last=None):
+  """ref.recurrence's results and a bound for each element.
+
+  h_t is a sum of terms b_s x_s a_{s+1} .. a_t.  The kernels form a and b to the relative errors ra = 2^-22 (1 + b |g|) and
+  rb = 2^-22 (1 + a |g|) (the argument of the exponential is rounded), and multiply and add in 32 bits in whatever order the
+  chunks give.  So each factor of a term costs ra + 2^-23, and each term passes at most 48 sums of partial results beside the
+  steps of the recurrence: with H_t = a H_{t-1} + b |x| the sum of the terms' sizes,
+    E_t = a (E_{t-1} + (ra + 2^-23) H_{t-1}) + b (rb + 2^-23) |x|,  |error of h_t| <= E_t + 48 2^-23 H_t,
+  which follows the local a_t.  The gradient's sum L_t = dh_t + a_{t+1} L_{t+1} is bounded in the same way;
+    dx = b L, dg = a b L (h_{t-1} - x)
+  carry the bounds of their factors, ra + rb for a and b and 2^-22 for the products and the difference."""
+  g, x = gate.double().cpu(), data.double().cpu()
+  a, b = torch.sigmoid(g), torch.sigmoid(-g)
+  ra, rb = 2.0 ** -22 * (1 + b * g.abs()) + 2.0 ** -23, 2.0 ** -22 * (1 + a * g.abs()) + 2.0 ** -23
+  seqs, c = ref.spans(offsets), x.size(1)
+  h0 = torch.zeros(len(seqs), c, dtype=torch.float64) if state is None else state.double().cpu()
+  r = {"out": torch.zeros_like(x), "last": h0.clone()}
+  if grad is not None:
+    r |= {"dgate": torch.zeros_like(x), "ddata": torch.zeros_like(x), "dstate": torch.zeros_like(h0)}
+    grad = grad.double().cpu()
+  r |= {n + "_tol": torch.zeros_like(t) for n, t in r.items()}
+  many = 48 * 2.0 ** -23
+  for i, (begin, end) in enumerate(seqs):
+    rows = range(end - 1, begin - 1, -1) if reverse else range(begin, end)
+    h, size, e = h0[i], h0[i].abs(), torch.zeros(c, dtype=torch.float64)
+    before, slack = torch.zeros(end - begin, c, dtype=torch.float64), torch.zeros(end - begin, c, dtype=torch.float64)
+    for n, t in enumerate(rows):
+      before[n], slack[n] = h, e + many * size
+      e = a[t] * (e + ra[t] * size) + b[t] * rb[t] * x[t].abs()
+      h, size = a[t] * h + b[t] * x[t], a[t] * size + b[t] * x[t].abs()
+      r["out"][t], r["out_tol"][t] = h, e + many * size
+    r["last"][i], r["last_tol"][i] = h, e + many * size
+    if grad is None:
+      continue
+    m = torch.zeros(c, dtype=torch.float64) if grad_last is None else grad_last[i].double().cpu()
+    size, e = m.abs(), torch.zeros(c, dtype=torch.float64)
+    for n, t in reversed(list(enumerate(rows))):
+      lam, lam_size, lam_e = grad[t] + m, grad[t].abs() + size, e + 2.0 ** -23 * (grad[t].abs() + size)
+      lam_e = lam_e + many * lam_size
+      gap, gap_e = (before[n] - x[t]).abs(), slack[n] + 2.0 ** -23 * (before[n].abs() + x[t].abs())
+      r["ddata"][t], r["ddata_tol"][t] = b[t] * lam, b[t] * (lam_e + (rb[t] + 2.0 ** -22) * lam_size)
+      r["dgate"][t] = a[t] * b[t] * lam * (before[n] - x[t])
+      r["dgate_tol"][t] = a[t] * b[t] * (lam_e * (gap + gap_e) + lam.abs() * (gap_e + (ra[t] + rb[t] + 2.0 ** -22) * gap))
+      e = a[t] * (e + (ra[t] + 2.0 ** -23) * lam_size)
+      m, size = a[t] * lam, a[t] * lam_size
+    r["dstate"][i], r["dstate_tol"][i] = m, e + many * size
+  return r
+
+
+def held(got, want, name, dtype):
+  """within the bound (and the result's rounding), and the bound is one that a missing term cannot meet"""
+  tol = want[name + "_tol"] + (ref.half_step(dtype) if name not in ("last", "dstate") else 2.0 ** -24) * want[name].abs()
+  if want[name].numel():
+    assert float(tol.max()) <= 2.0 ** -7 * float(want[name].abs().max()), (name, float(tol.max()), float(want[name].abs().max()))
+  within(got, want[name], tol, name)
+
+
+SKEWED = [
+    # sequences of a few rows on average with long ones among them; channels; rows behind the last
+    ([1] * 63 + [961], 64, 0), ([1] * 255 + [3800], 97, 0), ([3800] + [1] * 255, 8, 5), ([0] * 130 + [65, 64, 63, 1000, 0, 128], 20, 0),
+    ([1] * 40, 33, 500), ([2] * 100 + [300, 0, 1, 700] + [3] * 200, 256, 65), ([5] * 3000 + [6000] + [0] * 1000, 130, 0),
+]
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("case", SKEWED, ids=lambda c: "%d-rows-in-%d-x-%d+%d" % (sum(c[0]), len(c[0]), c[1], c[2]))
+def test_recurrence_of_single_rows_and_a_long_sequence(oc, case, dtype, reverse):
+  """a step of running sequences together with a new one, without carries: one launch, which must not walk the long one"""
+  lengths, channels, extra = case
+  gate, data, state, _, _ = recurrence_inputs(lengths, channels, dtype, 61, extra)
+  o = offs(lengths)
+  want = recurrence_bounds(gate, data, o, state, reverse)
+  args = [t.cuda() for t in (gate, data, o, state)]
+  out, last = oc.nn.octree_recurrence(*args, reverse)
+  held(out, want, "out", dtype)
+  held(last, want, "last", dtype)
+  room = torch.full_like(out, 5.0)
+  again, last2 = oc.nn.octree_recurrence(*args, reverse, out=room)
+  assert torch.equal(again[:sum(lengths)], out[:sum(lengths)]) and torch.equal(last2, last)
+  assert bool((room[sum(lengths):] == 5.0).all()) and bool((out[sum(lengths):] == 0).all())
+
+
+@pytest.mark.parametrize("lengths, extra", [([1] * 255 + [3800], 0), ([1] * 2047 + [20000], 0), ([1] * 1000, 15000)],
+                         ids=["3800-among-255", "20000-among-2047", "rows-of-none"])
+def test_skewed_batches_do_not_wait_for_one_thread(oc, lengths, extra):
+  """The call that keeps carries takes forms that are bounded by the rows; the one without took 20 times as long and more, a
+  thread a channel walking the longest sequence.  (Eight times is far from both.)"""
+  gate, data, state, _, _ = (t.cuda() for t in recurrence_inputs(lengths, 64, BF16, 62, extra))
+  o = offs(lengths).cuda()
+
+  def time(carries):
+    best = float("inf")
+    for _ in range(8):
+      begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+      begin.record()
+      oc.nn.octree_recurrence(gate, data, o, state, return_carries=carries)
+      end.record()
+      torch.cuda.synchronize()
+      best = min(best, begin.elapsed_time(end))
+    return best
+  bounded = time(True)
+  assert time(False) < 8 * max(bounded, 0.02)
