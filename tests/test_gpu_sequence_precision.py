@@ -186,3 +186,31 @@ def test_skewed_batches_do_not_wait_for_one_thread(oc, lengths, extra):
     return best
   bounded = time(True)
   assert time(False) < 8 * max(bounded, 0.02)
+
+
+LONG = [
+    # lengths, channels: a workgroup a sequence; chunks whose list is scanned in one launch, in two; chunks of 64 rows
+    ([1000, 3, 0, 777], 12), ([300] * 20, 33), ([5000], 12), ([20000], 24), ([9000, 0, 1, 7777, 300], 256), ([12000, 1, 0, 8003], 1680),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("case, reverse, ends", [
+    pytest.param(c, r, e, id="%s-%d%s-%s" % ("+".join(map(str, c[0][:5])), c[1], "-reverse" if r else "", "state" if e else "zeros"))
+    for c in LONG for r in (False, True) for e in (True, False) if c[1] < 1000 or r != e])
+def test_gradient_of_the_recurrence_over_long_sequences(oc, case, dtype, reverse, ends):
+  """every result within a bound that follows the local gates: of the forward call, and of the gradient with and without a
+  state to begin with and a gradient of the last one"""
+  lengths, channels = case
+  gate, data, state, dy, dl = recurrence_inputs(lengths, channels, dtype, 63, extra=9)
+  if not ends:
+    state = dl = None
+  o = offs(lengths)
+  want = recurrence_bounds(gate, data, o, state, reverse, dy, dl)
+  gate, data, state, dy, dl, o = (None if t is None else t.cuda() for t in (gate, data, state, dy, dl, o))
+  out, last, carries = oc.nn.octree_recurrence(gate, data, o, state, reverse, return_carries=True)
+  held(out, want, "out", dtype)
+  held(last, want, "last", dtype)
+  grads = oc.nn.octree_recurrence_grad(dy, gate, data, o, carries, state, dl, reverse)
+  for name, g in zip(("dgate", "ddata", "dstate"), grads):
+    held(g, want, name, dtype)
