@@ -908,11 +908,16 @@ Tensor octree_align_grad(Tensor des_grad, Tensor idx_tensor) {
 // microseconds, and otherwise makes copies, takes a caller's output or says what is wrong.
 namespace {
 
+bool in_ints(const Tensor& t) {              // (the library's sizes are ints)
+  for (int64_t n : t.sizes())
+    if (n > INT32_MAX) return false;
+  return true;
+}
 bool ready(const Tensor& t, int64_t ndim, at::ScalarType type, const at::Device& device) {
-  return t.defined() && t.dim() == ndim && t.scalar_type() == type && t.device() == device && !(ndim && t.size(ndim - 1) > 1 && t.stride(ndim - 1) != 1);
+  return t.defined() && in_ints(t) && t.dim() == ndim && t.scalar_type() == type && t.device() == device && !(ndim && t.size(ndim - 1) > 1 && t.stride(ndim - 1) != 1);
 }
 bool feature(const Tensor& t, int64_t ndim) {
-  return t.defined() && t.is_cuda() && t.dim() == ndim && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
+  return t.defined() && in_ints(t) && t.is_cuda() && t.dim() == ndim && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
       !(t.size(ndim - 1) > 1 && t.stride(ndim - 1) != 1) && t.get_device() == c10::hip::current_device();
 }
 bool aligned_rows(const Tensor& t) {

@@ -35,6 +35,7 @@ def _require(ok, message):
 def _rows(t, name, ndim, like=None):
   """`t` with `ndim` axes, the innermost contiguous; of the type of `like` and on its device"""
   _require(torch.is_tensor(t) and t.dim() == ndim, "%s must be a tensor of %d axes" % (name, ndim))
+  _require(max(t.shape) <= 2 ** 31 - 1, "%s is %s: an axis has at most 2147483647 entries" % (name, tuple(t.shape)))   # (C ints)
   _dtype_code(t)
   if like is not None:
     _require(t.dtype == like.dtype, "%s is %s, expected %s" % (name, t.dtype, like.dtype))
@@ -60,6 +61,7 @@ def _table(t, name, dtype, like, numel=None):
   _require(torch.is_tensor(t) and t.dim() == 1 and t.dtype == dtype, "%s must be a 1-D %s tensor" % (name, dtype))
   _require(t.device == like.device, "%s is on %s, expected %s" % (name, t.device, like.device))
   _require(numel is None or t.numel() == numel, "%s has %d entries, expected %s" % (name, t.numel(), numel))
+  _require(t.numel() <= 2 ** 31 - 1, "%s has %d entries: at most 2147483647" % (name, t.numel()))
   return t.contiguous()
 
 

@@ -1,0 +1,78 @@
+"""Sizes and scales that the operators along the node order of a level cannot take: said, not cut to 32 bits.  Tensors of one
+row stand for many (stride 0), so nothing here needs memory."""
+import importlib
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def pkg():
+  pkg = importlib.import_module("o-cnn_amd")
+  pkg.lib.get()
+  return pkg
+
+
+def offs(*n):
+  return torch.tensor(n, dtype=torch.int32)
+
+
+MANY = [2 ** 31, 2 ** 32 + 4]     # (the second is 4 in 32 bits)
+
+
+def calls(pkg, rows, device="cpu"):
+  """every operator on `rows` rows"""
+  nn = pkg.nn
+  x3 = torch.zeros(1, 1, 16, device=device).expand(rows, 1, 16)
+  x2 = torch.zeros(1, 8, device=device).expand(rows, 8)
+  few = torch.zeros(4, 1, 16, device=device)
+  o, lse = offs(0, 4).to(device), torch.zeros(1, 1, device=device).expand(rows, 1)
+  pos, packed = torch.zeros(1, 1, dtype=torch.int32, device=device), torch.zeros(1, dtype=torch.int64, device=device)
+  f = torch.zeros(8, dtype=torch.float64, device=device)
+  return {
+      "rotary": lambda: nn.octree_rotary(x3, pos.expand(rows, 1), f, [8]),
+      "rotary of packed": lambda: nn.octree_rotary(x3, packed.expand(rows), f, [8]),
+      "attention": lambda: nn.octree_attention(x3, x3, x3, o),
+      "attention of queries": lambda: nn.octree_attention(x3, few, few, o, o),
+      "attention of keys": lambda: nn.octree_attention(few, x3, x3, o, o),
+      "attention gradient": lambda: nn.octree_attention_grad(x3, x3, x3, x3, x3, lse, o),
+      "recurrence": lambda: nn.octree_recurrence(x2, x2, o),
+      "recurrence gradient": lambda: nn.octree_recurrence_grad(x2, x2, x2, o, x2),
+  }
+
+
+@pytest.mark.parametrize("rows", MANY)
+@pytest.mark.parametrize("name", ["rotary", "rotary of packed", "attention", "attention of queries", "attention of keys",
+                                  "attention gradient", "recurrence", "recurrence gradient"])
+def test_rows_beyond_32_bits_are_refused(pkg, name, rows):
+  with pytest.raises(pkg.nn.OcnnError, match="2147483647"):
+    calls(pkg, rows)[name]()
+
+
+@pytest.mark.parametrize("shape", [(4, 2 ** 32 + 1, 16), (4, 1, 2 ** 32 + 16)])
+def test_other_axes_beyond_32_bits_are_refused(pkg, shape):
+  x = torch.zeros(1, 1, 1).expand(shape)
+  with pytest.raises(pkg.nn.OcnnError, match="2147483647"):
+    pkg.nn.octree_attention(x, x, x, offs(0, 4))
+
+
+def test_tables_beyond_32_bits_are_refused(pkg):
+  o = offs(0).expand(2 ** 32 + 2)
+  x = torch.zeros(4, 1, 16)
+  with pytest.raises(pkg.nn.OcnnError, match="2147483647"):
+    pkg.nn.octree_attention(x, x, x, o)
+  with pytest.raises(pkg.nn.OcnnError, match="2147483647"):
+    pkg.nn.octree_recurrence(x[:, 0], x[:, 0], o)
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bits_are_refused_on_a_gpu(oc):
+  """the compiled path, which takes tensors on a GPU as they are"""
+  for rows in MANY:
+    for name, call in calls(oc, rows, "cuda").items():
+      with pytest.raises(oc.nn.OcnnError, match="2147483647"):
+        call()
+  aten = oc.lib.aten()
+  x = torch.zeros(1, 8, device="cuda").expand(2 ** 32 + 4, 8)
+  with pytest.raises(RuntimeError, match="documented shapes"):
+    aten.octree_recurrence(x, x, offs(0, 4).cuda())
