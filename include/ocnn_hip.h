@@ -686,6 +686,7 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
  *   heads % kv_heads == 0, at most 64 to 1: query head h reads key head h / (heads / kv_heads);
  *   k_offsets: where the rows of each sequence begin in k and v; k_lengths (device, may be NULL): how many of
  *     them are keys -- a cache with room to grow; key_mask (device, may be NULL): one byte a key row;
+ *   scale: any sign; scale x log2(e) is finite in 32 bits;
  *   dim: a multiple of 8 up to 128; sinks <= 64; rows_q x heads and rows_k: at most 2^30 - 1024; every row and head begins at a multiple of 16 bytes, less than
  *     2^22 elements from the one before.
  * The gradient takes out and lse of the forward call; key rows that are no keys get zeros.  Scores, statistics

@@ -20,6 +20,7 @@
 #include "sequence.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace ocnn {
 namespace {
@@ -1580,6 +1581,7 @@ int check_params(const ocnn_attention_params* p) {
       "%d channels a head: multiples of 8 up to 128", p->dim);
   OCNN_REQUIRE(p->left >= -1 && p->right >= -1, OCNN_E_BADARG, "window %d, %d: -1 for no bound", p->left, p->right);
   OCNN_REQUIRE(p->sinks >= 0 && p->sinks <= kMaxSinks, OCNN_E_UNSUPPORTED, "%d sinks: at most %d", p->sinks, kMaxSinks);
+  OCNN_REQUIRE(std::isfinite(p->scale * kLog2e), OCNN_E_BADARG, "scale %g: scale x log2(e) must be finite in 32 bits", p->scale);
   // (positions and rows of a tile more, plus a bound of 2^30 in front or behind, stay below 2^31)
   OCNN_REQUIRE((int64_t)p->rows_q * p->heads <= (1ll << 30) - 1024 && p->rows_k <= (1 << 30) - 1024, OCNN_E_UNSUPPORTED,
       "%d x %d query rows, %d key rows: at most 2^30 - 1024", p->rows_q, p->heads, p->rows_k);

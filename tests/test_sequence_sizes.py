@@ -1,5 +1,6 @@
 """Sizes and scales that the operators along the node order of a level cannot take: said, not cut to 32 bits.  Tensors of one
 row stand for many (stride 0), so nothing here needs memory."""
+import ctypes as C
 import importlib
 
 import pytest
@@ -65,6 +66,23 @@ def test_tables_beyond_32_bits_are_refused(pkg):
     pkg.nn.octree_recurrence(x[:, 0], x[:, 0], o)
 
 
+@pytest.mark.parametrize("scale", [1e300, -1e39, 3e38])
+def test_scales_beyond_32_bits_are_refused(pkg, scale):
+  """(infinite or NaN in the kernels, where every score of zero would become NaN)"""
+  x = torch.zeros(4, 1, 16)
+  with pytest.raises(pkg.nn.OcnnError, match="scale"):
+    pkg.nn.octree_attention(x, x, x, offs(0, 4), scale=scale)
+  with pytest.raises(RuntimeError, match="no CPU path"):
+    pkg.nn.octree_attention(x, x, x, offs(0, 4), scale=2e38)
+
+
+def test_c_entry_points_refuse_scales_that_are_not_finite(pkg):
+  for scale in (float("nan"), float("inf"), -float("inf")):
+    p = pkg.lib.AttentionParams(16, 16, 16, 64, 16, 32, 16, 32, 16, 16, 16, 0, 0, 1, 4, 8, 4, 2, 16, -1, -1, 0, 0, scale)
+    assert pkg.lib.get().ocnn_attention_workspace_bytes(C.byref(p), None, None) == -1
+    assert b"scale" in pkg.lib.get().ocnn_last_error()
+
+
 @pytest.mark.gpu
 def test_rows_beyond_32_bits_are_refused_on_a_gpu(oc):
   """the compiled path, which takes tensors on a GPU as they are"""
@@ -76,3 +94,12 @@ def test_rows_beyond_32_bits_are_refused_on_a_gpu(oc):
   x = torch.zeros(1, 8, device="cuda").expand(2 ** 32 + 4, 8)
   with pytest.raises(RuntimeError, match="documented shapes"):
     aten.octree_recurrence(x, x, offs(0, 4).cuda())
+
+
+@pytest.mark.gpu
+def test_scales_beyond_32_bits_are_refused_on_a_gpu(oc):
+  x, o = torch.zeros(4, 1, 16, device="cuda"), offs(0, 4).cuda()
+  for scale in (1e300, 3e38):
+    with pytest.raises(oc.nn.OcnnError, match="scale"):
+      oc.nn.octree_attention(x, x, x, o, scale=scale)
+  assert bool((oc.nn.octree_attention(x, x, x, o, scale=2e38) == 0).all())
