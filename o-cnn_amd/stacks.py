@@ -13,6 +13,8 @@ applies bias and ReLU to the accumulator before the store.
   node_mixer   attention with rotary positions and a gated recurrence along the nodes of a level,
                optional between the encoder and the decoder of unet_trunk
 """
+import functools
+
 import torch
 
 from . import nn as F
@@ -79,12 +81,19 @@ def lenet_trunk_rows(octree, depth, params, data=None, to_depth=2, constant_weig
   return F.from_rows(x, cin)
 
 
+@functools.lru_cache(maxsize=None)      # (a table stays: captured graphs may hold it)
+def _frequencies(pairs, device):
+  with torch.inference_mode(False):
+    return F.rotary_frequencies(pairs, device=device)
+
+
 def node_mixer(data, octree, depth, mix, nempty=False):
   """Mixing along the Morton order of a level, octree by octree, at inference (layers.OctreeAttention and
   layers.OctreeRecurrence train): data + out(attention(rotary(q), rotary(k), v)), and where `mix` has a "scan", that
   plus scan_out(recurrence(gate, value)).  The reference's networks stop at convolutions.
   mix: "qkv", "out" and optionally "scan", "scan_out": (w, b) of 1x1x1 convolutions; "heads", "kv_heads", "pairs"
-  (pairs of channels that turn with x, y, z), "left", "right", "sinks" as in nn.octree_attention."""
+  (pairs of channels that turn with x, y, z), "left", "right", "sinks" as in nn.octree_attention.
+  The first call for `pairs` on a GPU builds its frequencies from the host; later ones can be captured in a graph."""
   offsets = F.octree_offsets(octree, depth, nempty)
 
   def project(x, weights, to_rows=True):
@@ -99,7 +108,7 @@ def node_mixer(data, octree, depth, mix, nempty=False):
   if sum(mix["pairs"]):
     turned = joint[:, :heads + kv]
     F.octree_rotary(turned, F.octree_positions(octree, depth, nempty),
-                    F.rotary_frequencies(mix["pairs"], device=data.device), mix["pairs"], out=turned)
+                    _frequencies(tuple(mix["pairs"]), data.device), mix["pairs"], out=turned)
   mixed = F.octree_attention(joint[:, :heads], joint[:, heads:heads + kv], joint[:, heads + kv:], offsets,
                              left=mix["left"], right=mix["right"], sinks=mix["sinks"])
   data = data + project(mixed.flatten(1), mix["out"], to_rows=False)
