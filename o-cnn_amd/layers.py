@@ -250,11 +250,23 @@ class OctreeRotary(nn.Module):
     self.pairs, self.base, self.interleaved = [int(n) for n in pairs], float(base), interleaved
     self._frequencies = {}      # by device; kept out of the module's tensors: they stay 64 bits under .to(bfloat16)
 
-  def forward(self, data, positions):
+  def _table(self, device):
     from . import nn as ops
-    if data.device not in self._frequencies:
-      self._frequencies[data.device] = ops.rotary_frequencies(self.pairs, self.base, device=data.device)
-    return F.octree_rotary(data, positions, self._frequencies[data.device], self.pairs, self.interleaved)
+    if device not in self._frequencies:
+      with torch.inference_mode(False):       # (a table made there could not be saved for a backward pass later)
+        self._frequencies[device] = ops.rotary_frequencies(self.pairs, self.base, device=device)
+    return self._frequencies[device]
+
+  def _apply(self, fn, *args, **kwargs):
+    """Moving the module makes the table: building it copies from the host, which a graph cannot capture."""
+    out = super()._apply(fn, *args, **kwargs)
+    device = fn(torch.empty(0, dtype=torch.int64, device=next(iter(self._frequencies), "cpu"))).device
+    if device.type == "cuda":
+      self._table(device)
+    return out
+
+  def forward(self, data, positions):
+    return F.octree_rotary(data, positions, self._table(data.device), self.pairs, self.interleaved)
 
   def extra_repr(self):
     return 'pairs={}, base={}, interleaved={}'.format(self.pairs, self.base, self.interleaved)
