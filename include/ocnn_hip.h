@@ -690,8 +690,8 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
  *   dim: a multiple of 8 up to 128; sinks <= 64; rows_q x heads and rows_k: at most 2^30 - 1024; every row and head begins at a multiple of 16 bytes, less than
  *     2^22 elements from the one before.
  * The gradient takes out and lse of the forward call; key rows that are no keys get zeros.  Scores, statistics
- * and sums are fp32; bf16 probabilities are rounded to bf16 as operands of the second product, score gradients
- * to two bf16.  Results do not change from run to run.  Both calls need ocnn_attention_workspace_bytes bytes
+ * and sums are fp32; of bf16 calls, probabilities are rounded to bf16 once as operands of the second product of
+ * the forward call where sequences have many rows, and to two bf16 elsewhere, as are score gradients.  Results do not change from run to run.  Both calls need ocnn_attention_workspace_bytes bytes
  * (16-byte aligned; the first may need none). */
 typedef struct {
   const void *q, *k, *v;

@@ -127,6 +127,20 @@ __device__ inline uint32_t take_bf16(float& x, float& y) {
   return b;
 }
 
+// The same for weights, which are finite (a row that is not is taken again): what is left in one instruction each, x - 1 hi and
+// exact too.  (-1 and 0 in either order, from registers: as constants of a packed operand they might not be what they are here.)
+__device__ inline uint32_t take_weights(float& x, float& y) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t b = pack_bf16(x, y);
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first));
+  asm("" : "+s"(second));
+  const bf16x2 h = __builtin_bit_cast(bf16x2, b);
+  x = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), x, false);
+  y = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), y, false);
+  return b;
+}
+
 // The lane's pieces of a row (a column of a B operand), straight from memory; zeros where the row or the
 // channels do not exist.
 template <typename E, int DP>
@@ -267,7 +281,7 @@ template <typename E, int DP> struct ColumnFrags {            // (bf16 and plane
       for (int n = 0; n < kParts; ++n) {
         uintx4 b;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = take_bf16(t[2 * i], t[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) b[i] = kParts == 2 ? take_weights(t[2 * i], t[2 * i + 1]) : take_bf16(t[2 * i], t[2 * i + 1]);
         part[n] = __builtin_bit_cast(bf16x8, b);
       }
       if constexpr (S::kPlanes == 3) {
@@ -631,6 +645,11 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
   // powers without loss, so most tiles need neither a maximum nor a rescaling, and the second product does
   // not wait for a vote.  Only a weight beyond 2^100 of the base is too much: the tile says so, and the
   // workgroup takes all its tiles again, with the maximum of each (careful).
+  // Probabilities as operands: two bf16 for few rows, which wait for memory; one for tiles of them.  Off 64 bits, relative to
+  // the result (whose own rounding is 0.0016), and us, with one and with two: one query of 262147 keys 0.0021 0.0016, 64.1 62.7;
+  // 32 of 2048 keys 0.00041 0.00033, 17.1 17.7; two sequences of 8192 and 22184 rows, window 2047, 8 heads of 64: 0.0021
+  // 0.0016, but 178 229.
+  constexpr bool kFew = QW == 1;
   constexpr int N = QW == 4 ? 2 : 1;          // times 32 keys
   bool careful = QW == 1, over = false;       // (QW = 1 waits for memory: careful from the start)
   auto keys = [&](const L* kt, const L* vt, int j0, uint64_t live) {
@@ -677,7 +696,7 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
 #pragma unroll
     for (int i = 0; i < N; ++i) {             // the values of one half arrive while the other half's weights are formed
       vf[i].load(vt + i * 32 * S::kPitch);
-      if (i) vf[0].times(o, x[0]);
+      if (i) vf[0].template times<kFew>(o, x[0]);
       sums[2 * i] = sums[2 * i + 1] = 0.0f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -685,7 +704,7 @@ __global__ void __launch_bounds__(256, forward_waves<E>(DP)) attention_kernel(At
         sums[2 * i + (r & 1)] += x[i][r];
       }
     }
-    vf[N - 1].times(o, x[N - 1]);
+    vf[N - 1].template times<kFew>(o, x[N - 1]);
     float sum = sums[0] + sums[1];
     if (N == 2) sum += sums[2] + sums[3];
     l += sum;

@@ -214,3 +214,53 @@ def test_gradient_of_the_recurrence_over_long_sequences(oc, case, dtype, reverse
   grads = oc.nn.octree_recurrence_grad(dy, gate, data, o, carries, state, dl, reverse)
   for name, g in zip(("dgate", "ddata", "dstate"), grads):
     held(g, want, name, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["float32", "bfloat16"])
+def test_skewed_batches_repeat_in_graphs(oc, dtype):
+  """the launch that walks short sequences and scans long ones, captured twice, replayed with new inputs and at once"""
+  lengths = [2] * 100 + [300, 0, 1, 700] + [3] * 200
+  gate, data, state, _, _ = (t.cuda() for t in recurrence_inputs(lengths, 72, dtype, 66, 90))
+  o = offs(lengths).cuda()
+  run = lambda: oc.nn.octree_recurrence(gate, data, o, state, True)   # noqa: E731
+  run()
+  torch.cuda.synchronize()
+  graphs = []
+  for _ in range(2):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      outs = run()
+    graphs.append((g, outs))
+  side = torch.cuda.Stream()
+  for turn in range(4):
+    data.copy_(torch.randn(data.shape, generator=torch.Generator().manual_seed(turn)).to(dtype))
+    want = run()
+    torch.cuda.synchronize()
+    graphs[0][0].replay()
+    with torch.cuda.stream(side):
+      graphs[1][0].replay()
+    torch.cuda.synchronize()
+    for _, outs in graphs:
+      assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+
+
+# ---- probabilities as operands ------------------------------------------------------------------------------
+STEPS = [
+    # query lengths, key lengths, heads, kv heads, dim, window: few rows a sequence
+    ([1, 1, 1], [50, 1, 200], 8, 2, 64, dict(right=0)), ([1, 2, 0, 3], [300, 40, 9, 70], 4, 1, 128, dict(left=20, right=0, sinks=2)),
+    ([7], [600], 3, 1, 48, dict(left=30)), ([2, 1], [2000, 900], 6, 2, 24, {}), ([9, 20, 4], [9, 20, 4], 2, 2, 96, dict(right=0)),
+]
+
+
+@pytest.mark.parametrize("case", STEPS, ids=lambda c: "%s-of-%s-%dx%dx%d" % (
+    "+".join(map(str, c[0])), "+".join(map(str, c[1])), c[2], c[3], c[4]))
+def test_probabilities_of_few_rows_are_not_rounded_once(oc, case):
+  """The bound of ref.attention without the rounding of the probabilities, but for 2^-17 of each: two bf16.  (Products waiting
+  for memory, the second one costs nothing.)"""
+  qlen, klen, heads, kvh, dim, window = case
+  q, k, v, _ = attention_inputs(qlen, klen, heads, kvh, dim, BF16, 71)
+  qo, ko = offs(qlen), offs(klen)
+  want = ref.attention(q, k, v, qo, ko, **window)
+  size = ref.attention(q, k, v.abs(), qo, ko, **window)["out"]
+  out = oc.nn.octree_attention(q.cuda(), k.cuda(), v.cuda(), qo.cuda(), ko.cuda(), **window)
+  within(out, want["out"], want["out_tol"] + size * 2.0 ** -17 + ref.half_step(BF16) * want["out"].abs(), "out")
