@@ -25,9 +25,9 @@
 namespace ocnn {
 namespace {
 
-// The gradients of the scores are not rounded to bf16 once but held as two bf16 (one more product): rounded once they leave dq
-// and dk 1.42 times as far off as the rounding of dq and dk themselves does (16 x 1500 rows, window 512, 8 heads of 64, forward
-// and backward: 203 us rounded once, 224 us so).
+// Weights of the gradients -- score gradients and the probabilities of dV -- are not rounded to bf16 once but held as two bf16
+// (one more product): rounded once they leave dq, dk and dv 1.42 times as far off as the rounding of these themselves does
+// (16 x 1500 rows, window 512, 8 heads of 64, forward and backward: 203 us rounded once, 224 us the score gradients so, 237 all).
 constexpr bool kFine = true;
 // dO . o with the o that was rounded to bf16 leaves dq 2.0 times as far off as its own rounding does where a row sees 2 keys,
 // 1.19 times with 9, 1.06 with 33, 1.01 with 512.  Rows that see up to kFewKeys keys -- the first of a causal sequence, those
@@ -1409,7 +1409,7 @@ __global__ void __launch_bounds__(256, grad_kv_waves<E>(DP)) attention_grad_kv_k
     }
     qc.load(qt);
     if constexpr (Ahead<E, DP>::value) in_order();
-    gc.times(dv, x);
+    gc.template times<kFine>(dv, x);
     qc.template times<kFine>(dk, dp);
   };
 

@@ -264,3 +264,25 @@ def test_probabilities_of_few_rows_are_not_rounded_once(oc, case):
   size = ref.attention(q, k, v.abs(), qo, ko, **window)["out"]
   out = oc.nn.octree_attention(q.cuda(), k.cuda(), v.cuda(), qo.cuda(), ko.cuda(), **window)
   within(out, want["out"], want["out_tol"] + size * 2.0 ** -17 + ref.half_step(BF16) * want["out"].abs(), "out")
+
+
+@pytest.mark.parametrize("empty", [0, 330], ids=["few-workgroups", "many"])
+@pytest.mark.parametrize("lengths, heads, kvh, dim, window", [
+    ([300], 2, 1, 64, dict(right=0)), ([90, 200, 1], 4, 2, 32, dict(left=20, right=20, sinks=3)), ([140], 2, 2, 128, {}),
+    ([700], 2, 1, 96, dict(left=9, right=0, sinks=40))], ids=["300", "90+200+1", "140", "700"])
+def test_gradient_of_the_values_is_not_rounded_twice(oc, lengths, heads, kvh, dim, window, empty):
+  """dv = P^T dO with P off by 2 e_s + 2^-19 (1 + |lse|) (scores, lse, exponential) and 2^-17 (two bf16), rounded once"""
+  q, k, v, go = attention_inputs(lengths, lengths, heads, kvh, dim, BF16, 72)
+  o = offs(lengths)
+  want = ref.attention(q, k, v, o, o, grad=go, **window)
+  # sum over the rows of P |dO|, and the largest relative error of a probability: the scores' from their own largest size
+  size = ref.attention(q, k, v, o, o, grad=go.abs(), **window)["dv"]
+  e_s = dim ** 0.5 * 2.0 ** -24 * max(float((q[a:b, h].double().abs() @ k[a:b, h * kvh // heads].double().abs().t()).max())
+                                      for a, b in ref.spans(o) for h in range(heads))
+  rel = 2 * e_s + 2.0 ** -19 * (1 + float(want["lse"].abs().max())) + 2.0 ** -17
+  assert rel < 2.0 ** -11                    # (far below a rounding to bf16)
+  o = offs(lengths + [0] * empty).cuda()
+  q, k, v, go = (t.cuda() for t in (q, k, v, go))
+  out, lse = oc.nn.octree_attention(q, k, v, o, return_lse=True, **window)
+  dv = oc.nn.octree_attention_grad(go, q, k, v, out, lse, o, **window)[2]
+  within(dv, want["dv"], size * rel + ref.half_step(BF16) * want["dv"].abs(), "dv")
