@@ -637,7 +637,7 @@ int ocnn_octree_update_copy(void* out_dev, const void* in_dev, void* info, const
  * dim] or [rows, channels].  `offsets` (device, int32 [n_seq + 1], offsets[0] = 0, not decreasing)
  * says where each sequence begins; rows behind the last sequence belong to none: they are left as
  * they are, or set to zero with fill_rest != 0 (gradients: always zero).  Offsets are clamped to the
- * rows that exist.  These calls launch kernels only and can be captured in a HIP graph.
+ * rows that exist.  At most 65535 sequences.  These calls launch kernels only and can be captured in a HIP graph.
  *
  * ocnn_octree_offsets: those offsets (batch_size + 1) for the nodes (nempty: the non-empty nodes) of a
  * level, from its keys. */
@@ -650,7 +650,7 @@ int ocnn_octree_offsets(int* offsets, const void* octree_dev, const void* info, 
  * position[axis] * frequencies[p] (radians a unit; device, fp64 [P]), inverse != 0 by the negative: the
  * gradient.  The angle is formed in 64 bits.  positions: OCNN_POS_INT32 / OCNN_POS_F32 [rows, axes]
  * with rows `position_row` elements apart, at most 4 axes; OCNN_POS_XYZ: the packed coordinates of the
- * nodes (64-bit, 16 bits an axis, at most 3 axes), what octree_property "xyz" returns.
+ * nodes (64-bit, 16 bits an axis, at most 3 axes), what octree_property "xyz" returns.  At most 1024 heads of 1024 channels.
  * `out` may be `data` with the same strides; otherwise they must not overlap. */
 enum { OCNN_POS_INT32 = 0, OCNN_POS_F32 = 1, OCNN_POS_XYZ = 2 };
 int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void* data, int64_t row, int64_t head,

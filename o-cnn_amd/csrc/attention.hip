@@ -332,7 +332,8 @@ __device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 3"); }
 // Bits 0 .. n - 1
 __device__ inline uint32_t first_bits(int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; }
 // x where the lane's bit of accumulator row r is set, `other` (as bits) elsewhere; `bits` has been moved right by 4 in the
-// upper half of the wavefront.  Two integer instructions, and a NaN in x does not come through.
+// upper half of the wavefront.  A bit test and a select (the compiler
+// makes an and, a compare and a select of it, and waits between the last two); a NaN in x does not come through.
 __device__ inline float where_seen(uint32_t bits, int r, float x, uint32_t other) {
   const int n = 8 * (r >> 2) + (r & 3);
   const uint32_t keep = (uint32_t)(((int32_t)(bits << (31 - n))) >> 31);
@@ -469,9 +470,11 @@ __device__ inline int window_hi(const ocnn_attention_params& p, int pos, int key
 // four.  QW = 2: 64 packed rows, and each half of a tile has a wavefront of its own for them; joined at the end.  QW = 1 (few rows a sequence): 32 packed rows, and the wavefronts take every fourth tile of 32
 // keys each on their own, joined at the end.  Where rows x key heads leave compute units empty, the
 // tiles are dealt out over `splits` workgroups, joined by attention_join_kernel.
-// Measured: 4 sequences of about 16384 rows, window 2047, 8 heads of 64, bf16: 168-177 us (700 TFLOP/s), bound by VALU work
-// (60 % of the SIMD cycles: a 32 x 32 tile is 16 exponentials, shifts and sums a lane against 256 cycles of products); one query
-// of 262147 keys, 16 heads over 2 of 128, bf16: 48 us, 5.6 TB/s of keys and values, and 6 us for the join.
+// Measured: sequences of 8192 and 22184 rows, window 2047, 8 heads of 64, bf16: 168-172 us in a run of some hundred calls
+// (700 TFLOP/s), 175-205 in the first ones after a pause, when the chip's clock is lower.  A 32 x 32 tile is 16 each of
+// exponentials, multiply-adds and additions and 8 conversions a lane, about 420 cycles, against 256 of products: 61 % and 37 % of
+// the SIMD cycles, but only 18 % both at once, so the two take turns.  One query of 262147 keys, 16 heads over 2 of 128, bf16:
+// 45 us, 5.9 TB/s of keys and values, and 6 us for the join.
 template <typename E, int DP, int QW> struct ForwardShape {
   static constexpr int kKeys = QW == 1 ? 32 : 64;
   static constexpr int kTile = kKeys * Shape<E, DP>::kPitch * Shape<E, DP>::kPlanes;
@@ -943,7 +946,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnArgs a) {
 // Rows as in the forward kernel (QW = 4); the scores are computed again from lse.  rowsum(dO o) is formed
 // here, from the row's own registers, and left for the kernel of the keys.  No atomics: dQ and dK, dV each
 // have a kernel that owns their rows, at the price of computing the scores twice.
-// Measured: 16 x about 1500 rows, window 512, 8 heads over 4 of 64, bf16: 79 us (VALU 53 %, products 32 % of the SIMD cycles).
+// Measured: 16 x about 1500 rows, window 512, 8 heads over 4 of 64, bf16: 72 us (VALU 47 %, products 31 % of the SIMD cycles).
 template <typename T, int DP>
 __device__ __forceinline__ void grad_q_row_again(const AttnArgs& a, const Seq& s, int kv, int row, int t0, int t1, int sink_tiles,
     float lse2, float delta, float (&dq)[(DP + 63) / 64]) {
@@ -1220,8 +1223,8 @@ __global__ void __launch_bounds__(256, grad_q_waves<E>(DP)) attention_grad_q_ker
 // their tile ("far") are dealt out in items of kFarRows tokens to workgroups of their own, in which all four
 // wavefronts hold the same 32 sinks and share the rows (with a wavefront for every 32 keys, three of them had
 // nothing to do).  Their sums go to memory in 32 bits and are added in order by attention_sink_kernel.
-// Measured: 16 x about 1500 rows, window 512, 4 sinks, 8 heads over 4 of 64, bf16: 114 us and 5 us for the sinks (products 28 %,
-// VALU 36 %: two wavefronts a SIMD, one and a half loads of the chip).
+// Measured: 16 x about 1500 rows, window 512, 4 sinks, 8 heads over 4 of 64, bf16: 117 us and 5 us for the sinks (products 30 %,
+// VALU 33 %: two wavefronts a SIMD, one and a half loads of the chip).
 struct FarRange { int first; bool any; };        // tokens [first, queries) see the sinks only
 __device__ inline FarRange far_tokens(const AttnArgs& a, const Seq& s) {
   const ocnn_attention_params& p = a.p;

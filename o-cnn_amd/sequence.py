@@ -8,8 +8,9 @@ Tensors are row-major, a row a node: [rows, heads, dim] or [rows, channels] (row
 without its last one, or slices of one projection's output).  Tensors whose innermost axis is not
 contiguous, or whose rows do not begin at the multiples of 16 bytes that attention reads, are copied.
 All tensors of a call live on one GPU, which need not be the current one; work is queued on that GPU's
-current stream.  The forward and the gradient functions here launch kernels only and can be captured in
-a HIP graph; workspaces are allocated per call, so captured graphs share none.
+current stream.  A call takes at most 65535 sequences, and at most 2^31 - 1 entries on an axis.  The
+forward and the gradient functions here launch kernels only and can be captured in a HIP graph; workspaces
+are allocated per call, so captured graphs share none.
 """
 import ctypes as C
 import math
