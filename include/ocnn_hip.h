@@ -664,6 +664,8 @@ int ocnn_octree_rotary(void* out, int64_t out_row, int64_t out_head, const void*
  * [n_seq, channels] = the state behind the last step (of an empty sequence: the state it began with).
  * States are fp32.  carries: [carry_rows, channels] fp32 as ocnn_recurrence_shape says, kept for the
  * gradient; NULL where none is wanted (ocnn_recurrence_shape with carries = 0).  `out` may be neither `gate` nor `data`.
+ * `last` may be `state` itself (a step in place), and grad_state grad_last, where the call needs no workspace; they may not
+ * overlap otherwise.
  * The gradient takes that of `out` and of `last` (grad_last, may be NULL) and writes those of gate, data
  * and state (grad_state, may be NULL).  Results do not change from run to run. */
 int ocnn_recurrence_shape(int rows, int channels, int n_seq, int carries, int64_t* carry_rows, size_t* workspace_bytes,
@@ -689,7 +691,7 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
  *   scale: any sign; scale x log2(e) is finite in 32 bits;
  *   dim: a multiple of 8 up to 128; sinks <= 64; rows_q x heads and rows_k: at most 2^30 - 1024; every row and head begins at a multiple of 16 bytes, less than
  *     2^22 elements from the one before.
- * The gradient takes out and lse of the forward call; key rows that are no keys get zeros.  Scores, statistics
+ * Outputs may not overlap inputs.  The gradient takes out and lse of the forward call; key rows that are no keys get zeros.  Scores, statistics
  * and sums are fp32; of bf16 calls, probabilities are rounded to bf16 once as operands of the second product of
  * the forward call where sequences have many rows, and to two bf16 elsewhere, as are score gradients.  Results do not change from run to run.  Both calls need ocnn_attention_workspace_bytes bytes
  * (16-byte aligned; the first may need none). */

@@ -956,6 +956,13 @@ bool scan_blocks(int64_t rows, int64_t channels, int64_t n_seq, bool back) {
 }
 bool scan_narrow(int64_t channels, int64_t n_seq) { return n_seq * channels <= 512; }
 
+// A state written where one is read: a workgroup that takes a sequence from one end to the other has read it by then; chunks of
+// their own have not.
+bool states_apart(const float* out, const float* in, int n_seq, int channels, bool itself) {
+  const uintptr_t a = (uintptr_t)out, b = (uintptr_t)in, size = (uintptr_t)n_seq * channels * sizeof(float);
+  return !out || !in || (itself && a == b) || a + size <= b || b + size <= a;
+}
+
 int64_t scan_ids(int64_t rows, int n_seq, int shift) { return (rows >> shift) + n_seq + 1; }
 
 // the lists of runs in a workspace
@@ -1126,6 +1133,7 @@ int ocnn_octree_recurrence(void* out, int64_t out_row, float* last, float* carri
   if (rc) return rc;
   OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
   OCNN_REQUIRE(offsets && (rows == 0 || (out && gate && data)), OCNN_E_BADARG, "null pointer");
+  OCNN_REQUIRE(states_apart(last, state, n_seq, channels, need == 0), OCNN_E_BADARG, "last overlaps state");
   ScanArgs a = {};
   a.out = out; a.gate = gate; a.data = data; a.out_row = out_row; a.gate_row = gate_row; a.data_row = data_row;
   a.state = state; a.last = last; a.offsets = offsets;
@@ -1187,6 +1195,8 @@ int ocnn_octree_recurrence_grad(void* grad_gate, int64_t grad_gate_row, void* gr
   OCNN_REQUIRE(dtype == OCNN_F32 || dtype == OCNN_BF16, OCNN_E_BADARG, "dtype %d", dtype);
   OCNN_REQUIRE(offsets && carries && (rows == 0 || (grad_gate && grad_data && grad_out && gate && data)), OCNN_E_BADARG,
       "null pointer");
+  OCNN_REQUIRE(states_apart(grad_state, grad_last, n_seq, channels, need == 0) && states_apart(grad_state, state, n_seq, channels, false),
+      OCNN_E_BADARG, "grad_state overlaps a state");
   ScanArgs a = {};
   a.gate = gate; a.data = data; a.grad = grad_out; a.grad_gate = grad_gate; a.grad_data = grad_data;
   a.gate_row = gate_row; a.data_row = data_row; a.grad_row = grad_out_row; a.grad_gate_row = grad_gate_row;

@@ -103,3 +103,48 @@ def test_scales_beyond_32_bits_are_refused_on_a_gpu(oc):
     with pytest.raises(oc.nn.OcnnError, match="scale"):
       oc.nn.octree_attention(x, x, x, o, scale=scale)
   assert bool((oc.nn.octree_attention(x, x, x, o, scale=2e38) == 0).all())
+
+
+# ---- states in place ------------------------------------------------------------------------------------------
+def recurrence_entry(pkg, rows, channels, n_seq, state, last, ws=(None, 0), tensors=(16, 16, 16, 16), dtype=0):
+  """the C entry point with addresses: out, gate, data, offsets"""
+  i64, p = C.c_int64, C.c_void_p
+  out, gate, data, offsets = (p(t) for t in tensors)
+  return pkg.lib.get().ocnn_octree_recurrence(out, i64(channels), p(last), None, gate, i64(channels), data, i64(channels), p(state),
+                                              offsets, n_seq, rows, channels, 0, 0, dtype, p(ws[0]), C.c_size_t(ws[1]), None)
+
+
+def test_states_that_overlap_are_refused(pkg):
+  """chunks of a sequence read the state after others may have written the last one"""
+  L, i64, p = pkg.lib.get(), C.c_int64, C.c_void_p
+  base = 1 << 20
+  for last in (base, base + 4, base + 4 * 8 - 4, base - 4):
+    assert recurrence_entry(pkg, 5000, 8, 1, base, last, (4096, 1 << 30)) == -1
+    assert b"overlaps" in L.ocnn_last_error()
+  for last in (base + 4, base - 4):           # (a step: the state itself only)
+    assert recurrence_entry(pkg, 4, 8, 4, base, last) == -1 and b"overlaps" in L.ocnn_last_error()
+
+  def grad(rows, state, grad_last, grad_state):
+    a = p(4096)
+    return L.ocnn_octree_recurrence_grad(a, i64(8), a, i64(8), p(grad_state), a, i64(8), p(grad_last), a, i64(8), a, i64(8),
+                                         p(state), a, a, 1, rows, 8, 0, 0, a, C.c_size_t(1 << 30), None)
+  assert grad(5000, None, base, base) == -1 and b"overlaps" in L.ocnn_last_error()
+  assert grad(5000, base, None, base + 4) == -1 and b"overlaps" in L.ocnn_last_error()
+  assert grad(20, base, None, base) == -1 and b"overlaps" in L.ocnn_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[1] * 9, [1] * 80 + [400], [300, 0, 200]], ids=["walked", "walked-and-long", "a-workgroup-each"])
+def test_a_step_in_place(oc, lengths):
+  """the last state written over the one it began with"""
+  g = torch.Generator().manual_seed(1)
+  n, c = sum(lengths), 20
+  gate, data, state = (torch.randn(r, c, generator=g).cuda() for r in (n, n, len(lengths)))
+  o = offs(0, *torch.tensor(lengths).cumsum(0).tolist()).cuda()
+  want, last = oc.nn.octree_recurrence(gate, data, o, state)
+  out = torch.empty_like(want)
+  torch.cuda.synchronize()
+  assert recurrence_entry(oc, n, c, len(lengths), state.data_ptr(), state.data_ptr(),
+                          tensors=[t.data_ptr() for t in (out, gate, data, o)]) == 0
+  torch.cuda.synchronize()
+  assert torch.equal(out, want) and torch.equal(state, last)
